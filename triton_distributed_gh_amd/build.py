@@ -38,6 +38,9 @@ HIP_LIB = ROOT / "libtdist_hip.so"
 HIP_SAFE_LIB = ROOT / "libtdist_hip_safe.so"
 HOST_LIB = ROOT / "libtdist_host.so"
 
+# no packed fp32 instructions: some of their forms have given wrong results on this hardware now and then (hipcc's
+# host pass does not know the feature and warns about it)
+NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 HIPCC_FLAGS = [
     f"--offload-arch={ARCH}",
     "-O3",
@@ -47,6 +50,7 @@ HIPCC_FLAGS = [
     "-fno-gpu-sanitize",
     "-Wno-unused-result",
     "-Wno-pass-failed",
+    *NO_PACKED_FP32,
     f"-I{CSRC / 'include'}",
     "-D__HIP_PLATFORM_AMD__",
 ]

@@ -34,6 +34,7 @@ from pathlib import Path
 from typing import Any, Callable, Dict, List, Optional
 
 from .. import _lib
+from ..build import NO_PACKED_FP32
 
 _SCALARS = {"i1", "i8", "i16", "i32", "i64", "u8", "u16", "u32", "u64", "fp16", "bf16", "fp32", "fp64"}
 _POINTEES = _SCALARS | {"fp8e4nv", "fp8e5", "fp8e4b15", "void"}
@@ -301,7 +302,7 @@ def compile_kernel(path: str, kernel: str, workspace: Path, arch: str = "gfx950"
     """One ``.hip`` kernel source -> code object ``<workspace>/<stem>.hsaco``; returns its manifest entry."""
     co = Path(workspace) / f"{Path(path).stem}.hsaco"
     if build:
-        cmd = ["hipcc", "--genco", f"--offload-arch={arch}", "-O3", "-std=c++17",
+        cmd = ["hipcc", "--genco", f"--offload-arch={arch}", "-O3", "-std=c++17", *NO_PACKED_FP32,
                f"-I{Path(__file__).resolve().parent.parent / 'csrc' / 'include'}", path, "-o", str(co)]
         subprocess.run(cmd, check=True)
     return {"source": path, "kernel": kernel, "hsaco": str(co)}

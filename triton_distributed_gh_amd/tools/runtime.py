@@ -33,6 +33,7 @@ from pathlib import Path
 from typing import Dict, List, Optional, Sequence, Tuple, Union
 
 from .. import _lib
+from ..build import NO_PACKED_FP32
 
 INCLUDE_DIR = Path(__file__).resolve().parent.parent / "csrc" / "include"
 
@@ -82,7 +83,8 @@ def compile_hip(source: Union[str, Path], out: Union[str, Path, None] = None, ar
     src = Path(source).resolve()
     libs = [Path(p).resolve() for p in extern_libs]
     out = Path(out) if out is not None else src.with_suffix(".hsaco")
-    common = [f"--offload-arch={arch}", "-O3", "-std=c++17", "-fno-gpu-sanitize", f"-I{INCLUDE_DIR}", *extra_flags]
+    common = [f"--offload-arch={arch}", "-O3", "-std=c++17", "-fno-gpu-sanitize", *NO_PACKED_FP32, f"-I{INCLUDE_DIR}",
+              *extra_flags]
     flags = (["--genco"] if not libs else ["-fgpu-rdc", "--cuda-device-only", "-c"]) + common
     h = hashlib.sha1(" ".join(flags).encode())
     for f in [src, *libs]:
