@@ -1,0 +1,366 @@
+"""4-bit KV cache kernels: the bits of the CPU path, and attention against its definition in 64 bits."""
+import math
+
+import pytest
+import torch
+
+import kv4_oracle as oracle
+from kv4_oracle import int32
+from triton_distributed_gh_amd.ops import flash_decode, kv4
+
+pytestmark = pytest.mark.gpu
+
+FORMS = [(64, 32), (64, 64), (128, 32), (128, 64), (128, 128), (256, 32), (256, 64), (256, 128)]
+DTYPES = [torch.bfloat16, torch.float16]
+
+
+def _gen(seed=0):
+    return torch.Generator().manual_seed(seed)
+
+
+def _to(cache, device):
+    return kv4.Int4KVCache(*(t.to(device) for t in (cache.k_codes, cache.v_codes, cache.k_params, cache.v_params)))
+
+
+def _same(a, b):
+    """The same bits, but for the low of a group that holds a NaN or an infinity (its scale is NaN on both sides)."""
+    assert torch.equal(a.k_codes.cpu(), b.k_codes.cpu()) and torch.equal(a.v_codes.cpu(), b.v_codes.cpu())
+    for x, y in ((a.k_params.cpu(), b.k_params.cpu()), (a.v_params.cpu(), b.v_params.cpu())):
+        bad = x[..., 0].isnan()
+        assert torch.equal(bad, y[..., 0].isnan())
+        assert torch.equal(x[~bad], y[~bad])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D,group", FORMS)
+def test_append_and_read_give_the_bits_of_the_cpu_path(D, group, dtype):
+    gen = _gen(D + group)
+    B, S, H, page = 3, 45, 3, 48
+    table, pages = oracle.table_for(B, 100, page, gen)
+    cpu = kv4.Int4KVCache.alloc(pages, page, H, D, group=group, dtype=dtype)
+    gpu = _to(cpu, "cuda")
+    k, v = oracle.rows(gen, B, S, H, D, dtype=dtype), oracle.rows(gen, B, S, H, D, dtype=dtype)
+    k[0, 3, 1, 5], v[1, 2, 0, 7], v[2, 1, 2, D - 1] = math.nan, math.inf, -math.inf
+    k[2, 4], v[2, 4] = 1.5, 0.0                             # no range
+    k[1, 0, 0, ::2], k[1, 0, 0, 1::2] = torch.finfo(dtype).max, -torch.finfo(dtype).max
+    v[1, 1] *= 2.0 ** -20 if dtype == torch.float16 else 2.0 ** -124       # scales at the bottom of the type
+    offsets, news = int32([0, 31, 97]), int32([45, 13, 45])                # in order; in the middle; over the end
+    kv4.kv4_append(k, v, cpu, offsets, table, new_lens=news)
+    kv4.kv4_append(k.cuda(), v.cuda(), gpu, offsets.cuda(), table.cuda(), new_lens=news.cuda())
+    torch.cuda.synchronize()
+    _same(cpu, gpu)
+    cu, starts = int32([2, 60, 60, 110]), int32([0, 5, 60])
+    outs = []
+    for c, dev in ((cpu, "cpu"), (gpu, "cuda")):
+        out = tuple(torch.full((115, H, D), 7.0, dtype=dtype, device=dev) for _ in range(2))
+        outs.append(kv4.kv4_read(c, table.to(dev), cu.to(dev), 115, starts=starts.to(dev), out=out))
+    torch.cuda.synchronize()
+    for a, b in zip(*outs):
+        b = b.cpu()
+        assert (b[:2] == 7).all() and (b[110:] == 7).all()
+        assert torch.equal(a.isnan(), b.isnan()) and torch.equal(a.nan_to_num(0.0), b.nan_to_num(0.0))
+
+
+@pytest.mark.parametrize("S", [1, 2, 3, 4, 5, 17, 64])
+def test_append_token_counts_and_strided_rows(S):
+    gen = _gen(S)
+    B, H, D, group, page = 2, 5, 128, 64, 16
+    table, pages = oracle.table_for(B, 96, page, gen)
+    cpu = kv4.Int4KVCache.alloc(pages, page, H, D, group=group)
+    gpu = _to(cpu, "cuda")
+    qkv = oracle.rows(gen, B, S, 3 * H, D)                  # K and V as parts of one projection's rows
+    odd = oracle.rows(gen, B, S, H, D + 4)                  # rows that are not 16-byte aligned: copied by the call
+    offsets = int32([7, 30])
+    for k, v in ((qkv[:, :, H:2 * H], qkv[:, :, 2 * H:]), (odd[..., 4:], odd[..., :D]),
+                 (qkv[:, :, :H].transpose(0, 1).contiguous().transpose(0, 1), qkv[:, :, H:2 * H])):
+        dk, dv = (x.to("cuda") for x in (qkv, odd))
+        strided = {qkv.data_ptr(): dk, odd.data_ptr(): dv}
+
+        def there(x):
+            base = strided.get(x.untyped_storage().data_ptr())
+            return x.cuda() if base is None else torch.as_strided(base, x.shape, x.stride(), x.storage_offset())
+
+        kv4.kv4_append(k, v, cpu, offsets, table)
+        kv4.kv4_append(there(k), there(v), gpu, offsets.cuda(), table.cuda())
+        torch.cuda.synchronize()
+        _same(cpu, gpu)
+
+
+def test_append_leaves_everything_else_alone():
+    """Bytes around the written tokens, and pages of other sequences, keep their bits."""
+    gen = _gen(11)
+    H, D, group, page = 2, 128, 128, 16
+    cache, table, _, _ = oracle.filled(gen, [60, 60], H, D, group, page, device="cuda")
+    table = table.clone()
+    before = [t.clone() for t in (cache.k_codes, cache.v_codes, cache.k_params, cache.v_params)]
+    bad = table.clone()
+    bad[0, 1], bad[0, 2] = -5, cache.num_pages              # tokens 16 .. 47 of the first sequence go nowhere
+    k = oracle.rows(gen, 2, 40, H, D, device="cuda")
+    kv4.kv4_append(k, k, cache, int32([14, 100], "cuda"), bad)      # the second sequence is behind its table
+    torch.cuda.synchronize()
+    touched = torch.zeros(cache.num_pages, page, dtype=torch.bool)
+    touched[int(table[0, 0]), 14:] = True
+    touched[int(table[0, 3]), :6] = True
+    touched = touched.cuda()
+    now = (cache.k_codes, kv4._v_units(cache), cache.k_params, cache.v_params)
+    was = (before[0], kv4._v_units(kv4.Int4KVCache(*before)), before[2], before[3])
+    for i, (a, b) in enumerate(zip(was, now)):
+        if i == 1:                                          # [pages, H, quads, 16, halves, 4, 2] -> tokens in front
+            a, b = (x.permute(0, 2, 5, 1, 3, 4, 6).flatten(1, 2).flatten(2) for x in (a, b))
+        elif i == 0:
+            a, b = (x.transpose(1, 2).flatten(2) for x in (a, b))
+        else:
+            a, b = (x.permute(0, 3, 1, 2, 4).flatten(2) for x in (a, b))
+        assert torch.equal(a[~touched], b[~touched])
+        assert not torch.equal(a[touched], b[touched])
+
+
+@pytest.mark.parametrize("D,group", [(64, 32), (128, 64), (128, 128), (256, 32)])
+@pytest.mark.parametrize("B,S,norm", [(3, 1, True), (2, 7, True), (1, 150, False)])
+def test_projection_gives_the_bits_of_the_cpu_path(D, group, B, S, norm):
+    gen = _gen(D + S)
+    Hq, H, page = 6, 2, 32
+    table, pages = oracle.table_for(B, 192, page, gen)
+    cpu = kv4.Int4KVCache.alloc(pages, page, H, D, group=group)
+    gpu = _to(cpu, "cuda")
+    wide = oracle.rows(gen, B, S, (Hq + 2 * H) * D + 8)
+    qw, kw = ((1 + 0.1 * torch.randn(2, D, generator=gen)).bfloat16().unbind(0)) if norm else (None, None)
+    ang = torch.outer(torch.arange(160.0), 1e4 ** (-torch.arange(0, D, 2) / D))
+    cos, sin = ang.cos().contiguous(), ang.sin().contiguous()
+    offset = int32([0, 30, 41][:B])
+    pos = offset[:, None].long() + torch.arange(S)
+    pos[0, 0] = 10 ** 9                                     # behind the tables: their last row
+    args = (1e-6, 1e-5, pos, cos, sin)
+    total = torch.zeros(B, dtype=torch.int32)
+    qc = kv4.kv4_qkv_prep(wide[..., :-8], qw, kw, *args, cpu, offset, total, table, Hq)
+    dev = [x.cuda() if isinstance(x, torch.Tensor) else x for x in args]
+    total_g = torch.zeros(B, dtype=torch.int32, device="cuda")
+    qg = kv4.kv4_qkv_prep(wide.cuda()[..., :-8], *(w if w is None else w.cuda() for w in (qw, kw)), *dev, gpu, offset.cuda(), total_g,
+                          table.cuda(), Hq)
+    torch.cuda.synchronize()
+    assert torch.equal(total, total_g.cpu()) and total.tolist() == (offset + S).tolist()
+    assert torch.equal(qc, qg.cpu())
+    _same(cpu, gpu)
+
+
+def _check(got, want, lse_got, lse, dtype, v_max):
+    assert torch.equal(got.isnan().cpu(), want.isnan())
+    assert ((got.double().cpu() - want).abs() <= oracle.bounds(want, dtype, v_max)).all(), (got.double().cpu() - want).abs().max()
+    if lse_got is not None:
+        assert torch.equal(lse_got.cpu() == -math.inf, lse == -math.inf)
+        fine = lse != -math.inf
+        assert (lse_got.double().cpu() - lse)[fine].abs().max() <= 1e-3
+
+
+ATTEND = [
+    # lens, S, Hq, Hkv, D, group, page, splits
+    ([37, 0, 1, 2, 33], 1, 8, 2, 128, 64, 16, -1),
+    ([300, 129], 1, 40, 8, 64, 32, 16, 3),                  # five heads to a KV head
+    ([1000], 1, 32, 2, 128, 128, 64, 4),                    # sixteen
+    ([700, 31, 512], 1, 18, 1, 128, 32, 48, 2),             # eighteen: a second column block, ragged
+    ([513, 64, 5], 5, 8, 2, 256, 64, 32, 3),                # several tokens; a sequence shorter than them is no sequence, 5 is
+    ([260], 1, 4, 4, 256, 128, 16, -1),                     # no sharing
+    ([95, 200], 7, 12, 4, 256, 32, 16, 1),
+    ([1025], 9, 4, 2, 64, 64, 1040, 5),                     # one page of odd size for the sequence
+    ([15, 16, 17], 17, 4, 2, 128, 64, 16, 1),               # more queries than tokens: the first rows see nothing
+    ([4096], 1, 8, 1, 128, 64, 64, 32),
+    ([100] * 20, 1, 4, 1, 64, 32, 16, -1),
+]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lens,S,Hq,H,D,group,page,splits", ATTEND)
+def test_attention_against_the_definition(lens, S, Hq, H, D, group, page, splits, dtype):
+    gen = _gen(sum(lens) + S)
+    cache, table, ks, vs = oracle.filled(gen, lens, H, D, group, page, dtype, "cuda", room=max(lens) + 40)
+    q = oracle.rows(gen, len(lens), S, Hq, D, dtype=dtype, device="cuda")
+    keys, values = [oracle.held(x, group) for x in ks], [oracle.held(x, group) for x in vs]
+    v_max = max(float(x.abs().max()) if x.numel() else 0.0 for x in values)
+    n = int32(lens, "cuda")
+    for causal in (True, False) if S > 1 else (True,):
+        want, lse = oracle.attention(q, keys, values, D ** -0.5, causal=causal)
+        out = kv4.gqa_fwd_kv4(q, cache, n, table, kv_split=splits, causal=causal)
+        full = kv4.gqa_fwd_kv4(q, cache, n, table, kv_split=splits, causal=causal, return_lse=True)
+        torch.cuda.synchronize()
+        assert out.dtype == dtype and full.dtype == torch.float32
+        _check(out, want, None, None, dtype, v_max)
+        _check(full[..., :D], want, full[..., D], lse, torch.float32, v_max)
+        again = kv4.gqa_fwd_kv4(q, cache, n, table, kv_split=splits, causal=causal)
+        assert torch.equal(out, again)
+    if S == 1:
+        assert torch.equal(kv4.gqa_fwd_kv4(q[:, 0], cache, n, table, kv_split=splits), out[:, 0])
+
+
+@pytest.mark.parametrize("soft_cap", [0.0, 15.0])
+def test_large_scores_and_peaked_rows(soft_cap):
+    """Scores far apart (the running maximum moves in every block) and one token that takes nearly all the weight."""
+    gen = _gen(21)
+    H, Hq, D, group, page, L = 2, 8, 128, 64, 16, 900
+    cache, table, ks, vs = oracle.filled(gen, [L], H, D, group, page, torch.bfloat16, "cuda")
+    q = oracle.rows(gen, 1, 1, Hq, D, device="cuda") * 2
+    order = torch.argsort((ks[0][:, 0].float() @ q[0, 0, 0].float()))       # ascending scores for the first head
+    k, v = ks[0][order][None].contiguous(), vs[0][order][None].contiguous()
+    kv4.kv4_append(k, v, cache, int32([0], "cuda"), table)
+    keys, values = [oracle.held(k[0], group)], [oracle.held(v[0], group)]
+    for splits in (1, 4):
+        want, lse = oracle.attention(q, keys, values, 0.5, soft_cap)
+        got = kv4.gqa_fwd_kv4(q, cache, int32([L], "cuda"), table, scale=0.5, soft_cap=soft_cap, kv_split=splits)
+        torch.cuda.synchronize()
+        # the bound is for scores of a nat's 2e-4: a scale of 0.5 instead of 128^-0.5 is 5.7 times that, q twice as wide 2 more
+        half = torch.finfo(torch.bfloat16).eps / 2
+        tol = half * want.abs() + 12 * 2.0 ** -11 * float(values[0].abs().max())
+        assert ((got.double().cpu() - want).abs() <= tol).all()
+
+
+def test_garbage_outside_of_the_sequences_is_not_read_into_the_result():
+    gen = _gen(22)
+    lens, H, D, group, page = [21, 50], 2, 128, 32, 16
+    cache, table, ks, vs = oracle.filled(gen, lens, H, D, group, page, torch.bfloat16, "cuda", room=96)
+    q = oracle.rows(gen, 2, 2, 4, D, device="cuda")
+    n = int32(lens, "cuda")
+    clean = kv4.gqa_fwd_kv4(q, cache, n, table, kv_split=2)
+    there = torch.zeros(cache.num_pages, page, dtype=torch.bool, device="cuda")
+    for b, L in enumerate(lens):
+        for t in range(L):
+            there[table[b, t // page].long(), t % page] = True
+    for p in (cache.k_params, cache.v_params):              # every token that is in no sequence: NaN and infinity
+        x = p.permute(0, 3, 1, 2, 4)
+        x[~there] = torch.tensor([math.nan, math.inf], dtype=p.dtype, device="cuda")
+    cache.k_codes.transpose(1, 2)[~there] = 255
+    far = table.clone()
+    far[0, 2:], far[1, 4:] = -1, 10 ** 6                    # and no pages behind the lengths
+    dirty = kv4.gqa_fwd_kv4(q, cache, n, far, kv_split=2)
+    torch.cuda.synchronize()
+    assert torch.equal(clean, dirty)
+
+
+def test_masked_nan_reaches_the_query_that_sees_it_alone():
+    gen = _gen(23)
+    H, D, group, page = 1, 128, 64, 16
+    for splits in (1, 2):
+        cache, table, _, _ = oracle.filled(gen, [300], H, D, group, page, torch.bfloat16, "cuda")
+        k = torch.full((1, 1, H, D), math.nan, dtype=torch.bfloat16, device="cuda")
+        kv4.kv4_append(k, k, cache, int32([299], "cuda"), table)
+        out = kv4.gqa_fwd_kv4(oracle.rows(gen, 1, 3, 2, D, device="cuda"), cache, int32([300], "cuda"), table, kv_split=splits)
+        torch.cuda.synchronize()
+        assert out[0, :2].isfinite().all() and out[0, 2].isnan().all()
+
+
+def test_bad_pages_inside_a_sequence():
+    gen = _gen(24)
+    H, Hq, D, group, page = 2, 4, 64, 32, 16
+    cache, table, ks, vs = oracle.filled(gen, [90], H, D, group, page, torch.float16, "cuda")
+    bad = table.clone()
+    bad[0, 1], bad[0, 4] = -1, cache.num_pages
+    there = torch.ones(90, dtype=torch.bool)
+    there[16:32] = there[64:80] = False
+    q = oracle.rows(gen, 1, 3, Hq, D, dtype=torch.float16, device="cuda")
+    values = [oracle.held(vs[0], group)]
+    want, lse = oracle.attention(q, [oracle.held(ks[0], group)], values, D ** -0.5, there=[there])
+    got = kv4.gqa_fwd_kv4(q, cache, int32([90], "cuda"), bad, return_lse=True, kv_split=1)
+    torch.cuda.synchronize()
+    _check(got[..., :D], want, got[..., D], lse, torch.float32, float(values[0].abs().max()))
+    over = kv4.gqa_fwd_kv4(q, cache, int32([10 ** 6], "cuda"), table)       # a length beyond the table is the table's
+    assert torch.equal(over, kv4.gqa_fwd_kv4(q, cache, int32([96], "cuda"), table))
+
+
+def test_parts_of_a_sequence_on_two_ranks_merge():
+    gen = _gen(25)
+    lens, H, Hq, D, group, page = [[200, 64], [77, 0]], 2, 8, 128, 64, 16
+    q = oracle.rows(gen, 2, Hq, D, device="cuda")
+    parts, ks, vs = [], [], []
+    for n in lens:
+        cache, table, k, v = oracle.filled(gen, n, H, D, group, page, torch.bfloat16, "cuda")
+        parts.append(kv4.gqa_fwd_kv4(q, cache, int32(n, "cuda"), table, return_lse=True))
+        ks.append(k), vs.append(v)
+    out = flash_decode.gqa_fwd_batch_decode_inter_rank_combine(torch.stack(parts), int32(lens, "cuda"))
+    whole = [torch.cat([oracle.held(x[b], group) for x in y]) for y in (ks, vs) for b in range(2)]
+    want, _ = oracle.attention(q[:, None], whole[:2], whole[2:], D ** -0.5)
+    torch.cuda.synchronize()
+    _check(out, want[:, 0], None, None, torch.bfloat16, max(float(x.abs().max()) for x in whole[2:]))
+
+
+def test_strided_queries_and_another_stream():
+    gen = _gen(26)
+    lens, H, Hq, D, group, page = [70, 300], 2, 8, 128, 64, 16
+    cache, table, ks, vs = oracle.filled(gen, lens, H, D, group, page, torch.bfloat16, "cuda")
+    n = int32(lens, "cuda")
+    wide = oracle.rows(gen, 2, 3, Hq + 4, D, device="cuda")
+    q = wide[:, :, 2:2 + Hq]
+    want = kv4.gqa_fwd_kv4(q.contiguous(), cache, n, table, kv_split=2)
+    assert torch.equal(kv4.gqa_fwd_kv4(q, cache, n, table, kv_split=2), want)
+    unaligned = torch.empty(2 * 3 * Hq * D + 1, dtype=torch.bfloat16, device="cuda")[1:].view(2, 3, Hq, D)
+    unaligned.copy_(q)
+    assert torch.equal(kv4.gqa_fwd_kv4(unaligned, cache, n, table, kv_split=2), want)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        outs = [kv4.gqa_fwd_kv4(q, cache, n, table, kv_split=2) for _ in range(3)]
+    here = [kv4.gqa_fwd_kv4(q, cache, n, table, kv_split=2) for _ in range(3)]
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs + here)
+
+
+def test_decode_steps_replay_from_two_graphs():
+    """append + attention as a captured step; two graphs that share the cache replay in turn and equal the eager steps."""
+    gen = _gen(27)
+    B, H, Hq, D, group, page = 2, 2, 8, 128, 64, 16
+    start = [100, 37]
+    cache, table, _, _ = oracle.filled(gen, start, H, D, group, page, torch.bfloat16, "cuda", room=128)
+    twin = kv4.Int4KVCache(*(t.clone() for t in (cache.k_codes, cache.v_codes, cache.k_params, cache.v_params)))
+    steps = 6
+    k, v = (oracle.rows(gen, steps, B, 1, H, D, device="cuda") for _ in range(2))
+    q = oracle.rows(gen, steps, B, 1, Hq, D, device="cuda")
+    bufs = [k[0].clone(), v[0].clone(), q[0].clone()]
+    offset, total = int32(start, "cuda"), int32(start, "cuda")
+
+    def step(c, kk, vv, qq, splits):
+        kv4.kv4_append(kk, vv, c, offset, table)
+        torch.add(offset, 1, out=total)
+        return kv4.gqa_fwd_kv4(qq, c, total, table, kv_split=splits)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graphs = []
+    with torch.cuda.stream(side):
+        step(cache, *bufs, 2)
+        for splits in (1, 3):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=side):
+                out = step(cache, *bufs, splits)
+            graphs.append((g, out, splits))
+    torch.cuda.current_stream().wait_stream(side)
+    for i in range(steps):
+        g, out, splits = graphs[i % 2]
+        for b, x in zip(bufs, (k[i], v[i], q[i])):
+            b.copy_(x)
+        g.replay()
+        torch.cuda.synchronize()
+        eager = step(twin, k[i], v[i], q[i], splits)
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager)
+        offset += 1
+    _same(cache, twin)
+
+
+def test_pages_far_beyond_32_bit_offsets():
+    """Pages at the end of a cache of more than 4 GiB of codes."""
+    H, D, group, page = 8, 256, 128, 64
+    pages = (9 << 29) // (H * page * D // 2)                # 4.5 GiB of K codes
+    cache = kv4.Int4KVCache(torch.empty(pages, H, page, D // 2, dtype=torch.uint8, device="cuda"),
+                            torch.empty(pages, H, page // 4, 2 * D, dtype=torch.uint8, device="cuda"),
+                            *(torch.empty(pages, H, D // group, page, 2, dtype=torch.bfloat16, device="cuda") for _ in range(2)))
+    gen = _gen(28)
+    table = int32([[pages - 1, 3]], "cuda")
+    k, v = oracle.rows(gen, 1, 100, H, D, device="cuda"), oracle.rows(gen, 1, 100, H, D, device="cuda")
+    kv4.kv4_append(k, v, cache, int32([0], "cuda"), table)
+    got = kv4.kv4_read(cache, table, int32([0, 100], "cuda"), 100)
+    q = oracle.rows(gen, 1, 1, H, D, device="cuda")
+    out = kv4.gqa_fwd_kv4(q, cache, int32([100], "cuda"), table)
+    torch.cuda.synchronize()
+    kh, vh = oracle.held(k[0], group), oracle.held(v[0], group)
+    for g, w in zip(got, (kh, vh)):
+        assert ((g.double().cpu() - w).abs() <= (2.0 ** -8 + 2.0 ** -23) * w.abs() + 2.0 ** -26).all()
+    want, _ = oracle.attention(q, [kh], [vh], D ** -0.5)
+    _check(out, want, None, None, torch.bfloat16, float(vh.abs().max()))

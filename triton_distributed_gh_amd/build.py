@@ -60,6 +60,8 @@ if os.environ.get("TDIST_SPIN_TIMEOUT_MS"):
 if os.environ.get("TDIST_EXTRA_HIPCC_FLAGS"):
     # e.g. -DTDIST_EXP_...=1 for an A/B build of one experiment (objects are keyed by their flags)
     HIPCC_FLAGS += os.environ["TDIST_EXTRA_HIPCC_FLAGS"].split()
+# sources that need IEEE arithmetic (a stored code depends on a quotient; infinities and NaN reach the kernels)
+SOURCE_FLAGS = {"kv4": ["-fno-fast-math"], "kv4_attn": ["-fno-fast-math"]}
 HOST_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-pthread", f"-I{CSRC / 'include'}"]
 
 
@@ -79,6 +81,7 @@ def _digest(src: Path, flags: list[str]) -> str:
 
 def _compile_one(cc: str, src: Path, flags: list[str], verbose: bool, prefix: str = "") -> Path:
     OBJ_DIR.mkdir(parents=True, exist_ok=True)
+    flags = [*flags, *SOURCE_FLAGS.get(src.stem, [])]
     obj = OBJ_DIR / f"{prefix}{src.stem}.{_digest(src, [cc] + flags)}.o"
     if obj.exists():
         return obj

@@ -21,7 +21,7 @@ from .. import build
 def device_asm(source: str) -> str:
     """gfx950 assembly of ``csrc/ops/<source>`` built with the library's own flags."""
     src = build.CSRC / "ops" / source
-    cmd = [build._hipcc(), *build.HIPCC_FLAGS, "-S", "--cuda-device-only", "-o", "-", str(src)]
+    cmd = [build._hipcc(), *build.HIPCC_FLAGS, *build.SOURCE_FLAGS.get(src.stem, []), "-S", "--cuda-device-only", "-o", "-", str(src)]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"hipcc failed on {src}:\n{res.stderr[-2000:]}")
