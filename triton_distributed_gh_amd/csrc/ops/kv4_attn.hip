@@ -16,295 +16,509 @@
 //   codes are stored, so neither side moves between lanes.
 // The running maximum is only raised (and the sums rescaled) when a score exceeds it by 2^8: P up to 256 costs nothing
 // in floating point, and the cross-lane maximum leaves the loop.
-#include "tdist/gemm_gfx950.hpp"
 #include "tdist/kv4.hpp"
 
 namespace {
 
 using namespace tdist::kv4;
-using tdist::gemm::f32x4;
-using tdist::gemm::Frag;
-typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
-typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
-
+typedef __attribute__((ext_vector_type(4))) float f32x4;
 struct AttnArgs {
   Cache c;
   const uint16_t* q;        // [batch, S, q_heads, D]
-  const int* table;         // [batch, max_pages]
-  const int* kv_len;        // [batch], the S new tokens included
   float* partial;           // splits > 1: [rows, splits, D] sums over their own weight, rows = batch * S * q_heads
   float* partial_lse;       // and [rows, splits] log2-sum-exp2 (-inf: no token)
   void* out;                // [batch, S, q_heads, D] (out_mode 1) or fp32 [.., D + 1] with the log-sum-exp (out_mode 2)
   long long q_sb, q_ss, q_sh;
   int table_stride, max_pages;
+  int page_tiles;           // 16-token tiles of a page,
+  uint32_t page_magic;      // and floor(2^32 / page_tiles) + 1 (0: one tile a page)
   int batch, S, q_heads, splits, causal, out_mode;
   float scale, soft_cap;
 };
 
-// 16 + code as 16-bit numbers: the code sits below the leading significand bit of 16.0, at bit POS
-template <bool IS_BF16>
-struct Unpack {
-  static constexpr uint32_t MAGIC = IS_BF16 ? 0x41804180u : 0x4c004c00u;
-  static constexpr int POS = IS_BF16 ? 3 : 6;
-  template <int N>        // nibbles N and N + 4 of w
-  static __device__ __forceinline__ uint32_t pair(uint32_t w) {
-    constexpr uint32_t MASK = 0x000f000fu << POS;
-    if constexpr (POS > 4 * N) {
-      return ((w << (POS - 4 * N)) & MASK) | MAGIC;
-    } else {
-      return ((w >> (4 * N - POS)) & MASK) | MAGIC;
-    }
-  }
-};
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float log2_fast(float x) { return __builtin_amdgcn_logf(x); }
+__device__ __forceinline__ f32x4 mfma(const u32x4& a, const u32x4& b, const f32x4& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
 
-template <bool IS_BF16, int D, int G>
-__global__ __launch_bounds__(256) void kv4_attn_kernel(AttnArgs a) {
-  using F = Frag<IS_BF16>;
-  using QT = typename F::T;
+// The masks and offsets of the unpacking, kept in registers (a literal each would keep the and-or from being one instruction)
+struct Unpack {
+  uint32_t m0, m1, o0, o1;
+  __device__ __forceinline__ Unpack() {
+    asm volatile("s_mov_b32 %0, 0x000f000f" : "=s"(m0));
+    asm volatile("s_mov_b32 %0, 0x00f000f0" : "=s"(m1));
+    asm volatile("v_mov_b32 %0, 0x64006400" : "=v"(o0));
+    asm volatile("v_mov_b32 %0, 0x54005400" : "=v"(o1));
+  }
+  // nibbles n and n + 4 of a dword as two fp16 numbers: 1024 + code (n even) or 64 + code (n odd).  w8 = w >> 8.
+  __device__ __forceinline__ uint32_t even(uint32_t w) const { return (w & m0) | o0; }
+  __device__ __forceinline__ uint32_t odd(uint32_t w) const { return (w & m1) | o1; }
+};
+
+// One block of 32 tokens as it comes from the cache: two tiles of sixteen.  The parameters come one dword a lane and
+// group (lanes 0 .. 31 the tokens' of K, 32 .. 63 of V) and reach the lanes that need them through LDS.
+template <int D, int NG>
+struct Raw {
+  uint32_t k[2][D / 32], v[2][D / 32], params[NG];
+};
+// Where its tiles are: the first row of (page, KV head), the tile's first token in the page, and whether there is a page.
+struct Where {
+  long long row0[2];
+  int off[2];
+  bool there[2];
+};
+
+// the largest of a value over lanes 32 .. 63 (NaN only if all are)
+__device__ __forceinline__ float max_upper_half(float v) {
+  auto with = [&](int moved) { v = fmaxf(v, __builtin_bit_cast(float, moved)); };
+  with(__builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0xb1, 0xf, 0xf, true));       // neighbours
+  with(__builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x4e, 0xf, 0xf, true));       // pairs of them
+  with(__builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x141, 0xf, 0xf, true));      // fours (mirrored eight)
+  with(__builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x140, 0xf, 0xf, true));      // eights (mirrored sixteen)
+  return fmaxf(__builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 32)),
+               __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 48)));
+}
+
+template <int N>
+__device__ __forceinline__ void load_words(uint32_t (&dst)[N], const uint8_t* base, uint32_t lane_off) {
+  if constexpr (N == 2) {
+    const uint2 v = *(const uint2*)(base + lane_off);
+    dst[0] = v.x, dst[1] = v.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const u32x4 v = *(const u32x4*)(base + lane_off + 16 * i);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) dst[4 * i + j] = v[j];
+    }
+  }
+}
+
+// CB blocks of sixteen columns share what a wave unpacks.
+template <bool IS_BF16, int D, int G, int CB>
+__global__ __launch_bounds__(256, CB == 1 ? 2 : 1) void kv4_attn_kernel(AttnArgs a, const int* __restrict__ block_table,
+                                                                        const int* __restrict__ kv_len) {
   constexpr int KS = D / 32;            // MFMA steps over the head dim = dwords of a lane per K row
   constexpr int NT = D / 16;            // 16-channel tiles of V
   constexpr int NG = D / G;
   constexpr int GS = G / 32, GT = G / 16;
-  constexpr int VW = D / 32;            // dwords of V codes per lane and four tokens
   constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
-  constexpr float NONE = -1e30f;        // the running maximum before the first token
+  constexpr float NONE = -1e30f;        // the reference before the first token
+  constexpr float AT = 6.f, MOST = 14.f;  // log2 of the largest P: where a new reference puts it, and where it may grow to
   constexpr int DC = D < 128 ? D : 128; // channels merged at a time
   __shared__ float s_m[4][16], s_l[4][16];
   __shared__ __attribute__((aligned(16))) float s_o[4][16][DC + 4];
+  __shared__ __attribute__((aligned(16))) uint32_t s_params[4][2][NG][32];
 
   const int pairs = a.batch * a.c.kv_heads;
   const int cblk = blockIdx.x / pairs, pair = blockIdx.x - cblk * pairs;    // (columns of one KV head: on the same XCD if pairs % 8 == 0)
   const int b = pair / a.c.kv_heads, kvh = pair - b * a.c.kv_heads;
   const int group = a.q_heads / a.c.kv_heads, columns = group * a.S;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, lg = lane >> 4;
-  const int col = cblk * 16 + li;
-  const bool col_ok = col < columns;
-  const int row_s = col_ok ? col / group : 0, head = kvh * group + (col_ok ? col - row_s * group : 0);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, lg = lane >> 4;
+  const int col0 = cblk * 16 * CB;
 
-  // tokens: this column sees [0, limit), the block of columns [0, len), none of them masked below `full`
+  // tokens: a column sees [0, limit), the workgroup's columns [0, len), none of them misses one below `full`
   const long long room = (long long)a.max_pages * a.c.page_size;
-  const int L = (int)min((long long)max(a.kv_len[b], 0), room);
-  const int s_first = cblk * 16 / group, s_last = min(cblk * 16 + 15, columns - 1) / group;
-  const int limit = !col_ok ? 0 : a.causal ? L - a.S + row_s + 1 : L;
+  const int L = (int)min((long long)max(kv_len[b], 0), room);
+  const int s_first = col0 / group, s_last = min(col0 + 16 * CB - 1, columns - 1) / group;
   const int len = max(0, a.causal ? L - a.S + s_last + 1 : L);
   const int full = a.causal ? L - a.S + s_first + 1 : L;
   const int per = ((len + a.splits - 1) / a.splits + 127) & ~127;
-  const int start = (int)blockIdx.y * per, end = min(len, start + per);
-  if (a.splits > 1 && start >= end) {       // (the merge does not look at the sums of a split without tokens)
-    if (wave == 0 && lg == 0 && col_ok)
-      a.partial_lse[(((long long)b * a.S + row_s) * a.q_heads + head) * a.splits + blockIdx.y] = -INFINITY;
-    return;
-  }
-
-  QT qreg[KS];
-  float qsum[NG];
-  {
-    const uint16_t* qp = a.q + b * a.q_sb + row_s * a.q_ss + head * a.q_sh + lg * 8;
-    float part[NG];
+  const int start = min((long long)blockIdx.y * per, (long long)len), end = min(len, start + per);
+  int limit[CB];
+  u32x4 q[CB][KS];
+  float qsum[CB][NG], c0[CB][NG], qk[CB];
 #pragma unroll
-    for (int g = 0; g < NG; ++g) part[g] = 0.f;
+  for (int cb = 0; cb < CB; ++cb) {
+    const int col = col0 + cb * 16 + li;
+    const bool col_ok = col < columns;
+    const int row_s = col_ok ? col / group : 0, head = kvh * group + (col_ok ? col - row_s * group : 0);
+    limit[cb] = !col_ok ? 0 : a.causal ? L - a.S + row_s + 1 : L;
+    if (a.splits > 1 && start >= end) {       // (the merge does not look at the sums of a split without tokens)
+      if (wave == 0 && lg == 0 && col_ok)
+        a.partial_lse[(((long long)b * a.S + row_s) * a.q_heads + head) * a.splits + blockIdx.y] = -INFINITY;
+      continue;
+    }
+    // Q as fp16: bf16 rows are brought near 2^8 by a power of two per column, which loses nothing that a score could show
+    // (numbers 2^-32 of the column's largest).  A negative scale turns Q's sign, so that larger scores are larger weights.
+    const uint16_t* qp = a.q + b * a.q_sb + row_s * a.q_ss + head * a.q_sh + lg * 8;
+    const float sign = a.scale < 0.f ? -1.f : 1.f;
+    const float lead = fabsf(a.soft_cap > 0.f ? a.scale / a.soft_cap : a.scale * LOG2E);
+    u32x4 raw[KS];
+    float top = 0.f;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      u32x4 v = u32x4{0, 0, 0, 0};
-      if (col_ok) v = *(const u32x4*)(qp + 32 * s);
-      qreg[s] = __builtin_bit_cast(QT, v);
+      raw[s] = u32x4{0, 0, 0, 0};
+      if (col_ok) raw[s] = *(const u32x4*)(qp + 32 * s);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) part[s / GS] += from16<IS_BF16>(v[i] & 0xffffu) + low_of<IS_BF16>(v[i]);
+      for (int i = 0; i < 4; ++i)
+        top = fmaxf(top, fmaxf(fabsf(from16<IS_BF16>(raw[s][i] & 0xffffu)), fabsf(low_of<IS_BF16>(raw[s][i]))));
     }
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      part[g] += __shfl_xor(part[g], 16);
-      qsum[g] = part[g] + __shfl_xor(part[g], 32);
-    }
-  }
-
-  float m = NONE, l = 0.f, corr[NG];
-  f32x4 o[NT];
-#pragma unroll
-  for (int j = 0; j < NT; ++j) o[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int g = 0; g < NG; ++g) corr[g] = 0.f;
-  const float qk = a.soft_cap > 0.f ? a.scale / a.soft_cap : a.scale * LOG2E;
-  const int* table = a.table + (long long)b * a.table_stride;
-
-  for (int n0 = start + 32 * wave; n0 < end; n0 += 128) {
-    uint32_t kw[2][KS], vw[2][VW], kp[2][NG][4], vp[2][NG][4];
-    bool there[2];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int tok = __builtin_amdgcn_readfirstlane(n0 + 16 * t);
-      const Place at = place_of(a.c, table, tok < end ? tok : -1, a.max_pages);
-      there[t] = at.page >= 0;
-      const long long row0 = ((long long)max(at.page, 0) * a.c.kv_heads + kvh) * a.c.page_size;
-      const uint32_t* kc = (const uint32_t*)(a.c.k_codes + (row0 + at.off + li) * (D / 2)) + lg * KS;
-      const uint32_t* vc = (const uint32_t*)(a.c.v_codes + (row0 + at.off + 4 * lg) * (D / 2)) + li * VW;
-#pragma unroll
-      for (int i = 0; i < KS; ++i) kw[t][i] = kc[i];
-#pragma unroll
-      for (int i = 0; i < VW; ++i) vw[t][i] = vc[i];
-#pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        const long long at_p = row0 * NG + (long long)g * a.c.page_size + at.off + 4 * lg;
-        const u32x4 kk = *(const u32x4*)(a.c.k_params + at_p), vv = *(const u32x4*)(a.c.v_params + at_p);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) kp[t][g][i] = kk[i], vp[t][g][i] = vv[i];
-      }
-    }
-
-    // ---- scores (in units of log2): token n0 + 16 t + 4 lg + i, column li
-    float sc[2][4];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) sc[t][i] = 0.f;
-#pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        const float c0 = -16.f * qsum[g];
-        f32x4 acc = f32x4{c0, c0, c0, c0};
-#pragma unroll
-        for (int s = g * GS; s < (g + 1) * GS; ++s) {
-          using U = Unpack<IS_BF16>;
-          const uint32_t w = kw[t][s];
-          const u32x4 k = u32x4{U::template pair<0>(w), U::template pair<1>(w), U::template pair<2>(w), U::template pair<3>(w)};
-          acc = F::mfma(__builtin_bit_cast(QT, k), qreg[s], acc);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          sc[t][i] += scale_of<IS_BF16>(kp[t][g][i]) * acc[i] + low_of<IS_BF16>(kp[t][g][i]) * qsum[g];
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) sc[t][i] *= qk;
-      if (a.soft_cap > 0.f) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)       // cap tanh(x) = cap (1 - 2 / (e^2x + 1))
-          sc[t][i] = a.soft_cap * LOG2E * (1.f - 2.f / (exp2_fast(2.f * LOG2E * sc[t][i]) + 1.f));
-      }
-    }
-    // ---- masks: the parameters of tokens that are not there may hold anything, so they are cleared, not multiplied away
-    const bool masked = n0 + 32 > min(full, end) || !there[0] || !there[1];
-    if (masked) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int tok = n0 + 16 * t + 4 * lg + i;
-          if (!there[t] || tok >= min(limit, end)) sc[t][i] = -INFINITY;
-        }
-    }
-    float top = sc[0][0];
-#pragma unroll
-    for (int i = 1; i < 8; ++i) top = fmaxf(top, sc[i >> 2][i & 3]);
-    if (__any(top > m + 8.f)) {
+    float mul = sign, back = 1.f;
+    if (IS_BF16) {
       top = fmaxf(top, __shfl_xor(top, 16));
       top = fmaxf(top, __shfl_xor(top, 32));
-      const float m_new = fmaxf(m, top), f = exp2_fast(m - m_new);
-      m = m_new;
-      l *= f;
-#pragma unroll
-      for (int g = 0; g < NG; ++g) corr[g] *= f;
-#pragma unroll
-      for (int j = 0; j < NT; ++j) o[j] *= f;
+      int e = (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127;         // top in [2^e, 2^(e+1))
+      e = e < -100 ? -100 : e > 100 ? 100 : e;
+      mul = sign * __builtin_bit_cast(float, (uint32_t)(127 + 8 - e) << 23);
+      back = __builtin_bit_cast(float, (uint32_t)(127 - 8 + e) << 23);
     }
-    float p[2][4];
+    qk[cb] = fmaxf(lead * back, 1e-37f);      // (never 0: a masked score is -inf, and stays that)
+    float sum0[NG], sum1[NG];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      p[i >> 2][i & 3] = exp2_fast(sc[i >> 2][i & 3] - m);
-      l += p[i >> 2][i & 3];
+    for (int g = 0; g < NG; ++g) sum0[g] = sum1[g] = 0.f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t w = to16<false>(from16<IS_BF16>(raw[s][i] & 0xffffu) * mul) | to16<false>(low_of<IS_BF16>(raw[s][i]) * mul) << 16;
+        q[cb][s][i] = w;
+        (i & 1 ? sum1 : sum0)[s / GS] += from16<false>(w & 0xffffu) + from16<false>(w >> 16);
+      }
     }
-    // ---- O^T += V^T . P^T
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-      bf16x8 hi, lo;
+      sum0[g] += __shfl_xor(sum0[g], 16);
+      sum0[g] += __shfl_xor(sum0[g], 32);
+      sum1[g] += __shfl_xor(sum1[g], 16);
+      sum1[g] += __shfl_xor(sum1[g], 32);
+      qsum[cb][g] = sum0[g] + sum1[g];
+      c0[cb][g] = -1024.f * sum0[g] - 64.f * sum1[g];
+    }
+  }
+  if (a.splits > 1 && start >= end) return;
+
+  float m[CB], l[CB], corr[CB][NG], vs[NG];
+  f32x4 o[CB][NT];
+#pragma unroll
+  for (int cb = 0; cb < CB; ++cb) {
+    m[cb] = NONE, l[cb] = 0.f;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) o[cb][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int g = 0; g < NG; ++g) corr[cb][g] = 0.f;
+  }
+#pragma unroll
+  for (int g = 0; g < NG; ++g) vs[g] = 1.f;
+  bool scaled = false;
+  const Unpack u;
+  u32x4 neg0, neg1;                     // -(1024 + 8) and -(64 + 8)
+#pragma unroll
+  for (int i = 0; i < 4; ++i) neg0[i] = 0xe408e408u, neg1[i] = 0xd480d480u;
+
+  const int* table = block_table + (long long)b * a.table_stride;
+  const int last_tile = (end - 1) >> 4;
+  auto lookup = [&](int n0) -> Where {
+    Where w;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int want = (n0 >> 4) + t, tile = min(want, last_tile);
+      uint32_t i = a.page_magic ? (uint32_t)(((uint64_t)(uint32_t)tile * a.page_magic) >> 32) : (uint32_t)tile;
+      if (i * (uint32_t)a.page_tiles > (uint32_t)tile) --i;     // the quotient, or one more
+      const int page = table[i];
+      w.there[t] = want <= last_tile && page >= 0 && page < a.c.pages;
+      w.row0[t] = ((long long)(w.there[t] ? page : 0) * a.c.kv_heads + kvh) * a.c.page_size;
+      w.off[t] = (tile - (int)i * a.page_tiles) * 16;
+    }
+    return w;
+  };
+  const uint32_t k_lane = li * (D / 2) + lg * (D / 8), v_lane = lg * (2 * D) + li * (D / 8);
+  const uint32_t* p_lane = (lane < 32 ? a.c.k_params : a.c.v_params) + li;      // lane: token lane & 31 of K or V
+  uint32_t(*const params)[NG][32] = s_params[wave];
+  auto load = [&](const Where& w, Raw<D, NG>& r) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      load_words(r.k[t], a.c.k_codes + (w.row0[t] + w.off[t]) * (D / 2), k_lane);
+      load_words(r.v[t], a.c.v_codes + (w.row0[t] + w.off[t]) * (D / 2), v_lane);
+    }
+    const long long at0 = w.row0[0] * NG + w.off[0], at1 = w.row0[1] * NG + w.off[1];
+    const uint32_t* p = p_lane + (lane & 16 ? at1 : at0);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) r.params[g] = p[(long long)g * a.c.page_size];
+  };
+  auto compute = [&](int n0, bool there0, bool there1, const Raw<D, NG>& r) {
+    const bool masked = n0 + 32 > min(full, end) || !there0 || !there1;
+    // ---- the block's widest V scale; the parameters of tokens that are not there may hold anything
+    uint32_t param[NG];
+    float widest = 0x1p-20f;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) param[g] = r.params[g];
+    if (masked) {
+      const bool live = (lane & 16 ? there1 : there0) && n0 + (lane & 31) < end;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) param[g] = live ? param[g] : 0u;
+    }
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      params[lane >> 5][g][lane & 31] = param[g];
+      widest = fmaxf(widest, scale_of<IS_BF16>(param[g]) * vs[g]);
+    }
+    widest = max_upper_half(widest);
+    // ---- scores of token n0 + 16 t + 4 lg + i, column li of each block: sum(q value), still to be times qk
+    float sc[CB][8];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      f32x4 acc[CB];
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const u32x4 kp = *(const u32x4*)&params[0][g][16 * t + 4 * lg];
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb) acc[cb] = f32x4{c0[cb][g], c0[cb][g], c0[cb][g], c0[cb][g]};
+#pragma unroll
+        for (int s = g * GS; s < (g + 1) * GS; ++s) {
+          const uint32_t w = r.k[t][s], w8 = w >> 8;
+          const u32x4 k = u32x4{u.even(w), u.odd(w), u.even(w8), u.odd(w8)};
+#pragma unroll
+          for (int cb = 0; cb < CB; ++cb) acc[cb] = mfma(k, q[cb][s], acc[cb]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float s = scale_of<IS_BF16>(kp[i]), low = low_of<IS_BF16>(kp[i]);
+#pragma unroll
+          for (int cb = 0; cb < CB; ++cb) {
+            const float first = g == 0 ? low * qsum[cb][g] : __builtin_fmaf(low, qsum[cb][g], sc[cb][4 * t + i]);
+            sc[cb][4 * t + i] = __builtin_fmaf(s, acc[cb][i], first);
+          }
+        }
+      }
+    }
+    if (a.soft_cap > 0.f) {
+#pragma unroll
+      for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {         // cap tanh(x) = cap (1 - 2 / (e^2x + 1)), in units of log2, over qk
+          const float e = exp2_fast(2.f * LOG2E * qk[cb] * sc[cb][i]);
+          sc[cb][i] = a.soft_cap * LOG2E * (1.f - 2.f * __builtin_amdgcn_rcpf(e + 1.f));
+        }
+    }
+    float x_mul[CB];
+    uint32_t seen[CB];
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb) x_mul[cb] = a.soft_cap > 0.f ? 1.f : qk[cb], seen[cb] = 255u;
+    if (masked) {
+#pragma unroll
+      for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int tok = n0 + 16 * (i >> 2) + 4 * lg + (i & 3);
+          const bool see = (i < 4 ? there0 : there1) && tok < min(limit[cb], end);
+          sc[cb][i] = see ? sc[cb][i] : -INFINITY;
+          if (!see) seen[cb] &= ~(1u << i);
+        }
+    }
+    // ---- the references: P times a scale stays below 2^MOST (fp16), with as much room below for the small ones
+    const float wide = log2_fast(widest);
+    bool raise = false;
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb) {
+      float top = sc[cb][0];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) top = fmaxf(top, sc[cb][i]);
+      raise |= __builtin_fmaf(top, x_mul[cb], wide) > m[cb] + MOST;
+    }
+    if (__any(raise)) {
+      // scales far from 1 are brought there by a power of two per group, the same for all columns
+      float ratio[NG];
+      bool off = false;
+      widest = 0x1p-20f;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const float w = max_upper_half(fmaxf(0.f, scale_of<IS_BF16>(param[g]) * vs[g]));
+        int e = 0;
+        if (w > 0x1p3f || (w > 0.f && w < 0x1p-9f)) e = (int)(__builtin_bit_cast(uint32_t, w) >> 23) - 127;
+        e = min(max(e, -60), 60);             // (what is further off takes several blocks to arrive)
+        const int have = (int)(__builtin_bit_cast(uint32_t, vs[g]) >> 23) - 127;
+        e = min(max(e, have - 120), have + 120);
+        ratio[g] = __builtin_bit_cast(float, (uint32_t)(127 - e) << 23);
+        vs[g] *= ratio[g];
+        off |= vs[g] != 1.f;
+        widest = fmaxf(widest, w * ratio[g]);
+      }
+      scaled = off;
+      const float now = log2_fast(widest);
+#pragma unroll
+      for (int cb = 0; cb < CB; ++cb) {
+        float top = sc[cb][0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) top = fmaxf(top, sc[cb][i]);
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const float at = __builtin_fmaf(top, x_mul[cb], now);
+        const float to = at > m[cb] + MOST ? at - AT : m[cb];
+        const float f = exp2_fast(m[cb] - to);
+        m[cb] = to;
+        l[cb] *= f;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) corr[cb][g] *= f;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) o[cb][j] *= f * ratio[j / GT];
+      }
+    }
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        float s = scale_of<IS_BF16>(vp[i >> 2][g][i & 3]), low = low_of<IS_BF16>(vp[i >> 2][g][i & 3]);
-        if (masked) {
-          const bool off = sc[i >> 2][i & 3] == -INFINITY;
-          s = off ? 0.f : s, low = off ? 0.f : low;
+        sc[cb][i] = exp2_fast(__builtin_fmaf(sc[cb][i], x_mul[cb], -m[cb]));      // P from here on
+        l[cb] += sc[cb][i];
+      }
+    // ---- O^T += V^T . P^T, group by group: value = scale (code - 8) + (low + 8 scale)
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      float sv[8], zc[8];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const u32x4 vp = *(const u32x4*)&params[1][g][16 * t + 4 * lg];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          sv[4 * t + i] = scale_of<IS_BF16>(vp[i]);
+          zc[4 * t + i] = __builtin_fmaf(8.f, sv[4 * t + i], low_of<IS_BF16>(vp[i]));
         }
-        const float ps = p[i >> 2][i & 3] * s;
-        corr[g] += p[i >> 2][i & 3] * low - 16.f * ps;
-        hi[i] = (__bf16)ps;
-        lo[i] = (__bf16)(ps - (float)hi[i]);
+      }
+      if (scaled) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sv[i] *= vs[g];
+      }
+      u32x4 hi[CB], lo[CB];
+#pragma unroll
+      for (int cb = 0; cb < CB; ++cb) {
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+          float s2[2], c2[2];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) s2[k] = sc[cb][i + k] * sv[i + k], c2[k] = sc[cb][i + k] * zc[i + k];
+          if (masked) {                       // 0 times the NaN of a token that only other columns see
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const bool see = seen[cb] >> (i + k) & 1;
+              s2[k] = see ? s2[k] : 0.f, c2[k] = see ? c2[k] : 0.f;
+            }
+          }
+          corr[cb][g] += c2[0];
+          corr[cb][g] += c2[1];
+          typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
+          const f16x2 h = f16x2{(_Float16)s2[0], (_Float16)s2[1]};
+          hi[cb][i / 2] = __builtin_bit_cast(uint32_t, h);
+          if constexpr (!IS_BF16) {
+            const f16x2 rest = f16x2{(_Float16)(s2[0] - (float)h[0]), (_Float16)(s2[1] - (float)h[1])};
+            lo[cb][i / 2] = __builtin_bit_cast(uint32_t, rest);
+          }
+        }
       }
 #pragma unroll
       for (int j = g * GT; j < (g + 1) * GT; ++j) {
-        using U = Unpack<true>;
-        const uint32_t w0 = vw[0][j / 4 * 2], w1 = vw[0][j / 4 * 2 + 1], w2 = vw[1][j / 4 * 2], w3 = vw[1][j / 4 * 2 + 1];
-        u32x4 v;
-        if (j % 4 == 0) v = u32x4{U::pair<0>(w0), U::pair<0>(w1), U::pair<0>(w2), U::pair<0>(w3)};
-        else if (j % 4 == 1) v = u32x4{U::pair<1>(w0), U::pair<1>(w1), U::pair<1>(w2), U::pair<1>(w3)};
-        else if (j % 4 == 2) v = u32x4{U::pair<2>(w0), U::pair<2>(w1), U::pair<2>(w2), U::pair<2>(w3)};
-        else v = u32x4{U::pair<3>(w0), U::pair<3>(w1), U::pair<3>(w2), U::pair<3>(w3)};
-        o[j] = Frag<true>::mfma(__builtin_bit_cast(typename Frag<true>::T, v), __builtin_bit_cast(typename Frag<true>::T, hi), o[j]);
-        o[j] = Frag<true>::mfma(__builtin_bit_cast(typename Frag<true>::T, v), __builtin_bit_cast(typename Frag<true>::T, lo), o[j]);
-      }
-    }
-  }
-
-  // ---- one column's sums are spread over the four lane groups
-  l += __shfl_xor(l, 16);
-  l += __shfl_xor(l, 32);
+        const int h = j / 4, n = j % 4;
+        uint32_t w[4] = {r.v[0][2 * h], r.v[0][2 * h + 1], r.v[1][2 * h], r.v[1][2 * h + 1]};
+        if (n >= 2) {
 #pragma unroll
-  for (int g = 0; g < NG; ++g) {
-    corr[g] += __shfl_xor(corr[g], 16);
-    corr[g] += __shfl_xor(corr[g], 32);
-  }
-  if (lg == 0) s_m[wave][li] = m, s_l[wave][li] = l;
-  __syncthreads();
-
-  // thread (column c, part): merges the four waves' states for channels part * 4 + 64 i
-  const int mc = threadIdx.x >> 4, part = threadIdx.x & 15;
-  const int mcol = cblk * 16 + mc;
-  const float m_all = fmaxf(fmaxf(s_m[0][mc], s_m[1][mc]), fmaxf(s_m[2][mc], s_m[3][mc]));
-  float f[4], l_all = 0.f;
+          for (int i = 0; i < 4; ++i) w[i] >>= 8;
+        }
+        const u32x4 v = n & 1 ? u32x4{u.odd(w[0]), u.odd(w[1]), u.odd(w[2]), u.odd(w[3])}
+                              : u32x4{u.even(w[0]), u.even(w[1]), u.even(w[2]), u.even(w[3])};
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    f[w] = exp2_fast(s_m[w][mc] - m_all);
-    l_all += s_l[w][mc] * f[w];
-  }
-  const float inv = l_all != 0.f ? 1.f / l_all : 0.f;
-  const float lse = l_all != 0.f ? m_all + log2_fast(l_all) : -INFINITY;
-  const int ms = mcol / group, mh = kvh * group + (mcol - ms * group);
-  const long long row = ((long long)b * a.S + ms) * a.q_heads + mh;
-  float* prow = a.partial + (row * a.splits + blockIdx.y) * D;
-#pragma unroll
-  for (int d0 = 0; d0 < D; d0 += DC) {
-    if (d0) __syncthreads();
-#pragma unroll
-    for (int j = d0 / 16; j < (d0 + DC) / 16; ++j) {
-      f32x4 v = o[j];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] += corr[j / GT];
-      *(f32x4*)&s_o[wave][li][(j - d0 / 16) * 16 + 4 * lg] = v;
-    }
-    __syncthreads();
-    if (mcol < columns) {
-#pragma unroll
-      for (int i = 0; i < DC / 64; ++i) {
-        const int ch = part * 4 + 64 * i;
-        f32x4 r = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int w = 0; w < 4; ++w) r += *(const f32x4*)&s_o[w][mc][ch] * f[w];
-        r *= inv;
-        if (a.splits > 1) {
-          *(f32x4*)(prow + d0 + ch) = r;
-        } else if (a.out_mode == 2) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) ((float*)a.out)[row * (D + 1) + d0 + ch + k] = r[k];
-        } else {
-          const uint2 v = uint2{to16<IS_BF16>(r[0]) | to16<IS_BF16>(r[1]) << 16, to16<IS_BF16>(r[2]) | to16<IS_BF16>(r[3]) << 16};
-          *(uint2*)((uint16_t*)a.out + row * D + d0 + ch) = v;
+        for (int cb = 0; cb < CB; ++cb) {
+          o[cb][j] = mfma(n & 1 ? neg1 : neg0, hi[cb], o[cb][j]);
+          o[cb][j] = mfma(v, hi[cb], o[cb][j]);
+          if constexpr (!IS_BF16) {
+            o[cb][j] = mfma(n & 1 ? neg1 : neg0, lo[cb], o[cb][j]);
+            o[cb][j] = mfma(v, lo[cb], o[cb][j]);
+          }
         }
       }
     }
+  };
+
+  // a wave's blocks are 128 tokens apart: one is multiplied while the next is on its way and the pages of the one after
+  // that are looked up
+  int n0 = start + 32 * wave;
+  if (n0 < end) {
+    Raw<D, NG> r0, r1;
+    Where w0 = lookup(n0), w1;
+    load(w0, r0);
+    w1 = lookup(n0 + 128);
+    for (;;) {
+      const bool a0 = w0.there[0], a1 = w0.there[1];
+      if (n0 + 128 < end) load(w1, r1);
+      w0 = lookup(n0 + 256);
+      compute(n0, a0, a1, r0);
+      n0 += 128;
+      if (n0 >= end) break;
+      const bool b0 = w1.there[0], b1 = w1.there[1];
+      if (n0 + 128 < end) load(w0, r0);
+      w1 = lookup(n0 + 256);
+      compute(n0, b0, b1, r1);
+      n0 += 128;
+      if (n0 >= end) break;
+    }
   }
-  if (mcol < columns && part == 0) {
-    if (a.splits > 1) a.partial_lse[row * a.splits + blockIdx.y] = lse;
-    else if (a.out_mode == 2) ((float*)a.out)[row * (D + 1) + D] = lse * LN2;
+
+  // ---- merge: one column's sums are spread over the four lane groups, then over the four waves
+#pragma unroll
+  for (int cb = 0; cb < CB; ++cb) {
+    l[cb] += __shfl_xor(l[cb], 16);
+    l[cb] += __shfl_xor(l[cb], 32);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      corr[cb][g] += __shfl_xor(corr[cb][g], 16);
+      corr[cb][g] += __shfl_xor(corr[cb][g], 32);
+    }
+    if (cb) __syncthreads();
+    if (lg == 0) s_m[wave][li] = m[cb], s_l[wave][li] = l[cb];
+    __syncthreads();
+    // thread (column mc, part): channels part * 4 + 64 i of that column
+    const int mc = threadIdx.x >> 4, part = threadIdx.x & 15;
+    const int mcol = col0 + cb * 16 + mc;
+    const float m_all = fmaxf(fmaxf(s_m[0][mc], s_m[1][mc]), fmaxf(s_m[2][mc], s_m[3][mc]));
+    float f[4], l_all = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      f[w] = exp2_fast(s_m[w][mc] - m_all);
+      l_all += s_l[w][mc] * f[w];
+    }
+    const float inv = l_all != 0.f ? 1.f / l_all : 0.f;
+    const float lse = l_all != 0.f ? m_all + log2_fast(l_all) : -INFINITY;
+    const int ms = mcol / group, mh = kvh * group + (mcol - ms * group);
+    const long long row = ((long long)b * a.S + ms) * a.q_heads + mh;
+    float* prow = a.partial + (row * a.splits + blockIdx.y) * D;
+#pragma unroll
+    for (int d0 = 0; d0 < D; d0 += DC) {
+      if (d0) __syncthreads();
+#pragma unroll
+      for (int j = d0 / 16; j < (d0 + DC) / 16; ++j) {
+        f32x4 v = o[cb][j];
+        const float undo = 1.f / vs[j / GT];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = __builtin_fmaf(v[i], undo, corr[cb][j / GT]);
+        *(f32x4*)&s_o[wave][li][(j - d0 / 16) * 16 + 4 * lg] = v;
+      }
+      __syncthreads();
+      if (mcol < columns) {
+#pragma unroll
+        for (int i = 0; i < DC / 64; ++i) {
+          const int ch = part * 4 + 64 * i;
+          f32x4 r = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int w = 0; w < 4; ++w) r += *(const f32x4*)&s_o[w][mc][ch] * f[w];
+          r *= inv;
+          if (a.splits > 1) {
+            *(f32x4*)(prow + d0 + ch) = r;
+          } else if (a.out_mode == 2) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) ((float*)a.out)[row * (D + 1) + d0 + ch + k] = r[k];
+          } else {
+            const uint2 v = uint2{to16<IS_BF16>(r[0]) | to16<IS_BF16>(r[1]) << 16, to16<IS_BF16>(r[2]) | to16<IS_BF16>(r[3]) << 16};
+            *(uint2*)((uint16_t*)a.out + row * D + d0 + ch) = v;
+          }
+        }
+      }
+    }
+    if (mcol < columns && part == 0) {
+      if (a.splits > 1) a.partial_lse[row * a.splits + blockIdx.y] = lse;
+      else if (a.out_mode == 2) ((float*)a.out)[row * (D + 1) + D] = lse * LN2;
+    }
   }
 }
 
@@ -385,16 +599,24 @@ TDIST_API int tdist_kv4_attn(const void* k_codes, const void* v_codes, const voi
   TDIST_REQUIRE(q && table && kv_len && out, "null argument");
   TDIST_REQUIRE(((uintptr_t)q & 15) == 0 && ((uintptr_t)out & 7) == 0 && ((q_sb | q_ss | q_sh) & 7) == 0,
                 "q rows must keep 16-byte alignment");
-  const long long cblocks = ((long long)(q_heads / kv_heads) * S + 15) / 16, blocks = cblocks * batch * kv_heads;
+  const long long columns = (long long)(q_heads / kv_heads) * S, per_group = columns > 16 ? 2 : 1;
+  const long long blocks = (columns + 16 * per_group - 1) / (16 * per_group) * batch * kv_heads;
   TDIST_REQUIRE(blocks < (1ll << 31) && (long long)batch * S * q_heads < (1ll << 31), "too many query rows");
-  a.q = (const uint16_t*)q, a.table = table, a.kv_len = kv_len, a.partial = partial, a.out = out;
+  a.q = (const uint16_t*)q, a.partial = partial, a.out = out;
+  a.page_tiles = page_size / 16;
+  a.page_magic = a.page_tiles == 1 ? 0u : (uint32_t)((1ull << 32) / a.page_tiles) + 1u;
   a.partial_lse = partial ? partial + (long long)batch * S * q_heads * splits * head_dim : nullptr;
   a.q_sb = q_sb, a.q_ss = q_ss, a.q_sh = q_sh, a.table_stride = table_stride, a.max_pages = max_pages;
   a.batch = batch, a.S = S, a.q_heads = q_heads, a.splits = splits, a.causal = causal, a.out_mode = out_mode;
   a.scale = scale, a.soft_cap = soft_cap;
   const bool ok = dispatch(dtype, head_dim, group, [&](auto bf, auto d, auto g) {
-    hipLaunchKernelGGL((kv4_attn_kernel<decltype(bf)::value, decltype(d)::value, decltype(g)::value>),
-                       dim3((unsigned)blocks, splits), dim3(256), 0, (hipStream_t)stream, a);
+    auto launch = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3((unsigned)blocks, splits), dim3(256), 0, (hipStream_t)stream, a, table, kv_len);
+    };
+    constexpr bool BF = decltype(bf)::value;
+    constexpr int D = decltype(d)::value, G = decltype(g)::value;
+    if (per_group == 2) launch(kv4_attn_kernel<BF, D, G, 2>);
+    else launch(kv4_attn_kernel<BF, D, G, 1>);
   });
   TDIST_REQUIRE(ok, "head_dim 64 / 128 / 256 with groups of 32 / 64 / 128 channels (at most head_dim)");
   TDIST_HIP_TRY(hipGetLastError());

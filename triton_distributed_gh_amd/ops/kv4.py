@@ -23,7 +23,6 @@ captured into a graph.  None of it has a gradient: it refuses inputs that ask fo
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import dataclasses
 import math
@@ -35,7 +34,31 @@ from .. import _lib
 
 HEAD_DIMS = (64, 128, 256)
 GROUPS = (32, 64, 128)
-_LL = ctypes.c_longlong
+
+# argument types of the native calls (p pointer, i int, q long long, f float), so that plain integers can be passed; the
+# stream comes last everywhere
+_CACHE_ARGS = "ppppiiiii"
+_SIGNATURES = {
+    "tdist_kv4_append": _CACHE_ARGS + "pp" + "qqqqqq" + "ppp" + "iiiii" + "p",
+    "tdist_kv4_qkv_prep": _CACHE_ARGS + "pqqppffpppq" + "pppp" + "iiiii" + "p",
+    "tdist_kv4_read": _CACHE_ARGS + "pii" + "pp" + "iq" + "pp" + "qqqq" + "i" + "p",
+    "tdist_kv4_attn": _CACHE_ARGS + "pqqq" + "pii" + "ppp" + "iiiiii" + "ff" + "i" + "p",
+}
+_CTYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "q": ctypes.c_longlong, "f": ctypes.c_float}
+
+
+def _launch(name: str, device: torch.device, *args) -> None:
+    """One native call on the current stream of ``device``.  (A decode step makes a few of these per layer: a token's worth of
+    work on the GPU is shorter than a careless call, so streams and pointers are passed as plain integers.)"""
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _launch(name, device, *args)
+    fn = getattr(_lib.hip(), name)
+    if fn.argtypes is None:
+        fn.argtypes = [_CTYPES[c] for c in _SIGNATURES[name]]
+    code = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    if code:
+        _lib.check(code, name)
 
 
 def _require(cond: bool, msg: str) -> None:
@@ -43,7 +66,11 @@ def _require(cond: bool, msg: str) -> None:
         raise ValueError(msg)
 
 
-@dataclasses.dataclass
+def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
+
+
+@dataclasses.dataclass(frozen=True, eq=False)
 class Int4KVCache:
     """One layer's pages.  The four tensors are packed as csrc/include/tdist/kv4.hpp describes; ``kv4_read`` gives the values.
 
@@ -58,23 +85,25 @@ class Int4KVCache:
     def __post_init__(self):
         k, v, kp, vp = self.k_codes, self.v_codes, self.k_params, self.v_params
         _require(k.dim() == 4 and v.dim() == 4 and kp.dim() == 5, "a 4-bit cache has 4-dimensional codes and 5-dimensional parameters")
-        self.num_pages, self.kv_heads, self.page_size, self.head_dim = k.shape[0], k.shape[1], k.shape[2], k.shape[3] * 2
-        _require(self.head_dim in HEAD_DIMS, f"head_dim must be one of {HEAD_DIMS}, got {self.head_dim}")
-        _require(kp.shape[2] > 0 and self.head_dim % kp.shape[2] == 0, "the groups must divide the head")
-        self.group = self.head_dim // kp.shape[2]
-        _require(self.group in GROUPS, f"groups must be of {GROUPS} channels, got {self.group}")
-        _require(self.page_size > 0 and self.page_size % 16 == 0, f"pages must hold a multiple of 16 tokens, got {self.page_size}")
-        _require(self.num_pages > 0 and 0 < self.kv_heads <= 16384, "a cache needs pages, and 1 .. 16384 heads")
-        P, H, S, D = self.num_pages, self.kv_heads, self.page_size, self.head_dim
+        P, H, S, D = k.shape[0], k.shape[1], k.shape[2], k.shape[3] * 2
+        _require(D in HEAD_DIMS, f"head_dim must be one of {HEAD_DIMS}, got {D}")
+        _require(kp.shape[2] > 0 and D % kp.shape[2] == 0, "the groups must divide the head")
+        G = D // kp.shape[2]
+        _require(G in GROUPS, f"groups must be of {GROUPS} channels, got {G}")
+        _require(S > 0 and S % 16 == 0, f"pages must hold a multiple of 16 tokens, got {S}")
+        _require(P > 0 and 0 < H <= 16384, "a cache needs pages, and 1 .. 16384 heads")
         _require(tuple(v.shape) == (P, H, S // 4, 2 * D), f"v_codes must be {(P, H, S // 4, 2 * D)}, got {tuple(v.shape)}")
-        _require(kp.shape == vp.shape == (P, H, D // self.group, S, 2), f"parameters must be {(P, H, D // self.group, S, 2)}")
+        _require(kp.shape == vp.shape == (P, H, D // G, S, 2), f"parameters must be {(P, H, D // G, S, 2)}")
         _require(k.dtype == v.dtype == torch.uint8, "codes are uint8")
-        self.dtype, self.device = kp.dtype, k.device
         if kp.dtype not in (torch.bfloat16, torch.float16) or vp.dtype != kp.dtype:
             raise TypeError(f"a 4-bit cache stands for bf16 or fp16 rows, got {kp.dtype} / {vp.dtype}")
         for t in (k, v, kp, vp):
-            _require(t.device == self.device, "the four tensors of a cache live on one device")
+            _require(t.device == k.device, "the four tensors of a cache live on one device")
             _require(t.is_contiguous() and t.data_ptr() % 16 == 0, "cache tensors must be contiguous and 16-byte aligned")
+        native = (k.data_ptr(), v.data_ptr(), kp.data_ptr(), vp.data_ptr(), P, H, S, D, G)
+        for name, value in dict(num_pages=P, kv_heads=H, page_size=S, head_dim=D, group=G, dtype=kp.dtype, device=k.device,
+                                _native=native).items():
+            object.__setattr__(self, name, value)
 
     @classmethod
     def alloc(cls, num_pages: int, page_size: int, kv_heads: int, head_dim: int, group: int = 64, dtype=torch.bfloat16,
@@ -91,10 +120,6 @@ class Int4KVCache:
                    torch.zeros(num_pages, kv_heads, page_size // 4, 2 * head_dim, dtype=torch.uint8, device=device),
                    params(), params())
 
-    def _native_args(self):
-        return (_lib.ptr(self.k_codes), _lib.ptr(self.v_codes), _lib.ptr(self.k_params), _lib.ptr(self.v_params), self.num_pages,
-                self.kv_heads, self.page_size, self.head_dim, self.group)
-
 
 # ---- checks --------------------------------------------------------------------------------------------------------
 def _dt(dtype: torch.dtype) -> int:
@@ -105,34 +130,33 @@ def _check_data(cache: Int4KVCache, **rows: torch.Tensor) -> None:
     for name, t in rows.items():
         if t.dtype != cache.dtype:
             raise TypeError(f"{name} must be {cache.dtype} like the cache, got {t.dtype}")
-        _require(t.device == cache.device, f"{name} is on {t.device}, the cache on {cache.device}")
+        if t.device != cache.device:
+            raise ValueError(f"{name} is on {t.device}, the cache on {cache.device}")
         if t.requires_grad and torch.is_grad_enabled():
             raise RuntimeError(f"a 4-bit cache has no gradient: {name} requires one (detach it, or run under torch.no_grad())")
 
 
 def _check_index(cache: Int4KVCache, batch: int, block_table: torch.Tensor, **counts: Optional[torch.Tensor]) -> None:
-    _require(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[0] == batch
-             and (block_table.shape[1] <= 1 or block_table.stride(1) == 1) and block_table.device == cache.device,
-             f"block_table must be int32 [{batch}, max_pages] with contiguous rows on {cache.device}")
-    _require(block_table.shape[1] * cache.page_size < 2 ** 31, "a sequence holds less than 2^31 tokens")
+    if not (block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[0] == batch
+            and (block_table.shape[1] <= 1 or block_table.stride(1) == 1) and block_table.device == cache.device
+            and block_table.shape[1] * cache.page_size < 2 ** 31):
+        raise ValueError(f"block_table must be int32 [{batch}, max_pages] with contiguous rows of less than 2^31 tokens on "
+                         f"{cache.device}")
     for name, t in counts.items():
-        if t is not None:
-            n = batch + 1 if name == "cu_seqlens" else batch
-            _require(t.dtype == torch.int32 and t.shape == (n,) and t.is_contiguous() and t.device == cache.device,
-                     f"{name} must be contiguous int32 [{n}] on {cache.device}")
+        if t is None:
+            continue
+        n = batch + 1 if name == "cu_seqlens" else batch
+        if not (t.dtype == torch.int32 and t.dim() == 1 and t.shape[0] == n and (n <= 1 or t.stride(0) == 1)
+                and t.device == cache.device):
+            raise ValueError(f"{name} must be contiguous int32 [{n}] on {cache.device}")
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
     """``x`` itself where the kernels can take its rows 16 bytes at a time, else a contiguous copy."""
-    ok = x.stride(-1) == 1 and x.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in x.stride()[:-1])
-    return x if ok else x.clone(memory_format=torch.contiguous_format)
-
-
-def _on(device: torch.device):
-    """The launch device, where it is not the current one already."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+    *outer, last = x.stride()
+    if last == 1 and x.data_ptr() % 16 == 0 and not any(s % 8 for s in outer):
+        return x
+    return x.clone(memory_format=torch.contiguous_format)
 
 
 # ---- the packed layout in torch: CPU path and test oracle ----------------------------------------------------------
@@ -237,13 +261,9 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, cache: Int4KVCache, kv_offset: 
         _store_reference(cache, k.flatten(0, 1), v.flatten(0, 1), of.flatten(), pos.flatten(), block_table)
         return
     k, v = _rows(k), _rows(v)
-    with _on(cache.device):
-        _lib.check(
-            _lib.hip().tdist_kv4_append(
-                *cache._native_args(), _lib.ptr(k), _lib.ptr(v), _LL(k.stride(0)), _LL(k.stride(1)), _LL(k.stride(2)),
-                _LL(v.stride(0)), _LL(v.stride(1)), _LL(v.stride(2)), _lib.ptr(kv_offset), _lib.ptr(new_lens),
-                _lib.ptr(block_table), block_table.stride(0), block_table.shape[1], batch, S, _dt(cache.dtype),
-                _lib.stream_handle()), "tdist_kv4_append")
+    _launch("tdist_kv4_append", cache.device, *cache._native, k.data_ptr(), v.data_ptr(), *k.stride()[:3], *v.stride()[:3],
+            kv_offset.data_ptr(), _ptr(new_lens), block_table.data_ptr(), block_table.stride(0), block_table.shape[1], batch, S,
+            _dt(cache.dtype))
 
 
 def kv4_qkv_prep(qkv: torch.Tensor, q_w: Optional[torch.Tensor], k_w: Optional[torch.Tensor], q_eps: float, k_eps: float,
@@ -291,14 +311,10 @@ def kv4_qkv_prep(qkv: torch.Tensor, q_w: Optional[torch.Tensor], k_w: Optional[t
         return q
     qkv = _rows(qkv)
     q_w, k_w = (w if w is None else _rows(w) for w in (q_w, k_w))
-    with _on(cache.device):
-        q = torch.empty((batch, S, num_q_heads, D), dtype=qkv.dtype, device=qkv.device)
-        _lib.check(
-            _lib.hip().tdist_kv4_qkv_prep(
-                *cache._native_args(), _lib.ptr(qkv), _LL(qkv.stride(0)), _LL(qkv.stride(1)), _lib.ptr(q_w), _lib.ptr(k_w),
-                ctypes.c_float(q_eps), ctypes.c_float(k_eps), _lib.ptr(pos), _lib.ptr(cos), _lib.ptr(sin), _LL(cos.shape[0]),
-                _lib.ptr(q), _lib.ptr(kv_offset), _lib.ptr(total_out), _lib.ptr(block_table), block_table.stride(0),
-                block_table.shape[1], batch, S, num_q_heads, _lib.stream_handle()), "tdist_kv4_qkv_prep")
+    q = torch.empty((batch, S, num_q_heads, D), dtype=qkv.dtype, device=qkv.device)
+    _launch("tdist_kv4_qkv_prep", cache.device, *cache._native, qkv.data_ptr(), *qkv.stride()[:2], _ptr(q_w), _ptr(k_w), q_eps,
+            k_eps, pos.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0], q.data_ptr(), kv_offset.data_ptr(),
+            total_out.data_ptr(), block_table.data_ptr(), block_table.stride(0), block_table.shape[1], batch, S, num_q_heads)
     return q
 
 
@@ -337,12 +353,9 @@ def kv4_read(cache: Int4KVCache, block_table: torch.Tensor, cu_seqlens: torch.Te
         most = torch.finfo(cache.dtype).max
         k[r], v[r] = kk.clamp(max=most).to(cache.dtype), vv.clamp(max=most).to(cache.dtype)
         return k, v
-    with _on(cache.device):
-        _lib.check(
-            _lib.hip().tdist_kv4_read(
-                *cache._native_args(), _lib.ptr(block_table), block_table.stride(0), block_table.shape[1], _lib.ptr(cu_seqlens),
-                _lib.ptr(starts), batch, _LL(int(total)), _lib.ptr(k), _lib.ptr(v), _LL(k.stride(0)), _LL(k.stride(1)),
-                _LL(v.stride(0)), _LL(v.stride(1)), _dt(cache.dtype), _lib.stream_handle()), "tdist_kv4_read")
+    _launch("tdist_kv4_read", cache.device, *cache._native, block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
+            cu_seqlens.data_ptr(), _ptr(starts), batch, int(total), k.data_ptr(), v.data_ptr(), *k.stride()[:2], *v.stride()[:2],
+            _dt(cache.dtype))
     return k, v
 
 
@@ -412,15 +425,11 @@ def gqa_fwd_kv4(q: torch.Tensor, cache: Int4KVCache, kv_lens: torch.Tensor, bloc
     q4 = _rows(q4)
     blocks = batch * cache.kv_heads * ((Hq // cache.kv_heads * S + 15) // 16)
     splits = int(kv_split) if kv_split > 0 else auto_kv_splits(blocks, block_table.shape[1] * cache.page_size)
-    with _on(cache.device):
-        out = torch.empty(shape, dtype=torch.float32 if return_lse else q.dtype, device=q.device)
-        part = torch.empty(batch * S * Hq * splits * (D + 1), dtype=torch.float32, device=q.device) if splits > 1 else None
-        _lib.check(
-            _lib.hip().tdist_kv4_attn(
-                *cache._native_args(), _lib.ptr(q4), _LL(q4.stride(0)), _LL(q4.stride(1)), _LL(q4.stride(2)),
-                _lib.ptr(block_table), block_table.stride(0), block_table.shape[1], _lib.ptr(kv_lens), _lib.ptr(part),
-                _lib.ptr(out), batch, S, Hq, splits, 1 if causal else 0, 2 if return_lse else 1, ctypes.c_float(scale),
-                ctypes.c_float(soft_cap), _dt(cache.dtype), _lib.stream_handle()), "tdist_kv4_attn")
+    out = torch.empty(shape, dtype=torch.float32 if return_lse else q.dtype, device=q.device)
+    part = torch.empty(batch * S * Hq * splits * (D + 1), dtype=torch.float32, device=q.device) if splits > 1 else None
+    _launch("tdist_kv4_attn", cache.device, *cache._native, q4.data_ptr(), *q4.stride()[:3], block_table.data_ptr(),
+            block_table.stride(0), block_table.shape[1], kv_lens.data_ptr(), _ptr(part), out.data_ptr(), batch, S, Hq, splits,
+            1 if causal else 0, 2 if return_lse else 1, scale, soft_cap, _dt(cache.dtype))
     return out.squeeze(1) if flat else out
 
 
