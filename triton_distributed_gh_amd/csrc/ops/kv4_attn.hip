@@ -39,6 +39,8 @@ struct AttnArgs {
 typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 
+#define INLINE __attribute__((always_inline))     // (lambdas: a call would put what they capture into memory)
+
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float log2_fast(float x) { return __builtin_amdgcn_logf(x); }
 __device__ __forceinline__ f32x4 mfma(const u32x4& a, const u32x4& b, const f32x4& c) {
@@ -100,7 +102,7 @@ __device__ __forceinline__ void load_words(uint32_t (&dst)[N], const uint8_t* ba
 
 // CB blocks of sixteen columns share what a wave unpacks.
 template <bool IS_BF16, int D, int G, int CB>
-__global__ __launch_bounds__(256, CB == 1 ? 2 : 1) void kv4_attn_kernel(AttnArgs a, const int* __restrict__ block_table,
+__global__ __launch_bounds__(256, CB == 1 || D <= 128 ? 2 : 1) void kv4_attn_kernel(AttnArgs a, const int* __restrict__ block_table,
                                                                         const int* __restrict__ kv_len) {
   constexpr int KS = D / 32;            // MFMA steps over the head dim = dwords of a lane per K row
   constexpr int NT = D / 16;            // 16-channel tiles of V
@@ -108,6 +110,7 @@ __global__ __launch_bounds__(256, CB == 1 ? 2 : 1) void kv4_attn_kernel(AttnArgs
   constexpr int GS = G / 32, GT = G / 16;
   constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
   constexpr float NONE = -1e30f;        // the reference before the first token
+  constexpr float WIDE = 0x1p3f, NARROW = 0x1p-9f;      // V scales that are taken as they are
   constexpr float AT = 6.f, MOST = 14.f;  // log2 of the largest P: where a new reference puts it, and where it may grow to
   constexpr int DC = D < 128 ? D : 128; // channels merged at a time
   __shared__ float s_m[4][16], s_l[4][16];
@@ -128,69 +131,77 @@ __global__ __launch_bounds__(256, CB == 1 ? 2 : 1) void kv4_attn_kernel(AttnArgs
   const int len = max(0, a.causal ? L - a.S + s_last + 1 : L);
   const int full = a.causal ? L - a.S + s_first + 1 : L;
   const int per = ((len + a.splits - 1) / a.splits + 127) & ~127;
-  const int start = min((long long)blockIdx.y * per, (long long)len), end = min(len, start + per);
+  const int start = (int)min((long long)blockIdx.y * per, (long long)len), end = min(len, start + per);
+  if (a.splits > 1 && start >= end) {         // (the merge does not look at the sums of a split without tokens)
+    const int col = col0 + (int)threadIdx.x;
+    if (threadIdx.x < 16 * CB && col < columns)
+      a.partial_lse[(((long long)b * a.S + col / group) * a.q_heads + kvh * group + col % group) * a.splits + blockIdx.y] = -INFINITY;
+    return;
+  }
+
+  // Q as fp16: bf16 rows are brought near 2^8 by a power of two per column, which loses nothing that a score could show
+  // (numbers 2^-32 of the column's largest).  A negative scale turns Q's sign, so that larger scores are larger weights.
   int limit[CB];
   u32x4 q[CB][KS];
-  float qsum[CB][NG], c0[CB][NG], qk[CB];
-#pragma unroll
-  for (int cb = 0; cb < CB; ++cb) {
-    const int col = col0 + cb * 16 + li;
-    const bool col_ok = col < columns;
-    const int row_s = col_ok ? col / group : 0, head = kvh * group + (col_ok ? col - row_s * group : 0);
-    limit[cb] = !col_ok ? 0 : a.causal ? L - a.S + row_s + 1 : L;
-    if (a.splits > 1 && start >= end) {       // (the merge does not look at the sums of a split without tokens)
-      if (wave == 0 && lg == 0 && col_ok)
-        a.partial_lse[(((long long)b * a.S + row_s) * a.q_heads + head) * a.splits + blockIdx.y] = -INFINITY;
-      continue;
-    }
-    // Q as fp16: bf16 rows are brought near 2^8 by a power of two per column, which loses nothing that a score could show
-    // (numbers 2^-32 of the column's largest).  A negative scale turns Q's sign, so that larger scores are larger weights.
-    const uint16_t* qp = a.q + b * a.q_sb + row_s * a.q_ss + head * a.q_sh + lg * 8;
+  float qsum[CB][NG], qk[CB];
+  f32x4 c0[CB][NG];                           // what the accumulators start at
+  auto prepare_q = [&]() INLINE {
     const float sign = a.scale < 0.f ? -1.f : 1.f;
     const float lead = fabsf(a.soft_cap > 0.f ? a.scale / a.soft_cap : a.scale * LOG2E);
-    u32x4 raw[KS];
-    float top = 0.f;
+    u32x4 raw[CB][KS];
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      raw[s] = u32x4{0, 0, 0, 0};
-      if (col_ok) raw[s] = *(const u32x4*)(qp + 32 * s);
+    for (int cb = 0; cb < CB; ++cb) {
+      const int col = col0 + cb * 16 + li;
+      const bool col_ok = col < columns;
+      const int row_s = col_ok ? col / group : 0, head = kvh * group + (col_ok ? col - row_s * group : 0);
+      limit[cb] = !col_ok ? 0 : a.causal ? L - a.S + row_s + 1 : L;
+      const uint16_t* qp = a.q + b * a.q_sb + row_s * a.q_ss + head * a.q_sh + lg * 8;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        top = fmaxf(top, fmaxf(fabsf(from16<IS_BF16>(raw[s][i] & 0xffffu)), fabsf(low_of<IS_BF16>(raw[s][i]))));
-    }
-    float mul = sign, back = 1.f;
-    if (IS_BF16) {
-      top = fmaxf(top, __shfl_xor(top, 16));
-      top = fmaxf(top, __shfl_xor(top, 32));
-      int e = (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127;         // top in [2^e, 2^(e+1))
-      e = e < -100 ? -100 : e > 100 ? 100 : e;
-      mul = sign * __builtin_bit_cast(float, (uint32_t)(127 + 8 - e) << 23);
-      back = __builtin_bit_cast(float, (uint32_t)(127 - 8 + e) << 23);
-    }
-    qk[cb] = fmaxf(lead * back, 1e-37f);      // (never 0: a masked score is -inf, and stays that)
-    float sum0[NG], sum1[NG];
-#pragma unroll
-    for (int g = 0; g < NG; ++g) sum0[g] = sum1[g] = 0.f;
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t w = to16<false>(from16<IS_BF16>(raw[s][i] & 0xffffu) * mul) | to16<false>(low_of<IS_BF16>(raw[s][i]) * mul) << 16;
-        q[cb][s][i] = w;
-        (i & 1 ? sum1 : sum0)[s / GS] += from16<false>(w & 0xffffu) + from16<false>(w >> 16);
+      for (int s = 0; s < KS; ++s) {
+        raw[cb][s] = u32x4{0, 0, 0, 0};
+        if (col_ok) raw[cb][s] = *(const u32x4*)(qp + 32 * s);
       }
     }
 #pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      sum0[g] += __shfl_xor(sum0[g], 16);
-      sum0[g] += __shfl_xor(sum0[g], 32);
-      sum1[g] += __shfl_xor(sum1[g], 16);
-      sum1[g] += __shfl_xor(sum1[g], 32);
-      qsum[cb][g] = sum0[g] + sum1[g];
-      c0[cb][g] = -1024.f * sum0[g] - 64.f * sum1[g];
+    for (int cb = 0; cb < CB; ++cb) {
+      float mul = sign, back = 1.f;
+      if (IS_BF16) {
+        float top = 0.f;
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            top = fmaxf(top, fmaxf(fabsf(from16<IS_BF16>(raw[cb][s][i] & 0xffffu)), fabsf(low_of<IS_BF16>(raw[cb][s][i]))));
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        int e = (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127;       // top in [2^e, 2^(e+1))
+        e = e < -100 ? -100 : e > 100 ? 100 : e;
+        mul = sign * __builtin_bit_cast(float, (uint32_t)(127 + 8 - e) << 23);
+        back = __builtin_bit_cast(float, (uint32_t)(127 - 8 + e) << 23);
+      }
+      qk[cb] = fmaxf(lead * back, 1e-37f);    // (never 0: a masked score is -inf, and stays that)
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        float sum0 = 0.f, sum1 = 0.f;         // of the channels that unpack as 1024 + code, and as 64 + code
+#pragma unroll
+        for (int s = g * GS; s < (g + 1) * GS; ++s)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t w = to16<false>(from16<IS_BF16>(raw[cb][s][i] & 0xffffu) * mul) |
+                               to16<false>(low_of<IS_BF16>(raw[cb][s][i]) * mul) << 16;
+            q[cb][s][i] = w;
+            (i & 1 ? sum1 : sum0) += from16<false>(w & 0xffffu) + from16<false>(w >> 16);
+          }
+        sum0 += __shfl_xor(sum0, 16);
+        sum0 += __shfl_xor(sum0, 32);
+        sum1 += __shfl_xor(sum1, 16);
+        sum1 += __shfl_xor(sum1, 32);
+        qsum[cb][g] = sum0 + sum1;
+        const float c = -1024.f * sum0 - 64.f * sum1;
+        c0[cb][g] = f32x4{c, c, c, c};
+      }
     }
-  }
-  if (a.splits > 1 && start >= end) return;
+  };
 
   float m[CB], l[CB], corr[CB][NG], vs[NG];
   f32x4 o[CB][NT];
@@ -212,7 +223,7 @@ __global__ __launch_bounds__(256, CB == 1 ? 2 : 1) void kv4_attn_kernel(AttnArgs
 
   const int* table = block_table + (long long)b * a.table_stride;
   const int last_tile = (end - 1) >> 4;
-  auto lookup = [&](int n0) -> Where {
+  auto lookup = [&](int n0) INLINE -> Where {
     Where w;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -229,7 +240,7 @@ __global__ __launch_bounds__(256, CB == 1 ? 2 : 1) void kv4_attn_kernel(AttnArgs
   const uint32_t k_lane = li * (D / 2) + lg * (D / 8), v_lane = lg * (2 * D) + li * (D / 8);
   const uint32_t* p_lane = (lane < 32 ? a.c.k_params : a.c.v_params) + li;      // lane: token lane & 31 of K or V
   uint32_t(*const params)[NG][32] = s_params[wave];
-  auto load = [&](const Where& w, Raw<D, NG>& r) {
+  auto load = [&](const Where& w, Raw<D, NG>& r) INLINE {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       load_words(r.k[t], a.c.k_codes + (w.row0[t] + w.off[t]) * (D / 2), k_lane);
@@ -240,14 +251,17 @@ __global__ __launch_bounds__(256, CB == 1 ? 2 : 1) void kv4_attn_kernel(AttnArgs
 #pragma unroll
     for (int g = 0; g < NG; ++g) r.params[g] = p[(long long)g * a.c.page_size];
   };
-  auto compute = [&](int n0, bool there0, bool there1, const Raw<D, NG>& r) {
-    const bool masked = n0 + 32 > min(full, end) || !there0 || !there1;
+  // CAREFUL: the block has tokens that are not there or not seen by every column, the scores are capped, or V's scales are
+  // brought near 1.  Without it the block is straight code but for the one branch on the references; false: nothing has been
+  // done, the block needs care.
+  auto compute_as = [&](auto careful, int n0, bool there0, bool there1, const Raw<D, NG>& r) INLINE -> bool {
+    constexpr bool CAREFUL = decltype(careful)::value;
     // ---- the block's widest V scale; the parameters of tokens that are not there may hold anything
     uint32_t param[NG];
     float widest = 0x1p-20f;
 #pragma unroll
     for (int g = 0; g < NG; ++g) param[g] = r.params[g];
-    if (masked) {
+    if (CAREFUL) {
       const bool live = (lane & 16 ? there1 : there0) && n0 + (lane & 31) < end;
 #pragma unroll
       for (int g = 0; g < NG; ++g) param[g] = live ? param[g] : 0u;
@@ -255,7 +269,7 @@ __global__ __launch_bounds__(256, CB == 1 ? 2 : 1) void kv4_attn_kernel(AttnArgs
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       params[lane >> 5][g][lane & 31] = param[g];
-      widest = fmaxf(widest, scale_of<IS_BF16>(param[g]) * vs[g]);
+      widest = fmaxf(widest, CAREFUL ? scale_of<IS_BF16>(param[g]) * vs[g] : scale_of<IS_BF16>(param[g]));
     }
     widest = max_upper_half(widest);
     // ---- scores of token n0 + 16 t + 4 lg + i, column li of each block: sum(q value), still to be times qk
@@ -267,7 +281,7 @@ __global__ __launch_bounds__(256, CB == 1 ? 2 : 1) void kv4_attn_kernel(AttnArgs
       for (int g = 0; g < NG; ++g) {
         const u32x4 kp = *(const u32x4*)&params[0][g][16 * t + 4 * lg];
 #pragma unroll
-        for (int cb = 0; cb < CB; ++cb) acc[cb] = f32x4{c0[cb][g], c0[cb][g], c0[cb][g], c0[cb][g]};
+        for (int cb = 0; cb < CB; ++cb) acc[cb] = c0[cb][g];
 #pragma unroll
         for (int s = g * GS; s < (g + 1) * GS; ++s) {
           const uint32_t w = r.k[t][s], w8 = w >> 8;
@@ -286,7 +300,7 @@ __global__ __launch_bounds__(256, CB == 1 ? 2 : 1) void kv4_attn_kernel(AttnArgs
         }
       }
     }
-    if (a.soft_cap > 0.f) {
+    if (CAREFUL && a.soft_cap > 0.f) {
 #pragma unroll
       for (int cb = 0; cb < CB; ++cb)
 #pragma unroll
@@ -298,8 +312,8 @@ __global__ __launch_bounds__(256, CB == 1 ? 2 : 1) void kv4_attn_kernel(AttnArgs
     float x_mul[CB];
     uint32_t seen[CB];
 #pragma unroll
-    for (int cb = 0; cb < CB; ++cb) x_mul[cb] = a.soft_cap > 0.f ? 1.f : qk[cb], seen[cb] = 255u;
-    if (masked) {
+    for (int cb = 0; cb < CB; ++cb) x_mul[cb] = CAREFUL && a.soft_cap > 0.f ? 1.f : qk[cb], seen[cb] = 255u;
+    if (CAREFUL) {
 #pragma unroll
       for (int cb = 0; cb < CB; ++cb)
 #pragma unroll
@@ -324,21 +338,31 @@ __global__ __launch_bounds__(256, CB == 1 ? 2 : 1) void kv4_attn_kernel(AttnArgs
       // scales far from 1 are brought there by a power of two per group, the same for all columns
       float ratio[NG];
       bool off = false;
+      if (!CAREFUL) {
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          const float w = max_upper_half(fmaxf(0.f, scale_of<IS_BF16>(param[g])));
+          off |= w > WIDE || (w > 0.f && w < NARROW);
+        }
+        if (off) return false;
+      }
       widest = 0x1p-20f;
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
+        ratio[g] = 1.f;
         const float w = max_upper_half(fmaxf(0.f, scale_of<IS_BF16>(param[g]) * vs[g]));
-        int e = 0;
-        if (w > 0x1p3f || (w > 0.f && w < 0x1p-9f)) e = (int)(__builtin_bit_cast(uint32_t, w) >> 23) - 127;
-        e = min(max(e, -60), 60);             // (what is further off takes several blocks to arrive)
-        const int have = (int)(__builtin_bit_cast(uint32_t, vs[g]) >> 23) - 127;
-        e = min(max(e, have - 120), have + 120);
-        ratio[g] = __builtin_bit_cast(float, (uint32_t)(127 - e) << 23);
-        vs[g] *= ratio[g];
+        if (CAREFUL && (w > WIDE || (w > 0.f && w < NARROW))) {
+          const int have = (int)(__builtin_bit_cast(uint32_t, vs[g]) >> 23) - 127;
+          int e = (int)(__builtin_bit_cast(uint32_t, w) >> 23) - 127;
+          e = min(max(e, -60), 60);           // (what is further off takes several blocks to arrive)
+          e = min(max(e, have - 120), have + 120);
+          ratio[g] = __builtin_bit_cast(float, (uint32_t)(127 - e) << 23);
+          vs[g] *= ratio[g];
+        }
         off |= vs[g] != 1.f;
         widest = fmaxf(widest, w * ratio[g]);
       }
-      scaled = off;
+      scaled |= off;
       const float now = log2_fast(widest);
 #pragma unroll
       for (int cb = 0; cb < CB; ++cb) {
@@ -378,7 +402,7 @@ __global__ __launch_bounds__(256, CB == 1 ? 2 : 1) void kv4_attn_kernel(AttnArgs
           zc[4 * t + i] = __builtin_fmaf(8.f, sv[4 * t + i], low_of<IS_BF16>(vp[i]));
         }
       }
-      if (scaled) {
+      if (CAREFUL) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) sv[i] *= vs[g];
       }
@@ -390,7 +414,7 @@ __global__ __launch_bounds__(256, CB == 1 ? 2 : 1) void kv4_attn_kernel(AttnArgs
           float s2[2], c2[2];
 #pragma unroll
           for (int k = 0; k < 2; ++k) s2[k] = sc[cb][i + k] * sv[i + k], c2[k] = sc[cb][i + k] * zc[i + k];
-          if (masked) {                       // 0 times the NaN of a token that only other columns see
+          if (CAREFUL) {                      // 0 times the NaN of a token that only other columns see
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
               const bool see = seen[cb] >> (i + k) & 1;
@@ -429,29 +453,58 @@ __global__ __launch_bounds__(256, CB == 1 ? 2 : 1) void kv4_attn_kernel(AttnArgs
         }
       }
     }
+    return true;
   };
-
-  // a wave's blocks are 128 tokens apart: one is multiplied while the next is on its way and the pages of the one after
-  // that are looked up
+  // A wave's blocks are 128 tokens apart.  RING of them are in flight: while one is multiplied the next ones are on their way,
+  // and the pages of the one behind them are looked up.  The first ones start before Q is fetched.  Plain blocks first; from
+  // the first one that needs care on, all of them get it.
   int n0 = start + 32 * wave;
   if (n0 < end) {
-    Raw<D, NG> r0, r1;
-    Where w0 = lookup(n0), w1;
-    load(w0, r0);
-    w1 = lookup(n0 + 128);
+    constexpr int RING = D <= 128 && CB == 1 ? 3 : 2;
+    Raw<D, NG> ring[RING];
+    bool there[RING];
+#pragma unroll
+    for (int i = 0; i < RING - 1; ++i) {
+      const Where w = lookup(n0 + 128 * i);
+      load(w, ring[i]);
+      there[i] = w.there[0] && w.there[1];
+    }
+    there[RING - 1] = false;
+    Where ahead = lookup(n0 + 128 * (RING - 1));
+    prepare_q();
+    const int plain_end = a.soft_cap > 0.f ? 0 : min(full, end);
+    auto plain = [&](auto slot) INLINE -> bool {
+      constexpr int I = decltype(slot)::value, AHEAD = (I + RING - 1) % RING;
+      if (n0 + 32 > plain_end || !there[I]) return false;
+      load(ahead, ring[AHEAD]);               // (behind the last block: the last tile's page once more)
+      there[AHEAD] = ahead.there[0] && ahead.there[1];
+      ahead = lookup(n0 + 128 * RING);
+      if (!compute_as(std::false_type{}, n0, true, true, ring[I])) return false;
+      n0 += 128;
+      return true;
+    };
     for (;;) {
-      const bool a0 = w0.there[0], a1 = w0.there[1];
-      if (n0 + 128 < end) load(w1, r1);
-      w0 = lookup(n0 + 256);
-      compute(n0, a0, a1, r0);
-      n0 += 128;
-      if (n0 >= end) break;
-      const bool b0 = w1.there[0], b1 = w1.there[1];
-      if (n0 + 128 < end) load(w0, r0);
-      w1 = lookup(n0 + 256);
-      compute(n0, b0, b1, r1);
-      n0 += 128;
-      if (n0 >= end) break;
+      if (!plain(std::integral_constant<int, 0>{})) break;
+      if (!plain(std::integral_constant<int, 1>{})) break;
+      if constexpr (RING > 2) {
+        if (!plain(std::integral_constant<int, 2>{})) break;
+      }
+    }
+    if (n0 < end) {
+      Raw<D, NG> r, next;
+      Where w = lookup(n0);
+      load(w, r);
+      bool there0 = w.there[0], there1 = w.there[1];
+      w = lookup(n0 + 128);
+      for (;;) {
+        load(w, next);
+        const bool next0 = w.there[0], next1 = w.there[1];
+        w = lookup(n0 + 256);
+        compute_as(std::true_type{}, n0, there0, there1, r);
+        n0 += 128;
+        if (n0 >= end) break;
+        r = next, there0 = next0, there1 = next1;
+      }
     }
   }
 
@@ -522,40 +575,58 @@ __global__ __launch_bounds__(256, CB == 1 ? 2 : 1) void kv4_attn_kernel(AttnArgs
   }
 }
 
-// One workgroup merges the splits of one row; wave w takes splits w, w + 4, ...
+// One workgroup merges the splits of one row.  D / 4 lanes hold a split's sums, so 1024 / D splits are read at a time; eight
+// rounds of loads are issued before the first is used (64 splits of 128 channels: one trip to memory).
 template <bool IS_BF16, int D>
 __global__ __launch_bounds__(256) void kv4_merge_kernel(const float* __restrict__ partial, const float* __restrict__ lse, int splits,
                                                         void* __restrict__ out, int out_mode) {
-  constexpr int V = D / 64;             // channels of a lane
-  __shared__ float s_acc[4][D];
+  constexpr int LANES = D / 4, AT_ONCE = 256 / LANES, ROUNDS = 8;
+  __shared__ __attribute__((aligned(16))) float s_acc[AT_ONCE][D];
   const long long row = blockIdx.x;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, c4 = threadIdx.x % LANES, first = threadIdx.x / LANES;
   const float* l = lse + row * splits;
-  float top = -INFINITY;
-  for (int s = lane; s < splits; s += 64) top = fmaxf(top, l[s]);
+  const float* sums = partial + row * splits * D + c4 * 4;
+  f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+  float top = -INFINITY, sum = 0.f;
+  for (int s0 = 0; s0 < splits; s0 += AT_ONCE * ROUNDS) {
+    f32x4 v[ROUNDS];
+    float mine[ROUNDS];
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-  if (top == -INFINITY) top = 0.f;      // no split has a token (or what they have is NaN, which the weights keep)
-  float sum = 0.f;
-  for (int s = lane; s < splits; s += 64) sum += exp2_fast(l[s] - top);
+    for (int i = 0; i < ROUNDS; ++i) {
+      const int s = s0 + first + AT_ONCE * i;
+      v[i] = *(const f32x4*)(sums + (long long)min(s, splits - 1) * D);
+      mine[i] = s < splits ? l[s] : -INFINITY;
+    }
+    float peak = top;                     // over all of this pass's splits: every lane reads some of them
+    for (int s = s0 + lane; s < min(splits, s0 + AT_ONCE * ROUNDS); s += 64) peak = fmaxf(peak, l[s]);
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
-  float acc[V];
+    for (int o = 32; o > 0; o >>= 1) peak = fmaxf(peak, __shfl_xor(peak, o));
+    if (peak == -INFINITY) peak = 0.f;    // no split has a token (or what they have is NaN, which the weights keep)
+    const float f = exp2_fast(top - peak);
+    sum *= f;
+    acc *= f;
 #pragma unroll
-  for (int i = 0; i < V; ++i) acc[i] = 0.f;
-#pragma unroll 4
-  for (int s = wave; s < splits; s += 4) {
-    const float w = exp2_fast(l[s] - top);
-    const float* p = partial + (row * splits + s) * D + lane * V;
+    for (int i = 0; i < ROUNDS; ++i) {
+      const float w = exp2_fast(mine[i] - peak);
+      sum += w;
 #pragma unroll
-    for (int i = 0; i < V; ++i) acc[i] += w != 0.f ? w * p[i] : 0.f;     // (a split without tokens has written no sums)
+      for (int k = 0; k < 4; ++k) acc[k] += w != 0.f ? w * v[i][k] : 0.f;      // (a split without tokens has written no sums)
+    }
+    top = peak;
   }
-#pragma unroll
-  for (int i = 0; i < V; ++i) s_acc[wave][lane * V + i] = acc[i];
+  *(f32x4*)&s_acc[first][c4 * 4] = acc;
+  __shared__ float s_sum[AT_ONCE];
+  if (c4 == 0) s_sum[first] = sum;
   __syncthreads();
+  sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < AT_ONCE; ++i) sum += s_sum[i];
   const float inv = sum != 0.f ? 1.f / sum : 0.f;
   for (int c = threadIdx.x; c < D; c += 256) {
-    const float r = (s_acc[0][c] + s_acc[1][c] + s_acc[2][c] + s_acc[3][c]) * inv;
+    float r = 0.f;
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) r += s_acc[i][c];
+    r *= inv;
     if (out_mode == 2) ((float*)out)[row * (D + 1) + c] = r;
     else ((uint16_t*)out)[row * D + c] = to16<IS_BF16>(r);
   }

@@ -417,6 +417,7 @@ def gqa_fwd_kv4(q: torch.Tensor, cache: Int4KVCache, kv_lens: torch.Tensor, bloc
     _require(math.isfinite(soft_cap) and soft_cap >= 0, f"soft_cap must be 0 (off) or positive, got {soft_cap}")
     _require(kv_split == -1 or 1 <= kv_split <= 65535, f"kv_split must be -1 (automatic) or 1 .. 65535, got {kv_split}")
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    _require(math.isfinite(scale), f"scale must be finite, got {scale}")
     shape = (batch, S, Hq, D + 1) if return_lse else (batch, S, Hq, D)
     if not q.is_cuda:
         out, lse = attend_reference(q4, cache, kv_lens, block_table, scale, soft_cap, causal)
