@@ -16,6 +16,8 @@
 //   codes are stored, so neither side moves between lanes.
 // The running maximum is only raised (and the sums rescaled) when a score exceeds it by 2^8: P up to 256 costs nothing
 // in floating point, and the cross-lane maximum leaves the loop.
+#include <algorithm>
+
 #include "tdist/kv4.hpp"
 
 namespace {
@@ -32,13 +34,20 @@ struct AttnArgs {
   int table_stride, max_pages;
   int page_tiles;           // 16-token tiles of a page,
   uint32_t page_magic;      // and floor(2^32 / page_tiles) + 1 (0: one tile a page)
-  int batch, S, q_heads, splits, causal, out_mode;
+  int batch, S, q_heads, group, splits, causal, out_mode;
+  int first;                // of this launch's (column block, sequence) pairs
   float scale, soft_cap;
 };
 
 typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 
+#ifndef KV4_WAVES
+#define KV4_WAVES(D) (D <= 128 ? 2 : 1)
+#endif
+#ifndef KV4_RING
+#define KV4_RING(D, CB) (D <= 128 && CB == 1 ? 3 : 2)
+#endif
 #define INLINE __attribute__((always_inline))     // (lambdas: a call would put what they capture into memory)
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -102,7 +111,7 @@ __device__ __forceinline__ void load_words(uint32_t (&dst)[N], const uint8_t* ba
 
 // CB blocks of sixteen columns share what a wave unpacks.
 template <bool IS_BF16, int D, int G, int CB>
-__global__ __launch_bounds__(256, CB == 1 || D <= 128 ? 2 : 1) void kv4_attn_kernel(AttnArgs a, const int* __restrict__ block_table,
+__global__ __launch_bounds__(256, KV4_WAVES(D)) void kv4_attn_kernel(AttnArgs a, const int* __restrict__ block_table,
                                                                         const int* __restrict__ kv_len) {
   constexpr int KS = D / 32;            // MFMA steps over the head dim = dwords of a lane per K row
   constexpr int NT = D / 16;            // 16-channel tiles of V
@@ -117,25 +126,27 @@ __global__ __launch_bounds__(256, CB == 1 || D <= 128 ? 2 : 1) void kv4_attn_ker
   __shared__ __attribute__((aligned(16))) float s_o[4][16][DC + 4];
   __shared__ __attribute__((aligned(16))) uint32_t s_params[4][2][NG][32];
 
-  const int pairs = a.batch * a.c.kv_heads;
-  const int cblk = blockIdx.x / pairs, pair = blockIdx.x - cblk * pairs;    // (columns of one KV head: on the same XCD if pairs % 8 == 0)
-  const int b = pair / a.c.kv_heads, kvh = pair - b * a.c.kv_heads;
-  const int group = a.q_heads / a.c.kv_heads, columns = group * a.S;
+  const int kvh = blockIdx.x, split = blockIdx.y;       // (kv heads first: what shares a cache line's XCD shares its L2)
+  const int z = a.first + (int)blockIdx.z;
+  const int cblk = a.batch == 1 ? z : z / a.batch, b = z - cblk * a.batch;
+  const int group = a.group, columns = group * a.S;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, lg = lane >> 4;
   const int col0 = cblk * 16 * CB;
 
   // tokens: a column sees [0, limit), the workgroup's columns [0, len), none of them misses one below `full`
   const long long room = (long long)a.max_pages * a.c.page_size;
   const int L = (int)min((long long)max(kv_len[b], 0), room);
-  const int s_first = col0 / group, s_last = min(col0 + 16 * CB - 1, columns - 1) / group;
+  const bool one = a.S == 1;                  // (columns are heads: no division by a variable on the way to the first load)
+  const int s_first = one ? 0 : col0 / group, s_last = one ? 0 : min(col0 + 16 * CB - 1, columns - 1) / group;
   const int len = max(0, a.causal ? L - a.S + s_last + 1 : L);
   const int full = a.causal ? L - a.S + s_first + 1 : L;
-  const int per = ((len + a.splits - 1) / a.splits + 127) & ~127;
-  const int start = (int)min((long long)blockIdx.y * per, (long long)len), end = min(len, start + per);
+  const int per = a.splits == 1 ? len : ((len + a.splits - 1) / a.splits + 127) & ~127;
+  const int start = (int)min((long long)split * per, (long long)len), end = min(len, start + per);
   if (a.splits > 1 && start >= end) {         // (the merge does not look at the sums of a split without tokens)
     const int col = col0 + (int)threadIdx.x;
     if (threadIdx.x < 16 * CB && col < columns)
-      a.partial_lse[(((long long)b * a.S + col / group) * a.q_heads + kvh * group + col % group) * a.splits + blockIdx.y] = -INFINITY;
+      a.partial_lse[(((long long)b * a.S + (one ? 0 : col / group)) * a.q_heads + kvh * group + (one ? col : col % group)) * a.splits +
+                    split] = -INFINITY;
     return;
   }
 
@@ -145,15 +156,13 @@ __global__ __launch_bounds__(256, CB == 1 || D <= 128 ? 2 : 1) void kv4_attn_ker
   u32x4 q[CB][KS];
   float qsum[CB][NG], qk[CB];
   f32x4 c0[CB][NG];                           // what the accumulators start at
-  auto prepare_q = [&]() INLINE {
-    const float sign = a.scale < 0.f ? -1.f : 1.f;
-    const float lead = fabsf(a.soft_cap > 0.f ? a.scale / a.soft_cap : a.scale * LOG2E);
-    u32x4 raw[CB][KS];
+  u32x4 raw[CB][KS];
+  auto fetch_q = [&]() INLINE {
 #pragma unroll
     for (int cb = 0; cb < CB; ++cb) {
       const int col = col0 + cb * 16 + li;
       const bool col_ok = col < columns;
-      const int row_s = col_ok ? col / group : 0, head = kvh * group + (col_ok ? col - row_s * group : 0);
+      const int row_s = one || !col_ok ? 0 : col / group, head = kvh * group + (col_ok ? col - row_s * group : 0);
       limit[cb] = !col_ok ? 0 : a.causal ? L - a.S + row_s + 1 : L;
       const uint16_t* qp = a.q + b * a.q_sb + row_s * a.q_ss + head * a.q_sh + lg * 8;
 #pragma unroll
@@ -162,6 +171,10 @@ __global__ __launch_bounds__(256, CB == 1 || D <= 128 ? 2 : 1) void kv4_attn_ker
         if (col_ok) raw[cb][s] = *(const u32x4*)(qp + 32 * s);
       }
     }
+  };
+  auto prepare_q = [&]() INLINE {
+    const float sign = a.scale < 0.f ? -1.f : 1.f;
+    const float lead = fabsf(a.soft_cap > 0.f ? a.scale / a.soft_cap : a.scale * LOG2E);
 #pragma unroll
     for (int cb = 0; cb < CB; ++cb) {
       float mul = sign, back = 1.f;
@@ -456,11 +469,12 @@ __global__ __launch_bounds__(256, CB == 1 || D <= 128 ? 2 : 1) void kv4_attn_ker
     return true;
   };
   // A wave's blocks are 128 tokens apart.  RING of them are in flight: while one is multiplied the next ones are on their way,
-  // and the pages of the one behind them are looked up.  The first ones start before Q is fetched.  Plain blocks first; from
+  // and the pages of the one behind them are looked up.    Plain blocks first; from
   // the first one that needs care on, all of them get it.
   int n0 = start + 32 * wave;
   if (n0 < end) {
-    constexpr int RING = D <= 128 && CB == 1 ? 3 : 2;
+    fetch_q();
+    constexpr int RING = KV4_RING(D, CB);
     Raw<D, NG> ring[RING];
     bool there[RING];
 #pragma unroll
@@ -533,9 +547,9 @@ __global__ __launch_bounds__(256, CB == 1 || D <= 128 ? 2 : 1) void kv4_attn_ker
     }
     const float inv = l_all != 0.f ? 1.f / l_all : 0.f;
     const float lse = l_all != 0.f ? m_all + log2_fast(l_all) : -INFINITY;
-    const int ms = mcol / group, mh = kvh * group + (mcol - ms * group);
+    const int ms = one ? 0 : mcol / group, mh = kvh * group + (mcol - ms * group);
     const long long row = ((long long)b * a.S + ms) * a.q_heads + mh;
-    float* prow = a.partial + (row * a.splits + blockIdx.y) * D;
+    float* prow = a.partial + (row * a.splits + split) * D;
 #pragma unroll
     for (int d0 = 0; d0 < D; d0 += DC) {
       if (d0) __syncthreads();
@@ -569,7 +583,7 @@ __global__ __launch_bounds__(256, CB == 1 || D <= 128 ? 2 : 1) void kv4_attn_ker
       }
     }
     if (mcol < columns && part == 0) {
-      if (a.splits > 1) a.partial_lse[row * a.splits + blockIdx.y] = lse;
+      if (a.splits > 1) a.partial_lse[row * a.splits + split] = lse;
       else if (a.out_mode == 2) ((float*)a.out)[row * (D + 1) + D] = lse * LN2;
     }
   }
@@ -670,24 +684,28 @@ TDIST_API int tdist_kv4_attn(const void* k_codes, const void* v_codes, const voi
   TDIST_REQUIRE(q && table && kv_len && out, "null argument");
   TDIST_REQUIRE(((uintptr_t)q & 15) == 0 && ((uintptr_t)out & 7) == 0 && ((q_sb | q_ss | q_sh) & 7) == 0,
                 "q rows must keep 16-byte alignment");
-  const long long columns = (long long)(q_heads / kv_heads) * S, per_group = columns > 16 ? 2 : 1;
-  const long long blocks = (columns + 16 * per_group - 1) / (16 * per_group) * batch * kv_heads;
-  TDIST_REQUIRE(blocks < (1ll << 31) && (long long)batch * S * q_heads < (1ll << 31), "too many query rows");
+  const long long columns = (long long)(q_heads / kv_heads) * S, per_group = columns > 16 && head_dim <= 128 ? 2 : 1;
+  const long long blocks = (columns + 16 * per_group - 1) / (16 * per_group) * batch;
+  TDIST_REQUIRE(blocks < (1ll << 31) && columns < (1ll << 30) && (long long)batch * S * q_heads < (1ll << 31), "too many query rows");
   a.q = (const uint16_t*)q, a.partial = partial, a.out = out;
   a.page_tiles = page_size / 16;
   a.page_magic = a.page_tiles == 1 ? 0u : (uint32_t)((1ull << 32) / a.page_tiles) + 1u;
   a.partial_lse = partial ? partial + (long long)batch * S * q_heads * splits * head_dim : nullptr;
   a.q_sb = q_sb, a.q_ss = q_ss, a.q_sh = q_sh, a.table_stride = table_stride, a.max_pages = max_pages;
-  a.batch = batch, a.S = S, a.q_heads = q_heads, a.splits = splits, a.causal = causal, a.out_mode = out_mode;
+  a.batch = batch, a.S = S, a.q_heads = q_heads, a.group = q_heads / kv_heads, a.splits = splits, a.causal = causal, a.out_mode = out_mode;
   a.scale = scale, a.soft_cap = soft_cap;
   const bool ok = dispatch(dtype, head_dim, group, [&](auto bf, auto d, auto g) {
     auto launch = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, dim3((unsigned)blocks, splits), dim3(256), 0, (hipStream_t)stream, a, table, kv_len);
+      for (a.first = 0; a.first < blocks; a.first += 65535)       // (the limit of a grid's third dimension)
+        hipLaunchKernelGGL(kernel, dim3(kv_heads, splits, (unsigned)std::min(65535ll, blocks - a.first)), dim3(256), 0,
+                           (hipStream_t)stream, a, table, kv_len);
     };
     constexpr bool BF = decltype(bf)::value;
     constexpr int D = decltype(d)::value, G = decltype(g)::value;
-    if (per_group == 2) launch(kv4_attn_kernel<BF, D, G, 2>);
-    else launch(kv4_attn_kernel<BF, D, G, 1>);
+    if constexpr (D <= 128) {
+      if (per_group == 2) return launch(kv4_attn_kernel<BF, D, G, 2>);
+    }
+    launch(kv4_attn_kernel<BF, D, G, 1>);
   });
   TDIST_REQUIRE(ok, "head_dim 64 / 128 / 256 with groups of 32 / 64 / 128 channels (at most head_dim)");
   TDIST_HIP_TRY(hipGetLastError());
