@@ -274,3 +274,15 @@ def test_empty_calls():
     zero = torch.zeros(0, 3, 2, 64, dtype=torch.bfloat16)
     kv4.kv4_append(zero, zero, cache, int32([]), torch.zeros(0, 2, dtype=torch.int32))
     assert (cache.k_codes == 0).all()
+
+
+def test_argument_types_of_the_native_calls_match_the_sources():
+    import re
+
+    from triton_distributed_gh_amd import build
+
+    source = "".join((build.CSRC / "ops" / f).read_text() for f in ("kv4.hip", "kv4_attn.hip"))
+    for name, signature in kv4._SIGNATURES.items():
+        args = re.search(rf"TDIST_API int {name}\((.*?)\) \{{", source, re.S).group(1).split(",")
+        kinds = ["p" if "*" in a else "q" if "long long" in a else "f" if "float" in a else "i" for a in args]
+        assert "".join(kinds) == signature, name

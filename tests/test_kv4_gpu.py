@@ -61,7 +61,7 @@ def test_append_and_read_give_the_bits_of_the_cpu_path(D, group, dtype):
         assert torch.equal(a.isnan(), b.isnan()) and torch.equal(a.nan_to_num(0.0), b.nan_to_num(0.0))
 
 
-@pytest.mark.parametrize("S", [1, 2, 3, 4, 5, 17, 64])
+@pytest.mark.parametrize("S", [1, 2, 3, 4, 5, 17, 64, 65])
 def test_append_token_counts_and_strided_rows(S):
     gen = _gen(S)
     B, H, D, group, page = 2, 5, 128, 64, 16
@@ -84,6 +84,26 @@ def test_append_token_counts_and_strided_rows(S):
         kv4.kv4_append(there(k), there(v), gpu, offsets.cuda(), table.cuda())
         torch.cuda.synchronize()
         _same(cpu, gpu)
+
+
+@pytest.mark.parametrize("D,group,page", [(64, 32, 16), (128, 64, 48), (256, 128, 16)])
+def test_reads_that_start_anywhere(D, group, page):
+    """Sequences of 0 .. 70 rows that start at any token, in front of the first one and behind the last page too; more
+    sequences than a wave looks up at a time."""
+    gen = _gen(31)
+    B, H = 70, 2
+    cpu, table, _, _ = oracle.filled(gen, [96] * B, H, D, group, page)
+    lens = torch.randint(0, 71, (B,), generator=gen)
+    lens[3:9] = 0
+    starts = torch.randint(-5, 90, (B,), generator=gen).int()
+    cu = torch.cat([torch.zeros(1, dtype=torch.int32), lens.cumsum(0).int()])
+    total = int(cu[-1])
+    want = kv4.kv4_read(cpu, table, cu, total, starts=starts)
+    got = kv4.kv4_read(_to(cpu, "cuda"), table.cuda(), cu.cuda(), total, starts=starts.cuda())
+    some = kv4.kv4_read(_to(cpu, "cuda"), table.cuda(), cu.cuda(), total - 37, starts=starts.cuda())
+    torch.cuda.synchronize()
+    for a, b, c in zip(want, got, some):
+        assert torch.equal(a, b.cpu()) and torch.equal(a[:total - 37], c.cpu())
 
 
 def test_append_leaves_everything_else_alone():

@@ -8,27 +8,64 @@
 // row), D / 8 lanes on a row, so a group's minimum and maximum are G / 8 lanes' and stay inside a wave.
 // This file is compiled without fast-math: the code of a value next to a border is decided by IEEE arithmetic and is
 // the same on every path that writes a cache, the CPU's included.
+#include <algorithm>
+
 #include "tdist/kv4.hpp"
 
 namespace {
 
 using namespace tdist::kv4;
 
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
+
+// A wave works on a tile of TILE tokens in PASSES passes of ROWS rows of LANES lanes.
+template <int D>
+struct Tile {
+  static constexpr int LANES = D / 8, ROWS = 64 / LANES, TILE = D == 256 ? 8 : 16, PASSES = TILE / ROWS;
+};
+
 template <bool IS_BF16>
-__device__ __forceinline__ void unpack_row8(const uint4& v, float (&x)[8]) {
-  const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+__device__ __forceinline__ void unpack_row8(const u32x4& v, float (&x)[8]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    x[2 * i] = from16<IS_BF16>(u[i] & 0xffffu);
-    x[2 * i + 1] = low_of<IS_BF16>(u[i]);
+    x[2 * i] = from16<IS_BF16>(v[i] & 0xffffu);
+    x[2 * i + 1] = low_of<IS_BF16>(v[i]);
   }
 }
 template <bool IS_BF16>
-__device__ __forceinline__ uint4 pack_row8(const float (&x)[8]) {
-  uint32_t u[4];
+__device__ __forceinline__ u32x4 pack_row8(const float (&x)[8]) {
+  u32x4 u;
 #pragma unroll
   for (int i = 0; i < 4; ++i) u[i] = to16<IS_BF16>(x[2 * i]) | to16<IS_BF16>(x[2 * i + 1]) << 16;
-  return uint4{u[0], u[1], u[2], u[3]};
+  return u;
+}
+
+// Lane exchanges inside a row of sixteen without LDS.
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xf, 0xf, true);
+}
+constexpr int XOR1 = 0xb1, XOR2 = 0x4e, XOR3 = 0x1b, XOR7 = 0x141, XOR15 = 0x140, ROR8 = 0x128;
+__device__ __forceinline__ uint32_t xor4(uint32_t v) { return dpp<XOR7>(dpp<XOR3>(v)); }
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+  return __builtin_bit_cast(float, dpp<CTRL>(__builtin_bit_cast(uint32_t, v)));
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp(double v) {
+  const uint2 u = __builtin_bit_cast(uint2, v);
+  return __builtin_bit_cast(double, uint2{dpp<CTRL>(u.x), dpp<CTRL>(u.y)});
+}
+// op over N neighbouring lanes (N = 4 .. 32); every lane gets the result.  (Once fours agree, the mirrored eight is one, and
+// so on.)
+template <int N, class T, class Op>
+__device__ __forceinline__ T over_lanes(T v, Op op) {
+  v = op(v, dpp<XOR1>(v));
+  v = op(v, dpp<XOR2>(v));
+  if constexpr (N >= 8) v = op(v, dpp<XOR7>(v));
+  if constexpr (N >= 16) v = op(v, dpp<XOR15>(v));
+  if constexpr (N >= 32) v = op(v, __shfl_xor(v, 16));
+  return v;
 }
 
 // Codes of the lane's eight channels and the parameter dword of their group.
@@ -39,15 +76,12 @@ __device__ __forceinline__ uint4 pack_row8(const float (&x)[8]) {
 // a division's ten; scales so small or large that an intermediate could leave the normal range take the division.
 template <bool IS_BF16, int G>
 __device__ __forceinline__ uint32_t quantise8(const float (&x)[8], uint32_t (&code)[8]) {
-  float lo = x[0], hi = x[0], odd = x[0] * 0.f;       // odd: NaN if any value is an infinity or a NaN
+  float lo = x[0], hi = x[0], odd = 0.f;              // odd: NaN if any value is an infinity or a NaN
 #pragma unroll
-  for (int e = 1; e < 8; ++e) lo = fminf(lo, x[e]), hi = fmaxf(hi, x[e]), odd += x[e] * 0.f;
-#pragma unroll
-  for (int o = 1; o < G / 8; o <<= 1) {
-    lo = fminf(lo, __shfl_xor(lo, o));
-    hi = fmaxf(hi, __shfl_xor(hi, o));
-    odd += __shfl_xor(odd, o);
-  }
+  for (int e = 0; e < 8; ++e) lo = fminf(lo, x[e]), hi = fmaxf(hi, x[e]), odd = __builtin_fmaf(x[e], 0.f, odd);
+  lo = over_lanes<G / 8>(lo, [](float a, float b) { return fminf(a, b); });
+  hi = over_lanes<G / 8>(hi, [](float a, float b) { return fmaxf(a, b); });
+  odd = over_lanes<G / 8>(odd, [](float a, float b) { return a + b; });
   const float range = (hi - lo) + odd;
   const uint32_t s16 = range < INFINITY ? to16<IS_BF16>(range / 15.f) : to16<IS_BF16>(NAN);
   const float s = from16<IS_BF16>(s16);
@@ -67,73 +101,105 @@ __device__ __forceinline__ uint32_t quantise8(const float (&x)[8], uint32_t (&co
   return s16 | to16<IS_BF16>(lo) << 16;               // (lo is one of the row's 16-bit values)
 }
 
-// Quantises a row held eight channels a lane (lane l8 of D / 8) and writes it to (page, head, token `off` of the page).
-// Every lane of the wave calls it; rows that go nowhere have page < 0.
-template <bool IS_BF16, int D, int G, bool IS_V>
-__device__ __forceinline__ void store_row(const Cache& c, const float (&x)[8], int l8, int page, int head, int off) {
-  uint32_t code[8];
-  const uint32_t param = quantise8<IS_BF16, G>(x, code);
-  const long long row0 = ((long long)page * c.kv_heads + head) * c.page_size;      // first token of (page, head)
-  if constexpr (!IS_V) {
-    if (page < 0) return;
-    uint32_t w = 0;
+// Quantises a tile of rows of one head and writes rows lo .. hi - 1 of it.  `at`: the place of the tile's first token (a
+// multiple of TILE, so all of them are in one page).  rows(p, x): the lane's eight channels of pass p.  `stage`: 8 D bytes of LDS
+// of the wave's own.
+//
+// K rows are runs of their own.  A 16-byte run of V is one channel lane's four tokens: a whole tile is brought into that
+// order in LDS and leaves as 16-byte stores (2-byte stores to eight places: 42 us instead of @@ for 37 MB of rows); the
+// first and last tile of a sequence, whose runs are shared with other calls, are written unit by unit.
+template <bool IS_BF16, int D, int G, bool IS_V, class Rows>
+__device__ __forceinline__ void store_tile(const Cache& c, const Place& at, int head, int lo, int hi, char* stage, Rows&& rows) {
+  using T = Tile<D>;
+  const int lane = threadIdx.x & 63, l8 = lane % T::LANES;
+  const long long row0 = ((long long)at.page * c.kv_heads + head) * c.page_size;   // first token of (page, head)
+  const bool whole = lo <= 0 && hi >= T::TILE;
+  uint8_t* const vbase = c.v_codes + (row0 + at.off) * (D / 2);
 #pragma unroll
-    for (int n = 0; n < 4; ++n) w |= code[2 * n] << (4 * n) | code[2 * n + 1] << (16 + 4 * n);
-    const int word = (l8 & 3) * (D / 32) + (l8 >> 2);
-    *(uint32_t*)(c.k_codes + (row0 + off) * (D / 2) + word * 4) = w;
-  } else {
-    // the four lanes n = 0 .. 3 of a unit hold its four 16-channel tiles: two steps of exchange, in each of which a lane
-    // keeps half of what it has and gives the other half away, leave each lane two whole units
-    const int n = (l8 >> 1) & 3;
-    uint32_t u[4];
+  for (int p = 0; p < T::PASSES; ++p) {
+    if (hi <= p * T::ROWS || lo >= (p + 1) * T::ROWS) continue;                    // (uniform)
+    const int i = p * T::ROWS + lane / T::LANES;
+    const bool live = i >= lo && i < hi;
+    float x[8];
+    rows(p, x);
+    uint32_t code[8];
+    const uint32_t param = quantise8<IS_BF16, G>(x, code);
+    if constexpr (!IS_V) {
+      uint32_t w = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) u[i] = (code[2 * i] | code[2 * i + 1] << 16) << (4 * n);
-    const bool up1 = n & 1, up2 = n & 2;
-    const uint32_t a0 = (up1 ? u[2] : u[0]) | __shfl_xor(up1 ? u[0] : u[2], 2);
-    const uint32_t a1 = (up1 ? u[3] : u[1]) | __shfl_xor(up1 ? u[1] : u[3], 2);
-    const uint32_t b = (up2 ? a1 : a0) | __shfl_xor(up2 ? a0 : a1, 4);
-    if (page < 0) return;
-    const int ch = (l8 & 1) * 8 + (up1 ? 4 : 0) + (up2 ? 2 : 0);                    // this lane's units: channels ch, ch + 1
-    uint8_t* p = c.v_codes + row0 * (D / 2) + (long long)(off >> 2) * (2 * D) + (l8 >> 3) * 8 + (off & 3) * 2;
-    *(uint16_t*)(p + ch * (D / 8)) = (uint16_t)b;
-    *(uint16_t*)(p + (ch + 1) * (D / 8)) = (uint16_t)(b >> 16);
+      for (int n = 0; n < 4; ++n) w |= code[2 * n] << (4 * n) | code[2 * n + 1] << (16 + 4 * n);
+      const int word = (l8 & 3) * (D / 32) + (l8 >> 2);
+      if (live) *(uint32_t*)(c.k_codes + (row0 + at.off + i) * (D / 2) + word * 4) = w;
+    } else {
+      // the four lanes n = 0 .. 3 of a unit hold its four 16-channel tiles: two steps of exchange, in each of which a lane
+      // keeps half of what it has and gives the other half away, leave each lane two whole units
+      const int n = (l8 >> 1) & 3;
+      uint32_t u[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) u[k] = (code[2 * k] | code[2 * k + 1] << 16) << (4 * n);
+      const bool up1 = n & 1, up2 = n & 2;
+      const uint32_t a0 = (up1 ? u[2] : u[0]) | dpp<XOR2>(up1 ? u[0] : u[2]);
+      const uint32_t a1 = (up1 ? u[3] : u[1]) | dpp<XOR2>(up1 ? u[1] : u[3]);
+      const uint32_t b = (up2 ? a1 : a0) | xor4(up2 ? a0 : a1);
+      const int ch = (l8 & 1) * 8 + (up1 ? 4 : 0) + (up2 ? 2 : 0);                  // this lane's units: channels ch, ch + 1
+      const int to = (i >> 2) * (2 * D) + ch * (D / 8) + (l8 >> 3) * 8 + (i & 3) * 2;
+      if (whole) {
+        *(uint16_t*)(stage + to) = (uint16_t)b;
+        *(uint16_t*)(stage + to + D / 8) = (uint16_t)(b >> 16);
+      } else if (live) {
+        *(uint16_t*)(vbase + to) = (uint16_t)b;
+        *(uint16_t*)(vbase + to + D / 8) = (uint16_t)(b >> 16);
+      }
+    }
+    if (live && l8 % (G / 8) == 0) {
+      uint32_t* params = IS_V ? c.v_params : c.k_params;
+      params[row0 * (D / G) + (long long)(l8 / (G / 8)) * c.page_size + at.off + i] = param;
+    }
   }
-  if (l8 % (G / 8) == 0) {
-    uint32_t* params = IS_V ? c.v_params : c.k_params;
-    params[row0 * (D / G) + (long long)(l8 / (G / 8)) * c.page_size + off] = param;
+  if constexpr (IS_V) {
+    if (whole && lane * 16 < T::TILE * (D / 2)) *(u32x4*)(vbase + lane * 16) = *(const u32x4*)(stage + lane * 16);
   }
 }
 
-// grid: (tiles of tokens, Hkv heads of K then Hkv of V, batch)
+// grid: (tiles of tokens, Hkv heads of K then Hkv of V, batch), a wave per tile.  Tiles are aligned in the sequence.
 template <bool IS_BF16, int D, int G>
 __global__ __launch_bounds__(256) void kv4_append_kernel(Cache c, const uint16_t* __restrict__ k, const uint16_t* __restrict__ v,
                                                          long long k_sb, long long k_ss, long long k_sh, long long v_sb,
                                                          long long v_ss, long long v_sh, const int* __restrict__ kv_offset,
                                                          const int* __restrict__ new_lens, const int* __restrict__ table,
                                                          int table_stride, int max_pages, int S) {
-  constexpr int LANES = D / 8;
-  const int b = blockIdx.z, l8 = threadIdx.x % LANES;
-  const int s = blockIdx.x * (blockDim.x / LANES) + threadIdx.x / LANES;
+  using T = Tile<D>;
+  __shared__ __attribute__((aligned(16))) char stage[4][T::TILE * D / 2];
+  const int b = blockIdx.z, lane = threadIdx.x & 63, l8 = lane % T::LANES;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const bool is_v = (int)blockIdx.y >= c.kv_heads;
   const int head = blockIdx.y - (is_v ? c.kv_heads : 0);
-  const int count = new_lens ? min(new_lens[b], S) : S;
-  const bool live = s < count;
-  const long long pos = (long long)kv_offset[b] + s;
-  const Place at = place_of(c, table + (long long)b * table_stride, live ? pos : -1, max_pages);
-  float x[8];
-  uint4 raw = uint4{0, 0, 0, 0};
-  if (live)
-    raw = *(const uint4*)((is_v ? v + b * v_sb + s * v_ss + head * v_sh : k + b * k_sb + s * k_ss + head * k_sh) + l8 * 8);
-  unpack_row8<IS_BF16>(raw, x);
+  const int offset = kv_offset[b], count = new_lens ? min(new_lens[b], S) : S;
+  const long long s0 = (long long)(blockIdx.x * (blockDim.x >> 6) + wave) * T::TILE - (offset & (T::TILE - 1));   // the tile's first row
+  if (s0 >= count) return;
+  const Place at = place_of(c, table + (long long)b * table_stride, offset + s0, max_pages);
+  if (at.page < 0) return;
+  const int lo = s0 < 0 ? (int)-s0 : 0, hi = (int)min((long long)T::TILE, count - s0);
+  const uint16_t* src = is_v ? v + b * v_sb + head * v_sh : k + b * k_sb + head * k_sh;
+  const long long ss = is_v ? v_ss : k_ss;
+  u32x4 raw[T::PASSES];
+#pragma unroll
+  for (int p = 0; p < T::PASSES; ++p) {
+    const int i = p * T::ROWS + lane / T::LANES;
+    raw[p] = u32x4{0, 0, 0, 0};
+    if (i >= lo && i < hi) raw[p] = *(const u32x4*)(src + (s0 + i) * ss + l8 * 8);
+  }
+  auto rows = [&](int p, float (&x)[8]) { unpack_row8<IS_BF16>(raw[p], x); };
   if (is_v) {
-    store_row<IS_BF16, D, G, true>(c, x, l8, at.page, head, at.off);
+    store_tile<IS_BF16, D, G, true>(c, at, head, lo, hi, stage[wave], rows);
   } else {
-    store_row<IS_BF16, D, G, false>(c, x, l8, at.page, head, at.off);
+    store_tile<IS_BF16, D, G, false>(c, at, head, lo, hi, stage[wave], rows);
   }
 }
 
-// grid: (tiles of tokens, Hq heads of q, Hkv of K, Hkv of V, batch).  The norm's mean square and the rotation are taken in
-// 64 bits, so that a stored code does not depend on the order of a sum.
+// grid: (tiles of tokens, blocks of `heads_each` of the Hq + 2 Hkv heads, batch), a wave per tile and block: the rotation's
+// factors of a tile are fetched once for the heads of the block.  The norm's mean square and the rotation are taken in 64 bits,
+// so that a stored code does not depend on the order of a sum.
 template <int D, int G>
 __global__ __launch_bounds__(256) void kv4_qkv_prep_kernel(Cache c, const uint16_t* __restrict__ qkv, long long q_sb,
                                                            long long q_ss, const uint16_t* __restrict__ q_w,
@@ -143,113 +209,225 @@ __global__ __launch_bounds__(256) void kv4_qkv_prep_kernel(Cache c, const uint16
                                                            long long rope_rows, uint16_t* __restrict__ q_out,
                                                            const int* __restrict__ kv_offset, int* __restrict__ total_out,
                                                            const int* __restrict__ table, int table_stride, int max_pages,
-                                                           int S, int q_heads) {
-  constexpr int LANES = D / 8;
-  const int b = blockIdx.z, l8 = threadIdx.x % LANES;
-  const int s = blockIdx.x * (blockDim.x / LANES) + threadIdx.x / LANES;
-  const int head = blockIdx.y;
+                                                           int S, int q_heads, int heads_each) {
+  using T = Tile<D>;
+  __shared__ __attribute__((aligned(16))) char stage[4][T::TILE * D / 2];
+  const int b = blockIdx.z, lane = threadIdx.x & 63, l8 = lane % T::LANES;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int offset = kv_offset[b];
-  if (head == 0 && s == 0 && l8 == 0) total_out[b] = offset + S;
-  const bool live = s < S, is_q = head < q_heads, is_v = head >= q_heads + c.kv_heads;
-  const long long pos = (long long)offset + s;
-  const Place at = place_of(c, table + (long long)b * table_stride, live && !is_q ? pos : -1, max_pages);
-  float x[8];
-  uint4 raw = uint4{0, 0, 0, 0};
-  if (live) raw = *(const uint4*)(qkv + b * q_sb + s * q_ss + (long long)head * D + l8 * 8);
-  unpack_row8<true>(raw, x);
-  if (is_v) {
-    store_row<true, D, G, true>(c, x, l8, at.page, head - q_heads - c.kv_heads, at.off);
-    return;
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) total_out[b] = offset + S;
+  const long long s0 = (long long)(blockIdx.x * (blockDim.x >> 6) + wave) * T::TILE - (offset & (T::TILE - 1));
+  if (s0 >= S) return;
+  const int lo = s0 < 0 ? (int)-s0 : 0, hi = (int)min((long long)T::TILE, S - s0);
+  const int head0 = blockIdx.y * heads_each, heads = q_heads + 2 * c.kv_heads, head1 = min(head0 + heads_each, heads);
+  Place at = Place{-1, 0};
+  if (head1 > q_heads) at = place_of(c, table + (long long)b * table_stride, offset + s0, max_pages);
+  float cs[T::PASSES][8], sn[T::PASSES][8];
+  if (head0 < q_heads + c.kv_heads) {
+#pragma unroll
+    for (int p = 0; p < T::PASSES; ++p) {
+      const int i = p * T::ROWS + lane / T::LANES;
+      long long pos = i >= lo && i < hi ? positions[(long long)b * S + s0 + i] : 0;
+      pos = pos < 0 ? 0 : pos < rope_rows ? pos : rope_rows - 1;
+      const long long from = pos * (D / 2) + (l8 * 8) % (D / 2);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) cs[p][e] = cos_t[from + e], sn[p][e] = sin_t[from + e];
+    }
   }
-  const uint16_t* w = is_q ? q_w : k_w;
-  if (w) {
-    double ss = 0.;
+  const uint16_t* src = qkv + b * q_sb + l8 * 8;
+  auto fetch = [&](int head, u32x4 (&raw)[T::PASSES]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) ss += (double)x[e] * x[e];
-#pragma unroll
-    for (int o = 1; o < LANES; o <<= 1) ss += __shfl_xor(ss, o);
-    const float inv = (float)(1. / __builtin_sqrt(ss / D + (double)(is_q ? q_eps : k_eps)));
+    for (int p = 0; p < T::PASSES; ++p) {
+      const int i = p * T::ROWS + lane / T::LANES;
+      raw[p] = u32x4{0, 0, 0, 0};
+      if (i >= lo && i < hi) raw[p] = *(const u32x4*)(src + (s0 + i) * q_ss + (long long)head * D);
+    }
+  };
+  u32x4 raw[T::PASSES], next[T::PASSES];
+  fetch(head0, raw);
+  for (int head = head0; head < head1; ++head) {
+    if (head + 1 < head1) fetch(head + 1, next);
+    const bool is_q = head < q_heads, is_v = head >= q_heads + c.kv_heads;
+    const uint16_t* w = is_q ? q_w : is_v ? nullptr : k_w;
     float g[8];
-    unpack_row8<true>(*(const uint4*)(w + l8 * 8), g);
+    if (w) unpack_row8<true>(*(const u32x4*)(w + l8 * 8), g);
+    auto rows = [&](int p, float (&x)[8]) __attribute__((always_inline)) {
+      unpack_row8<true>(raw[p], x);
+      if (is_v) return;
+      if (w) {
+        double ss = 0.;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = from16<true>(to16<true>(x[e] * inv * g[e]));
-  }
-  {
-    // pairs (i, i + D / 2) are the same element of lanes l8 and l8 ^ (D / 16)
-    long long p = live ? positions[(long long)b * S + s] : 0;
-    p = p < 0 ? 0 : p < rope_rows ? p : rope_rows - 1;
-    const int i0 = (l8 * 8) % (D / 2);
-    const float* cs = cos_t + p * (D / 2) + i0;
-    const float* sn = sin_t + p * (D / 2) + i0;
-    const double sign = l8 < LANES / 2 ? -1. : 1.;
-    float y[8];
+        for (int e = 0; e < 8; ++e) ss = __builtin_fma((double)x[e], (double)x[e], ss);
+        ss = over_lanes<T::LANES>(ss, [](double a, double b) { return a + b; });
+        const float inv = (float)(1. / __builtin_sqrt(ss / D + (double)(is_q ? q_eps : k_eps)));
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float other = __shfl_xor(x[e], LANES / 2);
-      y[e] = (float)((double)x[e] * cs[e] + sign * other * sn[e]);
-      asm volatile("" : "+v"(y[e]));          // 64 -> 32 -> 16 bits as two roundings, which the compiler would merge
+        for (int e = 0; e < 8; ++e) x[e] = from16<true>(to16<true>(x[e] * inv * g[e]));
+      }
+      // pairs (i, i + D / 2) are the same element of lanes l8 and l8 ^ (D / 16)
+      const double sign = l8 < T::LANES / 2 ? -1. : 1.;
+      float y[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float other;
+        if constexpr (D == 128) {
+          other = dpp<ROR8>(x[e]);
+        } else if constexpr (D == 64) {
+          other = dpp<XOR7>(dpp<XOR3>(x[e]));
+        } else {
+          other = __shfl_xor(x[e], 16);
+        }
+        y[e] = (float)__builtin_fma((double)x[e], (double)cs[p][e], sign * other * sn[p][e]);
+        asm volatile("" : "+v"(y[e]));          // 64 -> 32 -> 16 bits as two roundings, which the compiler would merge
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = from16<true>(to16<true>(y[e]));
+    };
+    if (is_q) {
+#pragma unroll
+      for (int p = 0; p < T::PASSES; ++p) {
+        if (hi <= p * T::ROWS || lo >= (p + 1) * T::ROWS) continue;
+        const int i = p * T::ROWS + lane / T::LANES;
+        float x[8];
+        rows(p, x);
+        if (i >= lo && i < hi) *(u32x4*)(q_out + (((long long)b * S + s0 + i) * q_heads + head) * D + l8 * 8) = pack_row8<true>(x);
+      }
+    } else if (at.page >= 0) {
+      if (is_v) {
+        store_tile<true, D, G, true>(c, at, head - q_heads - c.kv_heads, lo, hi, stage[wave], rows);
+      } else {
+        store_tile<true, D, G, false>(c, at, head - q_heads, lo, hi, stage[wave], rows);
+      }
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = from16<true>(to16<true>(y[e]));
+    for (int p = 0; p < T::PASSES; ++p) raw[p] = next[p];
   }
-  if (is_q) {
-    if (live) *(uint4*)(q_out + (((long long)b * S + s) * q_heads + head) * D + l8 * 8) = pack_row8<true>(x);
-    return;
-  }
-  store_row<true, D, G, false>(c, x, l8, at.page, head - q_heads, at.off);
 }
 
-// grid: (tiles of output rows, Hkv heads of K then Hkv of V).  Row r belongs to the sequence b with cu[b] <= r < cu[b + 1].
+// Row r of the output belongs to the sequence b with cu[b] <= r < cu[b + 1].  A wave takes TILE rows of one head of K or V,
+// sequence by sequence; workgroups with neighbouring numbers take the heads of the same rows, which are neighbours in the
+// output.  V's runs of four tokens are turned into rows in LDS.
 template <bool IS_BF16, int D, int G>
 __global__ __launch_bounds__(256) void kv4_read_kernel(Cache c, const int* __restrict__ table, int table_stride, int max_pages,
                                                        const int* __restrict__ cu, const int* __restrict__ starts, int batch,
                                                        long long total, uint16_t* __restrict__ k_out,
                                                        uint16_t* __restrict__ v_out, long long k_st, long long k_sh,
                                                        long long v_st, long long v_sh) {
-  constexpr int LANES = D / 8;
+  using T = Tile<D>;
   constexpr float MOST = IS_BF16 ? 0x1.fep127f : 65504.f;
-  const int l8 = threadIdx.x % LANES;
-  const long long r = (long long)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
-  const bool is_v = (int)blockIdx.y >= c.kv_heads;
-  const int head = blockIdx.y - (is_v ? c.kv_heads : 0);
+  constexpr int QUADS = T::TILE / 4 + 1;        // of an unaligned tile
+  constexpr int ROW = D / 2 + 16;               // bytes of a token's units in LDS, and a gap so that neighbours meet other banks
+  __shared__ __attribute__((aligned(16))) char stages[4][QUADS * 4 * ROW];
+  const int lane = threadIdx.x & 63, l8 = lane % T::LANES;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  char* const stage = stages[wave];
+  const uint32_t tile = blockIdx.x / (2u * c.kv_heads), which = blockIdx.x - tile * 2u * c.kv_heads;
+  const bool is_v = (int)which >= c.kv_heads;
+  const int head = which - (is_v ? c.kv_heads : 0);
   const long long end = min(total, (long long)cu[batch]);
-  if (r >= end || r < cu[0]) return;
-  int b = 0, top = batch;                 // cu[b] <= r < cu[top]
-  while (top - b > 1) {
-    const int mid = (b + top) >> 1;
-    if (cu[mid] <= r) b = mid; else top = mid;
+  long long r = max(((long long)tile * (blockDim.x >> 6) + wave) * T::TILE, (long long)cu[0]);
+  const long long stop = min(((long long)tile * (blockDim.x >> 6) + wave + 1) * T::TILE, end);
+  if (r >= stop) return;
+  int b = 0;                                    // how many sequences end at or before r
+  for (int i = 0; i < batch; i += 64) {
+    const int ends = i + lane < batch ? cu[i + lane + 1] : 0x7fffffff;
+    b += __popcll(__ballot(ends <= r));
   }
-  const long long pos = (starts ? (long long)starts[b] : 0) + (r - cu[b]);
-  const Place at = place_of(c, table + (long long)b * table_stride, pos, max_pages);
-  const int off = at.off;
-  float x[8];
-  if (at.page < 0) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = 0.f;
-  } else {
-    const long long row0 = ((long long)at.page * c.kv_heads + head) * c.page_size;
-    uint32_t code[8];
-    if (!is_v) {
-      const int word = (l8 & 3) * (D / 32) + (l8 >> 2);
-      const uint32_t w = *(const uint32_t*)(c.k_codes + (row0 + off) * (D / 2) + word * 4);
-#pragma unroll
-      for (int n = 0; n < 4; ++n) code[2 * n] = w >> (4 * n) & 15u, code[2 * n + 1] = w >> (16 + 4 * n) & 15u;
+  b = min(__builtin_amdgcn_readfirstlane(b), batch - 1);
+  const uint8_t* const codes = is_v ? c.v_codes : c.k_codes;
+  const uint32_t* const params = is_v ? c.v_params : c.k_params;
+  uint16_t* const out = (is_v ? v_out + head * v_sh : k_out + head * k_sh) + l8 * 8;
+  const long long st = is_v ? v_st : k_st;
+
+  while (r < stop && b < batch) {
+    const long long pos = (starts ? (long long)starts[b] : 0) + (r - cu[b]);
+    int n = (int)min(stop, (long long)cu[b + 1]) - (int)r;               // rows of this sequence
+    if (pos < 0) n = (int)min((long long)n, -pos);                       // (in front of its first token, on their own)
+    if (n <= 0) {
+      ++b;
     } else {
-      const uint8_t* p = c.v_codes + row0 * (D / 2) + (long long)(off >> 2) * (2 * D) + (l8 >> 3) * 8 + (off & 3) * 2;
+      // at most two pages: rows below `cut` are in the first
+      const int* row = table + (long long)b * table_stride;
+      const Place first = place_of(c, row, pos, max_pages);
+      const int off = (int)((uint32_t)(pos < 0 ? 0 : pos) % (uint32_t)c.page_size), cut = c.page_size - off;
+      const Place second = n > cut ? place_of(c, row, pos + cut, max_pages) : Place{-1, 0};
+      const long long row_a = ((long long)first.page * c.kv_heads + head) * c.page_size + off;
+      const long long row_b = ((long long)second.page * c.kv_heads + head) * c.page_size - cut;
+      const long long top_a = row_a - off, top_b = row_b + cut;           // first rows of the pages
+      if (is_v) {
+        // quads q = 0 .. of the tokens off & ~3 ..; row i is token (off & 3) + i of them
+        const int shift = off & 3;
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        code[e] = (uint32_t)*(const uint16_t*)(p + ((l8 & 1) * 8 + e) * (D / 8)) >> (4 * ((l8 >> 1) & 3)) & 15u;
-    }
-    const uint32_t param = (is_v ? c.v_params : c.k_params)[row0 * (D / G) + (long long)(l8 / (G / 8)) * c.page_size + off];
-    const float s = scale_of<IS_BF16>(param), lo = low_of<IS_BF16>(param);
+        for (int k = 0; k < 2; ++k) {
+          const int quad = k * (T::TILE / 4) + (lane >> 4), i = quad * 4 - shift;      // i: its first token's row
+          if (quad < QUADS && (T::TILE / 4 == 4 || k == 1 || quad < T::TILE / 4) && i < n && i > -4) {
+            const bool in_b = i >= cut;
+            if ((in_b ? second.page : first.page) >= 0) {
+              const uint8_t* p = codes + ((in_b ? row_b : row_a) + i) * (D / 2) + (lane & 15) * (D / 8);
+              uint32_t w[D / 32];
+              if constexpr (D == 64) {
+                const uint2 v = *(const uint2*)p;
+                w[0] = v.x, w[1] = v.y;
+              } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float value = __builtin_fmaf(s, (float)code[e], lo);
-      x[e] = value > MOST ? MOST : value;               // (a scale that was rounded up; a NaN stays one)
+                for (int j = 0; j < D / 128; ++j) {
+                  const u32x4 v = *(const u32x4*)(p + 16 * j);
+#pragma unroll
+                  for (int m = 0; m < 4; ++m) w[4 * j + m] = v[m];
+                }
+              }
+#pragma unroll
+              for (int h = 0; h < D / 64; ++h)
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+                  *(uint16_t*)(stage + (quad * 4 + t) * ROW + h * 32 + (lane & 15) * 2) = (uint16_t)(w[2 * h + (t >> 1)] >> (16 * (t & 1)));
+            }
+          }
+        }
+      }
+      uint32_t word[T::PASSES], param[T::PASSES];
+#pragma unroll
+      for (int p = 0; p < T::PASSES; ++p) {
+        const int i = p * T::ROWS + lane / T::LANES;
+        const bool in_b = i >= cut;
+        word[p] = param[p] = 0;                 // (no page: zeros)
+        if (i < n && (in_b ? second.page : first.page) >= 0) {
+          const long long at = (in_b ? row_b : row_a) + i, page_top = in_b ? top_b : top_a;
+          if (!is_v) word[p] = *(const uint32_t*)(codes + at * (D / 2) + ((l8 & 3) * (D / 32) + (l8 >> 2)) * 4);
+          param[p] = params[page_top * (D / G) + (long long)(l8 / (G / 8)) * c.page_size + (at - page_top)];
+        }
+      }
+#pragma unroll
+      for (int p = 0; p < T::PASSES; ++p) {
+        const int i = p * T::ROWS + lane / T::LANES;
+        uint32_t lo4, hi4;                      // codes of channels (0, 4, 1, 5) and (2, 6, 3, 7), a byte each
+        if (is_v) {
+          const u32x4 v = *(const u32x4*)(stage + ((off & 3) + i) * ROW + (l8 >> 3) * 32 + (l8 & 1) * 16);
+          const int by = 4 * ((l8 >> 1) & 3);
+          const uint32_t a = v[0] >> by & 0x000f000fu, b2 = v[1] >> by & 0x000f000fu, c2 = v[2] >> by & 0x000f000fu,
+                         d = v[3] >> by & 0x000f000fu;
+          lo4 = a | c2 << 8, hi4 = b2 | d << 8;
+        } else {
+          lo4 = word[p] & 0x0f0f0f0fu, hi4 = word[p] >> 4 & 0x0f0f0f0fu;
+        }
+        const float s = scale_of<IS_BF16>(param[p]), low = low_of<IS_BF16>(param[p]);
+        const float code[8] = {(float)(lo4 & 0xffu), (float)(lo4 >> 16 & 0xffu), (float)(hi4 & 0xffu), (float)(hi4 >> 16 & 0xffu),
+                               (float)(lo4 >> 8 & 0xffu), (float)(lo4 >> 24), (float)(hi4 >> 8 & 0xffu), (float)(hi4 >> 24)};
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = __builtin_fmaf(s, code[e], low);
+        if (__any(__builtin_fmaf(s, 15.f, low) > MOST)) {                // (a scale that was rounded up)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = x[e] > MOST ? MOST : x[e];  // a NaN stays one
+        }
+        if (is_v && (i >= cut ? second.page : first.page) < 0) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = 0.f;
+        }
+        if (i < n) *(u32x4*)(out + (r + i) * st) = pack_row8<IS_BF16>(x);
+      }
+      r += n;
     }
   }
-  uint16_t* dst = is_v ? v_out + r * v_st + head * v_sh : k_out + r * k_st + head * k_sh;
-  *(uint4*)(dst + l8 * 8) = pack_row8<IS_BF16>(x);
 }
 
 // fn(<IS_BF16>, <D>, <G>) for the supported combinations; false if there is none.
@@ -274,6 +452,9 @@ bool cache_ok(const Cache& c) {
          (((uintptr_t)c.k_codes | (uintptr_t)c.v_codes | (uintptr_t)c.k_params | (uintptr_t)c.v_params) & 15) == 0;
 }
 
+// tiles that S tokens can touch, wherever the first one falls
+int tiles_of(int S, int tile) { return (int)(((long long)S + tile - 1 + tile - 1) / tile); }
+
 constexpr const char* BAD_CACHE = "a 4-bit cache needs four 16-byte aligned tensors, pages of a multiple of 16 tokens";
 constexpr const char* BAD_FORM = "head_dim 64 / 128 / 256 with groups of 32 / 64 / 128 channels (at most head_dim), dtype 0 (bf16) or 1 (fp16)";
 
@@ -292,11 +473,10 @@ TDIST_API int tdist_kv4_append(void* k_codes, void* v_codes, void* k_params, voi
   TDIST_REQUIRE(k && v && kv_offset && table, "null argument");
   TDIST_REQUIRE((((uintptr_t)k | (uintptr_t)v) & 15) == 0 && ((k_sb | k_ss | k_sh | v_sb | v_ss | v_sh) & 7) == 0,
                 "k / v rows must keep 16-byte alignment");
-  const int threads = (long long)S * head_dim <= 512 ? 64 : 256;      // (a decode step's one token fills part of a wave)
-  const int rows = threads / (head_dim / 8 > 0 ? head_dim / 8 : 1);
   const bool ok = dispatch(dtype, head_dim, group, [&](auto bf, auto d, auto g) {
+    const int tiles = tiles_of(S, Tile<decltype(d)::value>::TILE), waves = std::min(tiles, 4);
     hipLaunchKernelGGL((kv4_append_kernel<decltype(bf)::value, decltype(d)::value, decltype(g)::value>),
-                       dim3((S + rows - 1) / rows, 2 * kv_heads, batch), dim3(threads), 0, (hipStream_t)stream, c,
+                       dim3((tiles + waves - 1) / waves, 2 * kv_heads, batch), dim3(64 * waves), 0, (hipStream_t)stream, c,
                        (const uint16_t*)k, (const uint16_t*)v, k_sb, k_ss, k_sh, v_sb, v_ss, v_sh, kv_offset, new_lens, table,
                        table_stride, max_pages, S);
   });
@@ -319,15 +499,17 @@ TDIST_API int tdist_kv4_qkv_prep(void* k_codes, void* v_codes, void* k_params, v
   TDIST_REQUIRE(qkv && positions && cos_t && sin_t && q_out && kv_offset && total_out && table, "null argument");
   TDIST_REQUIRE((((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)q_w | (uintptr_t)k_w) & 15) == 0 && ((q_sb | q_ss) & 7) == 0,
                 "qkv rows, norm weights and q must keep 16-byte alignment");
-  const int threads = (long long)S * head_dim <= 512 ? 64 : 256;
-  const int rows = threads / (head_dim / 8 > 0 ? head_dim / 8 : 1);
   const bool ok = dispatch(0, head_dim, group, [&](auto bf, auto d, auto g) {
-    if constexpr (decltype(bf)::value)
+    if constexpr (decltype(bf)::value) {
+      const int tiles = tiles_of(S, Tile<decltype(d)::value>::TILE), waves = std::min(tiles, 4), heads = q_heads + 2 * kv_heads;
+      // heads that share a fetch of the rotation's factors, where there is work for the chip without that
+      const int each = (long long)tiles * heads * batch >= 4 * 8192 ? 4 : 1;
       hipLaunchKernelGGL((kv4_qkv_prep_kernel<decltype(d)::value, decltype(g)::value>),
-                         dim3((S + rows - 1) / rows, q_heads + 2 * kv_heads, batch), dim3(threads), 0, (hipStream_t)stream, c,
-                         (const uint16_t*)qkv, q_sb, q_ss, (const uint16_t*)q_w, (const uint16_t*)k_w, q_eps, k_eps, positions,
-                         cos_t, sin_t, rope_rows, (uint16_t*)q_out, kv_offset, total_out, table, table_stride, max_pages, S,
-                         q_heads);
+                         dim3((tiles + waves - 1) / waves, (heads + each - 1) / each, batch), dim3(64 * waves), 0,
+                         (hipStream_t)stream, c, (const uint16_t*)qkv, q_sb, q_ss, (const uint16_t*)q_w, (const uint16_t*)k_w,
+                         q_eps, k_eps, positions, cos_t, sin_t, rope_rows, (uint16_t*)q_out, kv_offset, total_out, table,
+                         table_stride, max_pages, S, q_heads, each);
+    }
   });
   TDIST_REQUIRE(ok, BAD_FORM);
   TDIST_HIP_TRY(hipGetLastError());
@@ -347,12 +529,14 @@ TDIST_API int tdist_kv4_read(const void* k_codes, const void* v_codes, const voi
   TDIST_REQUIRE(table && cu && k_out && v_out, "null argument");
   TDIST_REQUIRE((((uintptr_t)k_out | (uintptr_t)v_out) & 15) == 0 && ((k_st | k_sh | v_st | v_sh) & 7) == 0,
                 "output rows must keep 16-byte alignment");
-  const int rows = 256 / (head_dim / 8 > 0 ? head_dim / 8 : 1);
+  TDIST_REQUIRE(total / 8 * 2 * kv_heads < (1ll << 30), "too many rows for one call");
   const bool ok = dispatch(dtype, head_dim, group, [&](auto bf, auto d, auto g) {
+    const long long tiles = (total + Tile<decltype(d)::value>::TILE - 1) / Tile<decltype(d)::value>::TILE;
+    const int waves = (int)std::min(tiles, 4ll);
     hipLaunchKernelGGL((kv4_read_kernel<decltype(bf)::value, decltype(d)::value, decltype(g)::value>),
-                       dim3((unsigned)((total + rows - 1) / rows), 2 * kv_heads), dim3(256), 0, (hipStream_t)stream, c, table,
-                       table_stride, max_pages, cu, starts, batch, total, (uint16_t*)k_out, (uint16_t*)v_out, k_st, k_sh, v_st,
-                       v_sh);
+                       dim3((unsigned)((tiles + waves - 1) / waves * 2 * kv_heads)), dim3(64 * waves), 0, (hipStream_t)stream, c,
+                       table, table_stride, max_pages, cu, starts, batch, total, (uint16_t*)k_out, (uint16_t*)v_out, k_st, k_sh,
+                       v_st, v_sh);
   });
   TDIST_REQUIRE(ok, BAD_FORM);
   TDIST_HIP_TRY(hipGetLastError());
