@@ -19,10 +19,12 @@ using namespace tdist::kv4;
 typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
 
 // A wave works on a tile of TILE tokens in PASSES passes of ROWS rows of LANES lanes.
-template <int D>
+template <int D, int MOST = 16>
 struct Tile {
-  static constexpr int LANES = D / 8, ROWS = 64 / LANES, TILE = D == 256 ? 8 : 16, PASSES = TILE / ROWS;
+  static constexpr int LANES = D / 8, ROWS = 64 / LANES, TILE = MOST < 4 * ROWS ? MOST : 4 * ROWS, PASSES = TILE / ROWS;
 };
+template <int D>
+using PrepTile = Tile<D, 8>;        // (the rotation's factors of a tile are kept in registers)
 
 template <bool IS_BF16>
 __device__ __forceinline__ void unpack_row8(const u32x4& v, float (&x)[8]) {
@@ -68,35 +70,48 @@ __device__ __forceinline__ T over_lanes(T v, Op op) {
   return v;
 }
 
-// Codes of the lane's eight channels and the parameter dword of their group.
+// Codes of the lane's eight channels, as floats, and the parameter dword of their group.
 //
-// The quotient has to be the IEEE one.  With r = RN(1 / s), q0 = RN(d r) is within an ulp of it, d - q0 s is exact in
-// one fma and q = RN(q0 + (d - q0 s) r) is the correctly rounded quotient (Markstein's theorem; its one exception, a
-// divisor whose significand is all ones, cannot be a 16-bit number).  That is three operations a channel instead of
-// a division's ten; scales so small or large that an intermediate could leave the normal range take the division.
+// Both quotients, range / 15 and (x - low) / scale, have to be the IEEE ones.  With r = RN(1 / s) and q0 = RN(d r),
+// which is within an ulp of the quotient, d - q0 s is exact in one fma and RN(q0 + (d - q0 s) r) is the correctly rounded
+// quotient (Markstein's theorem); r itself comes from the hardware's reciprocal by one step of the same kind.  Its one
+// exception, a divisor whose significand is all ones, is neither 15 nor a 16-bit number.  That is three operations a channel
+// where a division takes ten; ranges so small or large that an intermediate could leave the normal numbers take the division.
 template <bool IS_BF16, int G>
-__device__ __forceinline__ uint32_t quantise8(const float (&x)[8], uint32_t (&code)[8]) {
-  float lo = x[0], hi = x[0], odd = 0.f;              // odd: NaN if any value is an infinity or a NaN
+__device__ __forceinline__ uint32_t quantise8(const float (&x)[8], float (&code)[8]) {
+  float lo = x[0], hi = x[0];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) lo = fminf(lo, x[e]), hi = fmaxf(hi, x[e]), odd = __builtin_fmaf(x[e], 0.f, odd);
+  for (int e = 1; e < 8; ++e) lo = fminf(lo, x[e]), hi = fmaxf(hi, x[e]);
   lo = over_lanes<G / 8>(lo, [](float a, float b) { return fminf(a, b); });
   hi = over_lanes<G / 8>(hi, [](float a, float b) { return fmaxf(a, b); });
-  odd = over_lanes<G / 8>(odd, [](float a, float b) { return a + b; });
-  const float range = (hi - lo) + odd;
-  const uint32_t s16 = range < INFINITY ? to16<IS_BF16>(range / 15.f) : to16<IS_BF16>(NAN);
-  const float s = from16<IS_BF16>(s16);
-  if (s > 0x1p-100f && s < 0x1p100f) {
-    const float r = 1.f / s;
+  float range = hi - lo;                              // infinite or NaN if a value is infinite
+  const bool nan = __builtin_isunordered(x[0], x[1]) || __builtin_isunordered(x[2], x[3]) ||
+                   __builtin_isunordered(x[4], x[5]) || __builtin_isunordered(x[6], x[7]);
+  if (__any(nan)) {                                   // (minimum and maximum pass over a NaN)
+    const float odd = over_lanes<G / 8>(nan ? NAN : 0.f, [](float a, float b) { return a + b; });
+    range += odd;
+  }
+  uint32_t s16;
+  if (!__any(range > 0.f && !(range > 0x1p-96f && range < 0x1p110f))) {
+    constexpr float R15 = 1.f / 15.f;
+    const float s0 = range * R15;
+    s16 = to16<IS_BF16>(__builtin_fmaf(__builtin_fmaf(-s0, 15.f, range), R15, s0));
+    const float s = from16<IS_BF16>(s16);
+    float r = __builtin_amdgcn_rcpf(s);
+    r = __builtin_fmaf(__builtin_fmaf(-s, r, 1.f), r, r);
+    r = s > 0.f ? r : 0.f;                            // no range, or a scale that is NaN or rounds to 0: codes 0
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float d = x[e] - lo;
       const float q0 = d * r;
-      const float q = __builtin_fmaf(__builtin_fmaf(-q0, s, d), r, q0);
-      code[e] = (uint32_t)fminf(__builtin_rintf(q), 15.f);
+      code[e] = __builtin_rintf(__builtin_fmaf(__builtin_fmaf(-q0, s, d), r, q0));
+      if constexpr (!IS_BF16) code[e] = code[e] > 15.f ? 15.f : code[e];   // a subnormal scale may be rounded down a long way
     }
   } else {
+    s16 = range < INFINITY ? to16<IS_BF16>(range / 15.f) : to16<IS_BF16>(NAN);
+    const float s = from16<IS_BF16>(s16);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) code[e] = s > 0.f ? (uint32_t)fminf(__builtin_rintf((x[e] - lo) / s), 15.f) : 0u;
+    for (int e = 0; e < 8; ++e) code[e] = s > 0.f ? fminf(__builtin_rintf((x[e] - lo) / s), 15.f) : 0.f;
   }
   return s16 | to16<IS_BF16>(lo) << 16;               // (lo is one of the row's 16-bit values)
 }
@@ -108,9 +123,8 @@ __device__ __forceinline__ uint32_t quantise8(const float (&x)[8], uint32_t (&co
 // K rows are runs of their own.  A 16-byte run of V is one channel lane's four tokens: a whole tile is brought into that
 // order in LDS and leaves as 16-byte stores (2-byte stores to eight places: 42 us instead of @@ for 37 MB of rows); the
 // first and last tile of a sequence, whose runs are shared with other calls, are written unit by unit.
-template <bool IS_BF16, int D, int G, bool IS_V, class Rows>
+template <bool IS_BF16, int D, int G, bool IS_V, class T, class Rows>
 __device__ __forceinline__ void store_tile(const Cache& c, const Place& at, int head, int lo, int hi, char* stage, Rows&& rows) {
-  using T = Tile<D>;
   const int lane = threadIdx.x & 63, l8 = lane % T::LANES;
   const long long row0 = ((long long)at.page * c.kv_heads + head) * c.page_size;   // first token of (page, head)
   const bool whole = lo <= 0 && hi >= T::TILE;
@@ -122,12 +136,14 @@ __device__ __forceinline__ void store_tile(const Cache& c, const Place& at, int 
     const bool live = i >= lo && i < hi;
     float x[8];
     rows(p, x);
-    uint32_t code[8];
+    float code[8];
     const uint32_t param = quantise8<IS_BF16, G>(x, code);
     if constexpr (!IS_V) {
-      uint32_t w = 0;
+      // (codes are put together as floats, exactly: one conversion for four)
+      float even = code[6], odd = code[7];
 #pragma unroll
-      for (int n = 0; n < 4; ++n) w |= code[2 * n] << (4 * n) | code[2 * n + 1] << (16 + 4 * n);
+      for (int n = 4; n >= 0; n -= 2) even = __builtin_fmaf(even, 16.f, code[n]), odd = __builtin_fmaf(odd, 16.f, code[n + 1]);
+      const uint32_t w = (uint32_t)even | (uint32_t)odd << 16;
       const int word = (l8 & 3) * (D / 32) + (l8 >> 2);
       if (live) *(uint32_t*)(c.k_codes + (row0 + at.off + i) * (D / 2) + word * 4) = w;
     } else {
@@ -136,7 +152,7 @@ __device__ __forceinline__ void store_tile(const Cache& c, const Place& at, int 
       const int n = (l8 >> 1) & 3;
       uint32_t u[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) u[k] = (code[2 * k] | code[2 * k + 1] << 16) << (4 * n);
+      for (int k = 0; k < 4; ++k) u[k] = (uint32_t)__builtin_fmaf(code[2 * k + 1], 65536.f, code[2 * k]) << (4 * n);
       const bool up1 = n & 1, up2 = n & 2;
       const uint32_t a0 = (up1 ? u[2] : u[0]) | dpp<XOR2>(up1 ? u[0] : u[2]);
       const uint32_t a1 = (up1 ? u[3] : u[1]) | dpp<XOR2>(up1 ? u[1] : u[3]);
@@ -191,15 +207,15 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(Cache c, const uint16_t
   }
   auto rows = [&](int p, float (&x)[8]) { unpack_row8<IS_BF16>(raw[p], x); };
   if (is_v) {
-    store_tile<IS_BF16, D, G, true>(c, at, head, lo, hi, stage[wave], rows);
+    store_tile<IS_BF16, D, G, true, T>(c, at, head, lo, hi, stage[wave], rows);
   } else {
-    store_tile<IS_BF16, D, G, false>(c, at, head, lo, hi, stage[wave], rows);
+    store_tile<IS_BF16, D, G, false, T>(c, at, head, lo, hi, stage[wave], rows);
   }
 }
 
 // grid: (tiles of tokens, blocks of `heads_each` of the Hq + 2 Hkv heads, batch), a wave per tile and block: the rotation's
-// factors of a tile are fetched once for the heads of the block.  The norm's mean square and the rotation are taken in 64 bits,
-// so that a stored code does not depend on the order of a sum.
+// factors of a tile are fetched once for the heads of the block.  K's mean square and rotation are taken in 64 bits, so that a
+// stored code does not depend on the order of a sum; Q's in 32.
 template <int D, int G>
 __global__ __launch_bounds__(256) void kv4_qkv_prep_kernel(Cache c, const uint16_t* __restrict__ qkv, long long q_sb,
                                                            long long q_ss, const uint16_t* __restrict__ q_w,
@@ -210,7 +226,7 @@ __global__ __launch_bounds__(256) void kv4_qkv_prep_kernel(Cache c, const uint16
                                                            const int* __restrict__ kv_offset, int* __restrict__ total_out,
                                                            const int* __restrict__ table, int table_stride, int max_pages,
                                                            int S, int q_heads, int heads_each) {
-  using T = Tile<D>;
+  using T = PrepTile<D>;
   __shared__ __attribute__((aligned(16))) char stage[4][T::TILE * D / 2];
   const int b = blockIdx.z, lane = threadIdx.x & 63, l8 = lane % T::LANES;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -243,7 +259,7 @@ __global__ __launch_bounds__(256) void kv4_qkv_prep_kernel(Cache c, const uint16
       if (i >= lo && i < hi) raw[p] = *(const u32x4*)(src + (s0 + i) * q_ss + (long long)head * D);
     }
   };
-  u32x4 raw[T::PASSES], next[T::PASSES];
+  u32x4 raw[T::PASSES], next[T::PASSES] = {};
   fetch(head0, raw);
   for (int head = head0; head < head1; ++head) {
     if (head + 1 < head1) fetch(head + 1, next);
@@ -255,29 +271,47 @@ __global__ __launch_bounds__(256) void kv4_qkv_prep_kernel(Cache c, const uint16
       unpack_row8<true>(raw[p], x);
       if (is_v) return;
       if (w) {
-        double ss = 0.;
+        float inv;
+        if (is_q) {
+          float ss = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss = __builtin_fma((double)x[e], (double)x[e], ss);
-        ss = over_lanes<T::LANES>(ss, [](double a, double b) { return a + b; });
-        const float inv = (float)(1. / __builtin_sqrt(ss / D + (double)(is_q ? q_eps : k_eps)));
+          for (int e = 0; e < 8; ++e) ss = __builtin_fmaf(x[e], x[e], ss);
+          ss = over_lanes<T::LANES>(ss, [](float a, float b) { return a + b; });
+          inv = __builtin_amdgcn_rsqf(ss * (1.f / D) + q_eps);
+        } else {
+          double ss = 0.;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) ss = __builtin_fma((double)x[e], (double)x[e], ss);
+          ss = over_lanes<T::LANES>(ss, [](double a, double b) { return a + b; });
+          inv = (float)(1. / __builtin_sqrt(ss / D + (double)k_eps));
+        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = from16<true>(to16<true>(x[e] * inv * g[e]));
       }
       // pairs (i, i + D / 2) are the same element of lanes l8 and l8 ^ (D / 16)
-      const double sign = l8 < T::LANES / 2 ? -1. : 1.;
-      float y[8];
+      float other[8], y[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        float other;
         if constexpr (D == 128) {
-          other = dpp<ROR8>(x[e]);
+          other[e] = dpp<ROR8>(x[e]);
         } else if constexpr (D == 64) {
-          other = dpp<XOR7>(dpp<XOR3>(x[e]));
+          other[e] = dpp<XOR7>(dpp<XOR3>(x[e]));
         } else {
-          other = __shfl_xor(x[e], 16);
+          other[e] = __shfl_xor(x[e], 16);
         }
-        y[e] = (float)__builtin_fma((double)x[e], (double)cs[p][e], sign * other * sn[p][e]);
-        asm volatile("" : "+v"(y[e]));          // 64 -> 32 -> 16 bits as two roundings, which the compiler would merge
+        if (l8 < T::LANES / 2) other[e] = -other[e];
+      }
+      if (is_q) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = __builtin_fmaf(x[e], cs[p][e], other[e] * sn[p][e]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float co = cs[p][e], si = sn[p][e];
+          asm volatile("" : "+v"(co), "+v"(si));      // (not all of them as 64-bit numbers ahead of the loop over the heads)
+          y[e] = (float)__builtin_fma((double)x[e], (double)co, (double)other[e] * si);
+          asm volatile("" : "+v"(y[e]));        // 64 -> 32 -> 16 bits as two roundings, which the compiler would merge
+        }
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] = from16<true>(to16<true>(y[e]));
@@ -293,9 +327,9 @@ __global__ __launch_bounds__(256) void kv4_qkv_prep_kernel(Cache c, const uint16
       }
     } else if (at.page >= 0) {
       if (is_v) {
-        store_tile<true, D, G, true>(c, at, head - q_heads - c.kv_heads, lo, hi, stage[wave], rows);
+        store_tile<true, D, G, true, T>(c, at, head - q_heads - c.kv_heads, lo, hi, stage[wave], rows);
       } else {
-        store_tile<true, D, G, false>(c, at, head - q_heads, lo, hi, stage[wave], rows);
+        store_tile<true, D, G, false, T>(c, at, head - q_heads, lo, hi, stage[wave], rows);
       }
     }
 #pragma unroll
@@ -303,13 +337,13 @@ __global__ __launch_bounds__(256) void kv4_qkv_prep_kernel(Cache c, const uint16
   }
 }
 
-// Row r of the output belongs to the sequence b with cu[b] <= r < cu[b + 1].  A wave takes TILE rows of one head of K or V,
+// Row r of the output belongs to the sequence b with cu[b] <= r < cu[b + 1].  A wave takes `rows_each` rows (TILE, or ROWS) of one head of K or V,
 // sequence by sequence; workgroups with neighbouring numbers take the heads of the same rows, which are neighbours in the
 // output.  V's runs of four tokens are turned into rows in LDS.
 template <bool IS_BF16, int D, int G>
 __global__ __launch_bounds__(256) void kv4_read_kernel(Cache c, const int* __restrict__ table, int table_stride, int max_pages,
                                                        const int* __restrict__ cu, const int* __restrict__ starts, int batch,
-                                                       long long total, uint16_t* __restrict__ k_out,
+                                                       long long total, int rows_each, uint16_t* __restrict__ k_out,
                                                        uint16_t* __restrict__ v_out, long long k_st, long long k_sh,
                                                        long long v_st, long long v_sh) {
   using T = Tile<D>;
@@ -324,20 +358,67 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(Cache c, const int* __res
   const bool is_v = (int)which >= c.kv_heads;
   const int head = which - (is_v ? c.kv_heads : 0);
   const long long end = min(total, (long long)cu[batch]);
-  long long r = max(((long long)tile * (blockDim.x >> 6) + wave) * T::TILE, (long long)cu[0]);
-  const long long stop = min(((long long)tile * (blockDim.x >> 6) + wave + 1) * T::TILE, end);
+  long long r = max(((long long)tile * (blockDim.x >> 6) + wave) * rows_each, (long long)cu[0]);
+  const long long stop = min(((long long)tile * (blockDim.x >> 6) + wave + 1) * rows_each, end);
   if (r >= stop) return;
-  int b = 0;                                    // how many sequences end at or before r
+  int b = 0, b_last = 0;                        // how many sequences end at or before r, and before the last row
   for (int i = 0; i < batch; i += 64) {
     const int ends = i + lane < batch ? cu[i + lane + 1] : 0x7fffffff;
     b += __popcll(__ballot(ends <= r));
+    b_last += __popcll(__ballot(ends < stop));
   }
   b = min(__builtin_amdgcn_readfirstlane(b), batch - 1);
+  b_last = min(__builtin_amdgcn_readfirstlane(b_last), batch - 1);
   const uint8_t* const codes = is_v ? c.v_codes : c.k_codes;
   const uint32_t* const params = is_v ? c.v_params : c.k_params;
   uint16_t* const out = (is_v ? v_out + head * v_sh : k_out + head * k_sh) + l8 * 8;
   const long long st = is_v ? v_st : k_st;
 
+  if (b_last > b + 1) {
+    // rows of many sequences (a decode step's, one each): every row finds its own place, V channel by channel
+    const int ends = b + lane < batch ? cu[b + lane + 1] : 0x7fffffff;
+#pragma unroll
+    for (int p = 0; p < T::PASSES; ++p) {
+      if (r + p * T::ROWS >= stop) break;
+      const long long mine = r + p * T::ROWS + lane / T::LANES;
+      int at_b = b;
+#pragma unroll
+      for (int j = 0; j < T::ROWS; ++j) {
+        const int passed = __popcll(__ballot(ends <= r + p * T::ROWS + j));
+        if (lane / T::LANES == j) at_b = b + passed;
+      }
+      if (b_last - b >= 64) {                   // (sixty sequences without rows between these: a lane each does not reach)
+        at_b = b;
+        for (int top = b_last + 1; top - at_b > 1;) {
+          const int mid = (at_b + top) >> 1;
+          if (cu[mid] <= mine) at_b = mid; else top = mid;
+        }
+      }
+      if (mine >= stop) continue;
+      const long long pos = (starts ? (long long)starts[at_b] : 0) + (mine - cu[at_b]);
+      const Place at = place_of(c, table + (long long)at_b * table_stride, pos, max_pages);
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = 0.f;
+      if (at.page >= 0) {
+        const long long row0 = ((long long)at.page * c.kv_heads + head) * c.page_size;
+        const uint32_t param = params[row0 * (D / G) + (long long)(l8 / (G / 8)) * c.page_size + at.off];
+        const float s = scale_of<IS_BF16>(param), low = low_of<IS_BF16>(param);
+        const uint8_t* k_at = codes + (row0 + at.off) * (D / 2) + ((l8 & 3) * (D / 32) + (l8 >> 2)) * 4;
+        const uint8_t* v_at = codes + row0 * (D / 2) + (at.off >> 2) * (2 * D) + (l8 & 1) * D + (l8 >> 3) * 8 + (at.off & 3) * 2;
+        const uint32_t w = is_v ? 0u : *(const uint32_t*)k_at;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t unit = is_v ? (uint32_t)*(const uint16_t*)(v_at + e * (D / 8)) >> (4 * ((l8 >> 1) & 3))
+                                     : w >> (4 * (e >> 1) + 16 * (e & 1));
+          x[e] = __builtin_fmaf(s, (float)(unit & 15u), low);
+          x[e] = x[e] > MOST ? MOST : x[e];
+        }
+      }
+      *(u32x4*)(out + mine * st) = pack_row8<IS_BF16>(x);
+    }
+    return;
+  }
   while (r < stop && b < batch) {
     const long long pos = (starts ? (long long)starts[b] : 0) + (r - cu[b]);
     int n = (int)min(stop, (long long)cu[b + 1]) - (int)r;               // rows of this sequence
@@ -501,9 +582,9 @@ TDIST_API int tdist_kv4_qkv_prep(void* k_codes, void* v_codes, void* k_params, v
                 "qkv rows, norm weights and q must keep 16-byte alignment");
   const bool ok = dispatch(0, head_dim, group, [&](auto bf, auto d, auto g) {
     if constexpr (decltype(bf)::value) {
-      const int tiles = tiles_of(S, Tile<decltype(d)::value>::TILE), waves = std::min(tiles, 4), heads = q_heads + 2 * kv_heads;
+      const int tiles = tiles_of(S, PrepTile<decltype(d)::value>::TILE), waves = std::min(tiles, 4), heads = q_heads + 2 * kv_heads;
       // heads that share a fetch of the rotation's factors, where there is work for the chip without that
-      const int each = (long long)tiles * heads * batch >= 4 * 8192 ? 4 : 1;
+      const int each = (long long)tiles * heads * batch >= 8 * 8192 ? 8 : 1;
       hipLaunchKernelGGL((kv4_qkv_prep_kernel<decltype(d)::value, decltype(g)::value>),
                          dim3((tiles + waves - 1) / waves, (heads + each - 1) / each, batch), dim3(64 * waves), 0,
                          (hipStream_t)stream, c, (const uint16_t*)qkv, q_sb, q_ss, (const uint16_t*)q_w, (const uint16_t*)k_w,
@@ -529,13 +610,16 @@ TDIST_API int tdist_kv4_read(const void* k_codes, const void* v_codes, const voi
   TDIST_REQUIRE(table && cu && k_out && v_out, "null argument");
   TDIST_REQUIRE((((uintptr_t)k_out | (uintptr_t)v_out) & 15) == 0 && ((k_st | k_sh | v_st | v_sh) & 7) == 0,
                 "output rows must keep 16-byte alignment");
-  TDIST_REQUIRE(total / 8 * 2 * kv_heads < (1ll << 30), "too many rows for one call");
+  TDIST_REQUIRE(total * kv_heads < (1ll << 31), "too many rows for one call");
   const bool ok = dispatch(dtype, head_dim, group, [&](auto bf, auto d, auto g) {
-    const long long tiles = (total + Tile<decltype(d)::value>::TILE - 1) / Tile<decltype(d)::value>::TILE;
+    // short sequences: as few of them in a wave as there can be
+    using T = Tile<decltype(d)::value>;
+    const int rows_each = total <= 4ll * batch ? T::ROWS : T::TILE;
+    const long long tiles = (total + rows_each - 1) / rows_each;
     const int waves = (int)std::min(tiles, 4ll);
     hipLaunchKernelGGL((kv4_read_kernel<decltype(bf)::value, decltype(d)::value, decltype(g)::value>),
                        dim3((unsigned)((tiles + waves - 1) / waves * 2 * kv_heads)), dim3(64 * waves), 0, (hipStream_t)stream, c,
-                       table, table_stride, max_pages, cu, starts, batch, total, (uint16_t*)k_out, (uint16_t*)v_out, k_st, k_sh,
+                       table, table_stride, max_pages, cu, starts, batch, total, rows_each, (uint16_t*)k_out, (uint16_t*)v_out, k_st, k_sh,
                        v_st, v_sh);
   });
   TDIST_REQUIRE(ok, BAD_FORM);
