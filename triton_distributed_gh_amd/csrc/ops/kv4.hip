@@ -70,44 +70,49 @@ __device__ __forceinline__ T over_lanes(T v, Op op) {
   return v;
 }
 
+// A group's range over the G / 8 lanes that hold it, and its smallest value; `nan`: one of the lane's values is a NaN (which
+// minimum and maximum pass over).  An infinite value makes the range infinite or NaN.
+template <int G>
+__device__ __forceinline__ float range_of(const float (&x)[8], float& lo, bool& nan) {
+  float hi = x[0];
+  lo = x[0];
+#pragma unroll
+  for (int e = 1; e < 8; ++e) lo = fminf(lo, x[e]), hi = fmaxf(hi, x[e]);
+  lo = over_lanes<G / 8>(lo, [](float a, float b) { return fminf(a, b); });
+  hi = over_lanes<G / 8>(hi, [](float a, float b) { return fmaxf(a, b); });
+  nan = __builtin_isunordered(x[0], x[1]) | __builtin_isunordered(x[2], x[3]) | __builtin_isunordered(x[4], x[5]) |
+        __builtin_isunordered(x[6], x[7]);
+  return hi - lo;
+}
+__device__ __forceinline__ bool ordinary(float range) { return range == 0.f || (range > 0x1p-96f && range < 0x1p110f); }
+
 // Codes of the lane's eight channels, as floats, and the parameter dword of their group.
 //
 // Both quotients, range / 15 and (x - low) / scale, have to be the IEEE ones.  With r = RN(1 / s) and q0 = RN(d r),
 // which is within an ulp of the quotient, d - q0 s is exact in one fma and RN(q0 + (d - q0 s) r) is the correctly rounded
 // quotient (Markstein's theorem); r itself comes from the hardware's reciprocal by one step of the same kind.  Its one
 // exception, a divisor whose significand is all ones, is neither 15 nor a 16-bit number.  That is three operations a channel
-// where a division takes ten; ranges so small or large that an intermediate could leave the normal numbers take the division.
-template <bool IS_BF16, int G>
-__device__ __forceinline__ uint32_t quantise8(const float (&x)[8], float (&code)[8]) {
-  float lo = x[0], hi = x[0];
-#pragma unroll
-  for (int e = 1; e < 8; ++e) lo = fminf(lo, x[e]), hi = fmaxf(hi, x[e]);
-  lo = over_lanes<G / 8>(lo, [](float a, float b) { return fminf(a, b); });
-  hi = over_lanes<G / 8>(hi, [](float a, float b) { return fmaxf(a, b); });
-  float range = hi - lo;                              // infinite or NaN if a value is infinite
-  const bool nan = __builtin_isunordered(x[0], x[1]) || __builtin_isunordered(x[2], x[3]) ||
-                   __builtin_isunordered(x[4], x[5]) || __builtin_isunordered(x[6], x[7]);
-  if (__any(nan)) {                                   // (minimum and maximum pass over a NaN)
-    const float odd = over_lanes<G / 8>(nan ? NAN : 0.f, [](float a, float b) { return a + b; });
-    range += odd;
-  }
+// where a division takes ten.  PLAIN: the range is ordinary, no intermediate can leave the normal numbers; the others divide.
+template <bool IS_BF16, int G, bool PLAIN>
+__device__ __forceinline__ uint32_t quantise8(const float (&x)[8], float lo, float range, bool nan, float (&code)[8]) {
   uint32_t s16;
-  if (!__any(range > 0.f && !(range > 0x1p-96f && range < 0x1p110f))) {
+  if (PLAIN) {
     constexpr float R15 = 1.f / 15.f;
     const float s0 = range * R15;
     s16 = to16<IS_BF16>(__builtin_fmaf(__builtin_fmaf(-s0, 15.f, range), R15, s0));
     const float s = from16<IS_BF16>(s16);
     float r = __builtin_amdgcn_rcpf(s);
     r = __builtin_fmaf(__builtin_fmaf(-s, r, 1.f), r, r);
-    r = s > 0.f ? r : 0.f;                            // no range, or a scale that is NaN or rounds to 0: codes 0
+    r = s > 0.f ? r : 0.f;                            // no range, or a scale that rounds to 0: codes 0
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float d = x[e] - lo;
       const float q0 = d * r;
       code[e] = __builtin_rintf(__builtin_fmaf(__builtin_fmaf(-q0, s, d), r, q0));
-      if constexpr (!IS_BF16) code[e] = code[e] > 15.f ? 15.f : code[e];   // a subnormal scale may be rounded down a long way
+      if constexpr (!IS_BF16) code[e] = fminf(code[e], 15.f);   // a subnormal scale may be rounded down a long way
     }
   } else {
+    range += over_lanes<G / 8>(nan ? NAN : 0.f, [](float a, float b) { return a + b; });
     s16 = range < INFINITY ? to16<IS_BF16>(range / 15.f) : to16<IS_BF16>(NAN);
     const float s = from16<IS_BF16>(s16);
 #pragma unroll
@@ -117,27 +122,23 @@ __device__ __forceinline__ uint32_t quantise8(const float (&x)[8], float (&code)
 }
 
 // Quantises a tile of rows of one head and writes rows lo .. hi - 1 of it.  `at`: the place of the tile's first token (a
-// multiple of TILE, so all of them are in one page).  rows(p, x): the lane's eight channels of pass p.  `stage`: 8 D bytes of LDS
-// of the wave's own.
+// multiple of TILE, so all of them are in one page).  rows(p, x): the lane's eight channels of pass p.  `stage`: TILE D / 2 bytes
+// of LDS of the wave's own.
 //
 // K rows are runs of their own.  A 16-byte run of V is one channel lane's four tokens: a whole tile is brought into that
-// order in LDS and leaves as 16-byte stores (2-byte stores to eight places: 42 us instead of @@ for 37 MB of rows); the
-// first and last tile of a sequence, whose runs are shared with other calls, are written unit by unit.
+// order in LDS and leaves as 16-byte stores; the first and last tile of a sequence, whose runs are shared with other calls, are
+// written unit by unit.  The passes of a whole tile are one stretch of straight code.
 template <bool IS_BF16, int D, int G, bool IS_V, class T, class Rows>
 __device__ __forceinline__ void store_tile(const Cache& c, const Place& at, int head, int lo, int hi, char* stage, Rows&& rows) {
   const int lane = threadIdx.x & 63, l8 = lane % T::LANES;
   const long long row0 = ((long long)at.page * c.kv_heads + head) * c.page_size;   // first token of (page, head)
-  const bool whole = lo <= 0 && hi >= T::TILE;
   uint8_t* const vbase = c.v_codes + (row0 + at.off) * (D / 2);
-#pragma unroll
-  for (int p = 0; p < T::PASSES; ++p) {
-    if (hi <= p * T::ROWS || lo >= (p + 1) * T::ROWS) continue;                    // (uniform)
+  uint32_t* const params = (IS_V ? c.v_params : c.k_params) + row0 * (D / G) + (long long)(l8 / (G / 8)) * c.page_size + at.off;
+
+  auto write = [&](auto whole_, int p, uint32_t param, const float (&code)[8]) __attribute__((always_inline)) {
+    constexpr bool WHOLE = decltype(whole_)::value;
     const int i = p * T::ROWS + lane / T::LANES;
-    const bool live = i >= lo && i < hi;
-    float x[8];
-    rows(p, x);
-    float code[8];
-    const uint32_t param = quantise8<IS_BF16, G>(x, code);
+    const bool live = WHOLE || (i >= lo && i < hi);
     if constexpr (!IS_V) {
       // (codes are put together as floats, exactly: one conversion for four)
       float even = code[6], odd = code[7];
@@ -159,7 +160,7 @@ __device__ __forceinline__ void store_tile(const Cache& c, const Place& at, int 
       const uint32_t b = (up2 ? a1 : a0) | xor4(up2 ? a0 : a1);
       const int ch = (l8 & 1) * 8 + (up1 ? 4 : 0) + (up2 ? 2 : 0);                  // this lane's units: channels ch, ch + 1
       const int to = (i >> 2) * (2 * D) + ch * (D / 8) + (l8 >> 3) * 8 + (i & 3) * 2;
-      if (whole) {
+      if (WHOLE) {
         *(uint16_t*)(stage + to) = (uint16_t)b;
         *(uint16_t*)(stage + to + D / 8) = (uint16_t)(b >> 16);
       } else if (live) {
@@ -167,17 +168,55 @@ __device__ __forceinline__ void store_tile(const Cache& c, const Place& at, int 
         *(uint16_t*)(vbase + to + D / 8) = (uint16_t)(b >> 16);
       }
     }
-    if (live && l8 % (G / 8) == 0) {
-      uint32_t* params = IS_V ? c.v_params : c.k_params;
-      params[row0 * (D / G) + (long long)(l8 / (G / 8)) * c.page_size + at.off + i] = param;
+    if (live && l8 % (G / 8) == 0) params[i] = param;
+  };
+
+  if (lo <= 0 && hi >= T::TILE) {
+    float x[T::PASSES][8], low[T::PASSES], range[T::PASSES];
+    bool nan[T::PASSES], odd = false;
+#pragma unroll
+    for (int p = 0; p < T::PASSES; ++p) {
+      rows(p, x[p]);
+      range[p] = range_of<G>(x[p], low[p], nan[p]);
+      odd |= nan[p] | !ordinary(range[p]);
     }
-  }
-  if constexpr (IS_V) {
-    if (whole && lane * 16 < T::TILE * (D / 2)) *(u32x4*)(vbase + lane * 16) = *(const u32x4*)(stage + lane * 16);
+    if (!__any(odd)) {
+#pragma unroll
+      for (int p = 0; p < T::PASSES; ++p) {
+        float code[8];
+        const uint32_t param = quantise8<IS_BF16, G, true>(x[p], low[p], range[p], false, code);
+        write(std::true_type{}, p, param, code);
+      }
+    } else {
+#pragma unroll
+      for (int p = 0; p < T::PASSES; ++p) {
+        float code[8];
+        const uint32_t param = quantise8<IS_BF16, G, false>(x[p], low[p], range[p], nan[p], code);
+        write(std::true_type{}, p, param, code);
+      }
+    }
+    if (IS_V && lane * 16 < T::TILE * (D / 2)) *(u32x4*)(vbase + lane * 16) = *(const u32x4*)(stage + lane * 16);
+  } else {
+#pragma unroll
+    for (int p = 0; p < T::PASSES; ++p) {
+      if (hi <= p * T::ROWS || lo >= (p + 1) * T::ROWS) continue;                  // (uniform)
+      float x[8], code[8], low;
+      bool nan;
+      rows(p, x);
+      const float range = range_of<G>(x, low, nan);
+      uint32_t param;
+      if (!__any(nan | !ordinary(range))) {
+        param = quantise8<IS_BF16, G, true>(x, low, range, false, code);
+      } else {
+        param = quantise8<IS_BF16, G, false>(x, low, range, nan, code);
+      }
+      write(std::false_type{}, p, param, code);
+    }
   }
 }
 
-// grid: (tiles of tokens, Hkv heads of K then Hkv of V, batch), a wave per tile.  Tiles are aligned in the sequence.
+// A wave per tile and head; workgroups with neighbouring numbers take the heads (Hkv of K, then Hkv of V) of the same tokens,
+// whose rows are neighbours in memory.  Tiles are aligned in the sequence.  grid: (tiles x heads, batch)
 template <bool IS_BF16, int D, int G>
 __global__ __launch_bounds__(256) void kv4_append_kernel(Cache c, const uint16_t* __restrict__ k, const uint16_t* __restrict__ v,
                                                          long long k_sb, long long k_ss, long long k_sh, long long v_sb,
@@ -186,12 +225,13 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(Cache c, const uint16_t
                                                          int table_stride, int max_pages, int S) {
   using T = Tile<D>;
   __shared__ __attribute__((aligned(16))) char stage[4][T::TILE * D / 2];
-  const int b = blockIdx.z, lane = threadIdx.x & 63, l8 = lane % T::LANES;
+  const int b = blockIdx.y, lane = threadIdx.x & 63, l8 = lane % T::LANES;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const bool is_v = (int)blockIdx.y >= c.kv_heads;
-  const int head = blockIdx.y - (is_v ? c.kv_heads : 0);
+  const uint32_t tile = blockIdx.x / (2u * c.kv_heads), which = blockIdx.x - tile * 2u * c.kv_heads;
+  const bool is_v = (int)which >= c.kv_heads;
+  const int head = which - (is_v ? c.kv_heads : 0);
   const int offset = kv_offset[b], count = new_lens ? min(new_lens[b], S) : S;
-  const long long s0 = (long long)(blockIdx.x * (blockDim.x >> 6) + wave) * T::TILE - (offset & (T::TILE - 1));   // the tile's first row
+  const long long s0 = ((long long)tile * (blockDim.x >> 6) + wave) * T::TILE - (offset & (T::TILE - 1));   // the tile's first row
   if (s0 >= count) return;
   const Place at = place_of(c, table + (long long)b * table_stride, offset + s0, max_pages);
   if (at.page < 0) return;
@@ -213,7 +253,7 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(Cache c, const uint16_t
   }
 }
 
-// grid: (tiles of tokens, blocks of `heads_each` of the Hq + 2 Hkv heads, batch), a wave per tile and block: the rotation's
+// grid: (tiles of tokens x blocks of `heads_each` of the Hq + 2 Hkv heads, batch), a wave per tile and block: the rotation's
 // factors of a tile are fetched once for the heads of the block.  K's mean square and rotation are taken in 64 bits, so that a
 // stored code does not depend on the order of a sum; Q's in 32.
 template <int D, int G>
@@ -228,14 +268,16 @@ __global__ __launch_bounds__(256) void kv4_qkv_prep_kernel(Cache c, const uint16
                                                            int S, int q_heads, int heads_each) {
   using T = PrepTile<D>;
   __shared__ __attribute__((aligned(16))) char stage[4][T::TILE * D / 2];
-  const int b = blockIdx.z, lane = threadIdx.x & 63, l8 = lane % T::LANES;
+  const int b = blockIdx.y, lane = threadIdx.x & 63, l8 = lane % T::LANES;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int heads = q_heads + 2 * c.kv_heads;
+  const uint32_t blocks = (heads + heads_each - 1) / heads_each, tile = blockIdx.x / blocks, block = blockIdx.x - tile * blocks;
   const int offset = kv_offset[b];
-  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) total_out[b] = offset + S;
-  const long long s0 = (long long)(blockIdx.x * (blockDim.x >> 6) + wave) * T::TILE - (offset & (T::TILE - 1));
+  if (blockIdx.x == 0 && threadIdx.x == 0) total_out[b] = offset + S;
+  const long long s0 = ((long long)tile * (blockDim.x >> 6) + wave) * T::TILE - (offset & (T::TILE - 1));
   if (s0 >= S) return;
   const int lo = s0 < 0 ? (int)-s0 : 0, hi = (int)min((long long)T::TILE, S - s0);
-  const int head0 = blockIdx.y * heads_each, heads = q_heads + 2 * c.kv_heads, head1 = min(head0 + heads_each, heads);
+  const int head0 = block * heads_each, head1 = min(head0 + heads_each, heads);
   Place at = Place{-1, 0};
   if (head1 > q_heads) at = place_of(c, table + (long long)b * table_stride, offset + s0, max_pages);
   float cs[T::PASSES][8], sn[T::PASSES][8];
@@ -549,7 +591,8 @@ TDIST_API int tdist_kv4_append(void* k_codes, void* v_codes, void* k_params, voi
   const Cache c{(uint8_t*)k_codes, (uint8_t*)v_codes, (uint32_t*)k_params, (uint32_t*)v_params, pages, kv_heads, page_size};
   TDIST_REQUIRE(cache_ok(c), BAD_CACHE);
   TDIST_REQUIRE(dtype == 0 || dtype == 1, BAD_FORM);
-  TDIST_REQUIRE(batch >= 0 && batch <= 65535 && S >= 0 && max_pages >= 0, "bad batch / token count");
+  TDIST_REQUIRE(batch >= 0 && batch <= 65535 && S >= 0 && max_pages >= 0 && (long long)S * kv_heads < (1ll << 31),
+                "bad batch / token count");
   if (batch == 0 || S == 0) return 0;
   TDIST_REQUIRE(k && v && kv_offset && table, "null argument");
   TDIST_REQUIRE((((uintptr_t)k | (uintptr_t)v) & 15) == 0 && ((k_sb | k_ss | k_sh | v_sb | v_ss | v_sh) & 7) == 0,
@@ -557,7 +600,7 @@ TDIST_API int tdist_kv4_append(void* k_codes, void* v_codes, void* k_params, voi
   const bool ok = dispatch(dtype, head_dim, group, [&](auto bf, auto d, auto g) {
     const int tiles = tiles_of(S, Tile<decltype(d)::value>::TILE), waves = std::min(tiles, 4);
     hipLaunchKernelGGL((kv4_append_kernel<decltype(bf)::value, decltype(d)::value, decltype(g)::value>),
-                       dim3((tiles + waves - 1) / waves, 2 * kv_heads, batch), dim3(64 * waves), 0, (hipStream_t)stream, c,
+                       dim3((tiles + waves - 1) / waves * 2 * kv_heads, batch), dim3(64 * waves), 0, (hipStream_t)stream, c,
                        (const uint16_t*)k, (const uint16_t*)v, k_sb, k_ss, k_sh, v_sb, v_ss, v_sh, kv_offset, new_lens, table,
                        table_stride, max_pages, S);
   });
@@ -574,7 +617,8 @@ TDIST_API int tdist_kv4_qkv_prep(void* k_codes, void* v_codes, void* k_params, v
                                  int batch, int S, int q_heads, void* stream) {
   const Cache c{(uint8_t*)k_codes, (uint8_t*)v_codes, (uint32_t*)k_params, (uint32_t*)v_params, pages, kv_heads, page_size};
   TDIST_REQUIRE(cache_ok(c), BAD_CACHE);
-  TDIST_REQUIRE(batch >= 0 && batch <= 65535 && S >= 0 && max_pages >= 0 && q_heads > 0 && q_heads <= 32767 && rope_rows > 0,
+  TDIST_REQUIRE(batch >= 0 && batch <= 65535 && S >= 0 && max_pages >= 0 && q_heads > 0 && q_heads <= 32767 && rope_rows > 0 &&
+                    (long long)S * (q_heads + 2 * kv_heads) < (1ll << 31),
                 "bad batch / token / head count");
   if (batch == 0 || S == 0) return 0;
   TDIST_REQUIRE(qkv && positions && cos_t && sin_t && q_out && kv_offset && total_out && table, "null argument");
@@ -584,9 +628,9 @@ TDIST_API int tdist_kv4_qkv_prep(void* k_codes, void* v_codes, void* k_params, v
     if constexpr (decltype(bf)::value) {
       const int tiles = tiles_of(S, PrepTile<decltype(d)::value>::TILE), waves = std::min(tiles, 4), heads = q_heads + 2 * kv_heads;
       // heads that share a fetch of the rotation's factors, where there is work for the chip without that
-      const int each = (long long)tiles * heads * batch >= 8 * 8192 ? 8 : 1;
+      const int each = (int)std::max(1ll, std::min(8ll, (long long)tiles * heads * batch / 6144));
       hipLaunchKernelGGL((kv4_qkv_prep_kernel<decltype(d)::value, decltype(g)::value>),
-                         dim3((tiles + waves - 1) / waves, (heads + each - 1) / each, batch), dim3(64 * waves), 0,
+                         dim3((tiles + waves - 1) / waves * ((heads + each - 1) / each), batch), dim3(64 * waves), 0,
                          (hipStream_t)stream, c, (const uint16_t*)qkv, q_sb, q_ss, (const uint16_t*)q_w, (const uint16_t*)k_w,
                          q_eps, k_eps, positions, cos_t, sin_t, rope_rows, (uint16_t*)q_out, kv_offset, total_out, table,
                          table_stride, max_pages, S, q_heads, each);
