@@ -286,3 +286,32 @@ def test_argument_types_of_the_native_calls_match_the_sources():
         args = re.search(rf"TDIST_API int {name}\((.*?)\) \{{", source, re.S).group(1).split(",")
         kinds = ["p" if "*" in a else "q" if "long long" in a else "f" if "float" in a else "i" for a in args]
         assert "".join(kinds) == signature, name
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_attention_layer_over_a_4bit_cache(dtype):
+    from kv4_layer_checks import attention_layer
+
+    attention_layer("cpu", dtype)
+
+
+def test_engine_with_a_4bit_cache(monkeypatch):
+    monkeypatch.setenv("RANDOM_PARAMS", "1")
+    monkeypatch.setenv("TDIST_NO_HF_CONFIG", "1")
+    from triton_distributed_gh_amd.models import Engine, KV4_Cache, ModelConfig
+
+    config = ModelConfig(model_name="tdist/tiny-dense", max_length=64, dtype=torch.bfloat16, rank=0, world_size=1)
+    with pytest.raises(ValueError):
+        Engine(config, kv_cache_bits=8)
+    eng = Engine(config, kv_cache_bits=4)
+    ids = torch.randint(0, 1000, (2, 9), generator=_gen(3))
+    first = eng.serve(ids, gen_len=4)
+    assert isinstance(eng.kv_cache, KV4_Cache) and eng.kv_cache.get_kv_len().tolist() == [13, 13]
+    assert first.shape == (2, 4) and torch.equal(first, eng.serve(ids, gen_len=4))
+
+
+def test_facade_serves_the_operators():
+    import triton_dist.kernels.amd.kv4 as facade
+    from triton_dist.models.kv_cache import KV4_Cache  # noqa: F401
+
+    assert facade is kv4

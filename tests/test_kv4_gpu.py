@@ -408,3 +408,56 @@ def test_pages_far_beyond_32_bit_offsets():
         assert ((g.double().cpu() - w).abs() <= (2.0 ** -8 + 2.0 ** -23) * w.abs() + 2.0 ** -26).all()
     want, _ = oracle.attention(q, [kh], [vh], D ** -0.5)
     _check(out, want, None, None, torch.bfloat16, float(vh.abs().max()))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_attention_layer_over_a_4bit_cache(dtype):
+    from kv4_layer_checks import attention_layer
+
+    attention_layer("cuda", dtype)
+
+
+@pytest.mark.parametrize("backend", ["torch", "triton_dist_AR"])
+def test_engine_decodes_from_a_graph_over_a_4bit_cache(backend, monkeypatch):
+    monkeypatch.setenv("RANDOM_PARAMS", "1")
+    monkeypatch.setenv("TDIST_NO_HF_CONFIG", "1")
+    from triton_distributed_gh_amd.models import Engine, KV4_Cache, ModelConfig
+    from triton_distributed_gh_amd.utils.testing import VirtualCluster
+
+    config = ModelConfig(model_name="tdist/tiny-dense-d128", max_length=128, dtype=torch.bfloat16, rank=0, world_size=1)
+    vc = VirtualCluster(1, heap_bytes=1 << 26)
+    try:
+        eng = Engine(config, env=vc.envs[0], kv_cache_bits=4)
+        eng.backend = backend
+        ids = torch.randint(0, 1000, (3, 37), generator=_gen(33))
+        replayed = eng.serve(ids, gen_len=12)
+        assert isinstance(eng.kv_cache, KV4_Cache)
+        eng.no_graph = True
+        assert torch.equal(replayed, eng.serve(ids, gen_len=12))
+    finally:
+        vc.close()
+
+
+def test_sequence_parallel_decode_over_4bit_shards():
+    from triton_distributed_gh_amd.layers import SpGQAFlashDecodeAttention
+    from triton_distributed_gh_amd.utils.testing import VirtualCluster
+
+    gen = _gen(34)
+    w, Hq, H, D, group, page = 2, 8, 2, 128, 64, 16
+    lens = [[70, 16], [33, 0]]
+    q = oracle.rows(gen, 2, Hq, D, device="cuda")
+    shards = [oracle.filled(gen, n, H, D, group, page, torch.bfloat16, "cuda") for n in lens]
+    whole = [torch.cat([oracle.held(s[i][b], group) for s in shards]) for i in (2, 3) for b in range(2)]
+    want, _ = oracle.attention(q[:, None], whole[:2], whole[2:], D ** -0.5)
+    vc = VirtualCluster(w, heap_bytes=1 << 26)
+    try:
+        layers = vc.collective(lambda r, env: SpGQAFlashDecodeAttention(r, 0, w, 1, Hq, H, D, D, page_size=page, scale=D ** -0.5,
+                                                                        max_allowed_batch=2, env=env))
+        n = int32(lens, "cuda")
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for out in vc.run(lambda r, env: layers[r](q, shards[r][0], None, n, shards[r][1])):
+                torch.cuda.synchronize()
+                _check(out, want[:, 0], None, None, torch.bfloat16, max(float(x.abs().max()) for x in whole[2:]))
+    finally:
+        vc.close()

@@ -34,6 +34,7 @@ ALIASES = {
     "kernels.amd.all_gather_gemm": ["ops.ag_gemm", "ops.compat_names"],
     "kernels.amd.gemm_reduce_scatter": ["ops.gemm_rs", "ops.compat_names"],
     "kernels.amd.common_ops": ["ops.common_ops"],
+    "kernels.amd.kv4": ["ops.kv4"],
     "kernels.nvidia": ["ops.compat_nvidia", "ops.allgather", "ops.moe", "ops.flash_decode", "ops.all_to_all",
                        "ops.sp_ag_attention", "ops.gemm_ar", "ops.allreduce", "ops.reduce_scatter", "ops.ep_a2a",
                        "ops.p2p", "ops.common_ops", "ops.compat_names"],

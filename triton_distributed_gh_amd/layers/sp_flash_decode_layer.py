@@ -9,6 +9,7 @@ from __future__ import annotations
 import torch
 
 from ..ops.flash_decode import gqa_fwd_batch_decode_inter_rank_combine, gqa_fwd_batch_decode_intra_rank
+from ..ops.kv4 import Int4KVCache, gqa_fwd_kv4
 from ..utils.distributed import get_env
 from .low_latency_allgather_layer import AllGatherLayer
 
@@ -42,14 +43,19 @@ class SpGQAFlashDecodeAttention(torch.nn.Module):
     def forward(self, q, k_cache, v_cache, global_kv_lens, block_table):
         """q [batch, q_heads, D] (same on every rank); k/v_cache: this rank's pages
         [pages, page_size, kv_heads, D]; global_kv_lens int32 [num_ranks, batch]; block_table
-        [batch, max_pages] for this rank's shard.  Returns [batch, q_heads, D]."""
+        [batch, max_pages] for this rank's shard.  ``k_cache`` may be this rank's pages in 4 bits (``Int4KVCache``, which
+        holds K and V; ``v_cache`` None).  Returns [batch, q_heads, D]."""
         batch = q.shape[0]
         D = self.v_head_dim
         assert global_kv_lens.shape == (self.num_ranks, batch)
         assert batch <= self.max_allowed_batch, f"only {self.max_allowed_batch} queries per decode step"
-        part = gqa_fwd_batch_decode_intra_rank(q, k_cache, v_cache, self.workspace, [1] * batch,
-                                               global_kv_lens[self.rank].contiguous(), block_table, self.scale,
-                                               soft_cap=self.soft_cap, kv_split=self.kv_split)
+        if isinstance(k_cache, Int4KVCache):
+            part = gqa_fwd_kv4(q, k_cache, global_kv_lens[self.rank].contiguous(), block_table, self.scale,
+                               soft_cap=float(self.soft_cap), kv_split=self.kv_split, return_lse=True)
+        else:
+            part = gqa_fwd_batch_decode_intra_rank(q, k_cache, v_cache, self.workspace, [1] * batch,
+                                                   global_kv_lens[self.rank].contiguous(), block_table, self.scale,
+                                                   soft_cap=self.soft_cap, kv_split=self.kv_split)
         if self.num_ranks == 1:
             return part[..., :D].to(q.dtype)
         nbytes_per_rank = part.numel() * 4

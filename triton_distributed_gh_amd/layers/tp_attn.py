@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import torch
 
-from ..ops import elementwise, flash_decode
+from ..ops import elementwise, flash_decode, kv4
 from ..ops.ag_gemm import ag_gemm_intra_node, create_ag_gemm_intra_node_context
 from ..ops.allreduce import AllReduceMethod, all_reduce, create_allreduce_ctx
 from ..ops.flash_attn import flash_attn_with_kvcache
@@ -115,6 +115,8 @@ class TP_Attn:
         """qkv [bsz, q_len, (q + 2 kv) / w] -> attention output [bsz, q_len, q / w]."""
         bsz, q_len, _ = qkv.shape
         D = self.head_dim
+        if hasattr(kv_cache, "kv4_layer"):
+            return self._attend_kv4(qkv, position_ids, cos_sin_cache, kv_cache, layer_idx)
         k_cache, v_cache, kv_offset = kv_cache.update_kv_cache(None, None, layer_idx)
         total = getattr(kv_cache, "total_len", None)
         if (total is not None and kv_offset.dtype == torch.int32 and k_cache.dim() == 4 and k_cache.shape[0] == bsz
@@ -146,6 +148,28 @@ class TP_Attn:
         k_cache, v_cache, kv_offset = kv_cache.update_kv_cache(k, v, layer_idx)
         out = flash_attn_with_kvcache(q=q, k_cache=k_cache, v_cache=v_cache, k=k, v=v, cache_seqlens=kv_offset,
                                       causal=True)
+        return out.reshape(bsz, q_len, -1)
+
+    def _attend_kv4(self, qkv: torch.Tensor, position_ids, cos_sin_cache, kv_cache, layer_idx: int) -> torch.Tensor:
+        """``_attend`` over a cache in 4 bits: one launch quantises K / V as the projection leaves them, one or two attend."""
+        bsz, q_len, _ = qkv.shape
+        D, cache = self.head_dim, kv_cache.kv4_layer(layer_idx)
+        pos = position_ids.expand(bsz, q_len)
+        if cache.dtype == torch.bfloat16:
+            q = kv4.kv4_qkv_prep(qkv, getattr(self, "q_norm_w", None), getattr(self, "k_norm_w", None),
+                                 getattr(self, "q_norm_eps", 0.0), getattr(self, "k_norm_eps", 0.0), pos, cos_sin_cache[0],
+                                 cos_sin_cache[1], cache, kv_cache.kv_offset, kv_cache.total_len, kv_cache.block_table,
+                                 self.q_size // D)
+        else:
+            q, k, v = (x.reshape(bsz, q_len, -1, D) for x in qkv.split([self.q_size, self.kv_size, self.kv_size], dim=-1))
+            if hasattr(self, "q_norm_eps"):
+                q = layer_norm(q.reshape(-1, D), self.q_norm_eps, self.q_norm_w).view(q.shape)
+            if hasattr(self, "k_norm_eps"):
+                k = layer_norm(k.reshape(-1, D), self.k_norm_eps, self.k_norm_w).view(k.shape)
+            q, k = (apply_rotary_pos_emb(x.contiguous(), cos_sin_cache, pos) for x in (q, k))
+            kv4.kv4_append(k, v, cache, kv_cache.kv_offset, kv_cache.block_table)
+            torch.add(kv_cache.kv_offset, q_len, out=kv_cache.total_len)
+        out = kv4.flash_attn_with_kv4cache(q, cache, kv_cache.total_len, kv_cache.block_table)
         return out.reshape(bsz, q_len, -1)
 
     def _all_reduce_torch(self, out):

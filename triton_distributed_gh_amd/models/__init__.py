@@ -1,7 +1,7 @@
 """Model zoo entry points (reference: python/triton_dist/models/__init__.py:25-64)."""
 from .config import KNOWN_ARCHS, ArchConfig, ModelConfig  # noqa: F401
 from .dense import DenseLLM
-from .kv_cache import KV_Cache, PagedKVCache  # noqa: F401
+from .kv_cache import KV4_Cache, KV_Cache, PagedKVCache  # noqa: F401
 from .qwen_moe import Qwen3MoE
 
 

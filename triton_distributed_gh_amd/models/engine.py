@@ -22,14 +22,19 @@ import torch.distributed as dist
 from ..ops.allreduce import AllReduceMethod
 from . import AutoLLM, AutoTokenizer
 from .config import ModelConfig
-from .kv_cache import KV_Cache
+from .kv_cache import KV4_Cache, KV_Cache
 from .utils import logger, sample_token
 
 
 class Engine:
 
     def __init__(self, model_config: ModelConfig, temperature: float = 0.0, top_p: float = 0.95, verbose: bool = False,
-                 group=None, env=None):
+                 group=None, env=None, kv_cache_bits: int = 16):
+        """``kv_cache_bits`` 4: the KV cache is held in 4 bits (``KV4_Cache``) - prompts and decode steps of every back-end write
+        and attend over it."""
+        if kv_cache_bits not in (16, 4):
+            raise ValueError(f"kv_cache_bits must be 16 or 4, got {kv_cache_bits}")
+        self.kv_cache_bits = kv_cache_bits
         self.logger = logger
         self.model_config, self.group, self.env = model_config, group, env
         self.temperature, self.top_p, self.verbose = temperature, top_p, verbose
@@ -48,9 +53,9 @@ class Engine:
 
     def _init_kv_cache(self, bsz: int):
         m = self.model
-        self.kv_cache = KV_Cache(num_layers=m.num_layers, kv_heads=m.num_key_value_heads, head_dim=m.head_dim,
-                                 batch_size=bsz, dtype=m.dtype, max_length=m.max_length, world_size=m.world_size,
-                                 device=m.device)
+        cache = KV4_Cache if self.kv_cache_bits == 4 else KV_Cache
+        self.kv_cache = cache(num_layers=m.num_layers, kv_heads=m.num_key_value_heads, head_dim=m.head_dim,
+                              batch_size=bsz, dtype=m.dtype, max_length=m.max_length, world_size=m.world_size, device=m.device)
 
     def _barrier(self):
         if self.model.device.type == "cuda":
