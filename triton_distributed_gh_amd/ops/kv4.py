@@ -246,8 +246,8 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, cache: Int4KVCache, kv_offset: 
     ``kv_offset`` int32 [batch]; ``new_lens`` (int32 [batch], optional): only the first ``new_lens[b]`` rows are tokens, the
     rest padding.  Tokens without a page are dropped.  Pages that are written must belong to one sequence: two sequences
     that write the same token of a page leave a mixture."""
-    _require(k.dim() == 4 and k.shape == v.shape and k.shape[2:] == (cache.kv_heads, cache.head_dim),
-             f"k and v must be [batch, S, {cache.kv_heads}, {cache.head_dim}], got {tuple(k.shape)} and {tuple(v.shape)}")
+    if not (k.dim() == 4 and k.shape == v.shape and k.shape[2] == cache.kv_heads and k.shape[3] == cache.head_dim):
+        raise ValueError(f"k and v must be [batch, S, {cache.kv_heads}, {cache.head_dim}], got {tuple(k.shape)} and {tuple(v.shape)}")
     batch, S = k.shape[:2]
     _check_data(cache, k=k, v=v)
     _check_index(cache, batch, block_table, kv_offset=kv_offset, new_lens=new_lens)
@@ -278,16 +278,21 @@ def kv4_qkv_prep(qkv: torch.Tensor, q_w: Optional[torch.Tensor], k_w: Optional[t
     D, Hkv = cache.head_dim, cache.kv_heads
     if cache.dtype != torch.bfloat16:
         raise TypeError(f"kv4_qkv_prep writes bf16 caches, got {cache.dtype}")
-    _require(qkv.dim() == 3 and num_q_heads > 0 and qkv.shape[2] == (num_q_heads + 2 * Hkv) * D,
-             f"qkv must be [batch, S, {(num_q_heads + 2 * Hkv) * D}], got {tuple(qkv.shape)}")
+    if not (qkv.dim() == 3 and num_q_heads > 0 and qkv.shape[2] == (num_q_heads + 2 * Hkv) * D):
+        raise ValueError(f"qkv must be [batch, S, {(num_q_heads + 2 * Hkv) * D}], got {tuple(qkv.shape)}")
     batch, S = qkv.shape[:2]
-    _check_data(cache, qkv=qkv, **{n: w for n, w in (("q_w", q_w), ("k_w", k_w)) if w is not None})
+    _check_data(cache, qkv=qkv)
     for w in (q_w, k_w):
-        _require(w is None or (w.shape == (D,) and w.is_contiguous()), f"norm weights are contiguous [{D}]")
-    _require(position_ids.shape == (batch, S) and position_ids.device == cache.device, f"position_ids must be [{batch}, {S}]")
+        if w is not None:
+            _check_data(cache, norm_weight=w)
+            if not (w.dim() == 1 and w.shape[0] == D and w.is_contiguous()):
+                raise ValueError(f"norm weights are contiguous [{D}]")
+    if not (position_ids.shape == (batch, S) and position_ids.device == cache.device):
+        raise ValueError(f"position_ids must be [{batch}, {S}] on {cache.device}")
     for t in (cos, sin):
-        _require(t.dtype == torch.float32 and t.dim() == 2 and t.shape[1] == D // 2 and t.shape[0] > 0 and t.is_contiguous()
-                 and t.device == cache.device and t.shape == cos.shape, f"cos / sin must be contiguous fp32 [positions, {D // 2}]")
+        if not (t.dtype == torch.float32 and t.dim() == 2 and t.shape[1] == D // 2 and t.shape[0] > 0 and t.is_contiguous()
+                and t.device == cache.device and t.shape == cos.shape):
+            raise ValueError(f"cos / sin must be contiguous fp32 [positions, {D // 2}] on {cache.device}")
     _check_index(cache, batch, block_table, kv_offset=kv_offset, total_out=total_out)
     if batch == 0 or S == 0:
         total_out.copy_(kv_offset)
@@ -330,10 +335,12 @@ def kv4_read(cache: Int4KVCache, block_table: torch.Tensor, cu_seqlens: torch.Te
     scale carries beyond the type's largest number comes out as that number."""
     batch = block_table.shape[0] if block_table.dim() == 2 else -1
     _check_index(cache, batch, block_table, cu_seqlens=cu_seqlens, starts=starts)
-    _require(0 <= total < 2 ** 31, f"total must be a row count, got {total}")
+    if not 0 <= total < 2 ** 31:
+        raise ValueError(f"total must be a row count, got {total}")
     shape = (int(total), cache.kv_heads, cache.head_dim)
     if out is None:
-        k, v = (torch.empty(shape, dtype=cache.dtype, device=cache.device) for _ in range(2))
+        k = torch.empty(shape, dtype=cache.dtype, device=cache.device)
+        v = torch.empty_like(k)
     else:
         k, v = out
         _check_data(cache, k_out=k, v_out=v)
@@ -416,16 +423,16 @@ def gqa_fwd_kv4(q: torch.Tensor, cache: Int4KVCache, kv_lens: torch.Tensor, bloc
     ``flash_decode.gqa_fwd_batch_decode_inter_rank_combine`` merges over ranks that hold parts of the sequences."""
     flat = q.dim() == 3
     q4 = q.unsqueeze(1) if flat else q
-    _require(q4.dim() == 4 and q4.shape[3] == cache.head_dim and q4.shape[2] > 0 and q4.shape[2] % cache.kv_heads == 0,
-             f"q must be [batch, S, heads, {cache.head_dim}] with a multiple of {cache.kv_heads} heads, got {tuple(q.shape)}")
+    if q4.dim() != 4 or q4.shape[3] != cache.head_dim or q4.shape[2] == 0 or q4.shape[2] % cache.kv_heads:
+        raise ValueError(f"q must be [batch, S, heads, {cache.head_dim}] with a multiple of {cache.kv_heads} heads, got {tuple(q.shape)}")
     batch, S, Hq, D = q4.shape
     _check_data(cache, q=q)
     _check_index(cache, batch, block_table, kv_lens=kv_lens)
-    _require(math.isfinite(soft_cap) and soft_cap >= 0, f"soft_cap must be 0 (off) or positive, got {soft_cap}")
-    _require(kv_split == -1 or 1 <= kv_split <= 65535, f"kv_split must be -1 (automatic) or 1 .. 65535, got {kv_split}")
-    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    _require(math.isfinite(scale), f"scale must be finite, got {scale}")
-    shape = (batch, S, Hq, D + 1) if return_lse else (batch, S, Hq, D)
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not (math.isfinite(scale) and math.isfinite(soft_cap) and soft_cap >= 0):
+        raise ValueError(f"scale must be finite, soft_cap 0 (off) or positive, got {scale} and {soft_cap}")
+    if not (kv_split == -1 or 1 <= kv_split <= 65535):
+        raise ValueError(f"kv_split must be -1 (automatic) or 1 .. 65535, got {kv_split}")
     if not q.is_cuda:
         out, lse = attend_reference(q4, cache, kv_lens, block_table, scale, soft_cap, causal)
         out = torch.cat([out, lse.unsqueeze(-1)], -1) if return_lse else out.to(q.dtype)
@@ -433,7 +440,8 @@ def gqa_fwd_kv4(q: torch.Tensor, cache: Int4KVCache, kv_lens: torch.Tensor, bloc
     q4 = _rows(q4)
     splits = int(kv_split) if kv_split > 0 else auto_kv_splits(batch, cache.kv_heads, Hq // cache.kv_heads * S, D,
                                                                block_table.shape[1] * cache.page_size)
-    out = torch.empty(shape, dtype=torch.float32 if return_lse else q.dtype, device=q.device)
+    out = torch.empty((batch, S, Hq, D + 1), dtype=torch.float32, device=q.device) if return_lse else \
+        torch.empty_like(q4, memory_format=torch.contiguous_format)
     part = torch.empty(batch * S * Hq * splits * (D + 1), dtype=torch.float32, device=q.device) if splits > 1 else None
     _launch("tdist_kv4_attn", cache.device, *cache._native, q4.data_ptr(), *q4.stride()[:3], block_table.data_ptr(),
             block_table.stride(0), block_table.shape[1], kv_lens.data_ptr(), _ptr(part), out.data_ptr(), batch, S, Hq, splits,
