@@ -43,10 +43,10 @@ typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 
 #ifndef KV4_WAVES
-#define KV4_WAVES(D) (D <= 128 ? 2 : 1)
+#define KV4_WAVES(D) 2
 #endif
 #ifndef KV4_RING
-#define KV4_RING(D, CB) (D <= 128 && CB == 1 ? 3 : 2)
+#define KV4_RING(D, CB) (CB == 2 || D == 256 ? 1 : 3)
 #endif
 #define INLINE __attribute__((always_inline))     // (lambdas: a call would put what they capture into memory)
 
@@ -230,9 +230,9 @@ __global__ __launch_bounds__(256, KV4_WAVES(D)) void kv4_attn_kernel(AttnArgs a,
   for (int g = 0; g < NG; ++g) vs[g] = 1.f;
   bool scaled = false;
   const Unpack u;
-  u32x4 neg0, neg1;                     // -(1024 + 8) and -(64 + 8)
+  u32x4 neg0, neg1;                     // -1024 and -64
 #pragma unroll
-  for (int i = 0; i < 4; ++i) neg0[i] = 0xe408e408u, neg1[i] = 0xd480d480u;
+  for (int i = 0; i < 4; ++i) neg0[i] = 0xe400e400u, neg1[i] = 0xd400d400u;
 
   const int* table = block_table + (long long)b * a.table_stride;
   const int last_tile = (end - 1) >> 4;
@@ -253,21 +253,26 @@ __global__ __launch_bounds__(256, KV4_WAVES(D)) void kv4_attn_kernel(AttnArgs a,
   const uint32_t k_lane = li * (D / 2) + lg * (D / 8), v_lane = lg * (2 * D) + li * (D / 8);
   const uint32_t* p_lane = (lane < 32 ? a.c.k_params : a.c.v_params) + li;      // lane: token lane & 31 of K or V
   uint32_t(*const params)[NG][32] = s_params[wave];
-  auto load = [&](const Where& w, Raw<D, NG>& r) INLINE {
+  auto load_k = [&](const Where& w, Raw<D, NG>& r) INLINE {         // and the parameters of both
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      load_words(r.k[t], a.c.k_codes + (w.row0[t] + w.off[t]) * (D / 2), k_lane);
-      load_words(r.v[t], a.c.v_codes + (w.row0[t] + w.off[t]) * (D / 2), v_lane);
-    }
+    for (int t = 0; t < 2; ++t) load_words(r.k[t], a.c.k_codes + (w.row0[t] + w.off[t]) * (D / 2), k_lane);
     const long long at0 = w.row0[0] * NG + w.off[0], at1 = w.row0[1] * NG + w.off[1];
     const uint32_t* p = p_lane + (lane & 16 ? at1 : at0);
 #pragma unroll
     for (int g = 0; g < NG; ++g) r.params[g] = p[(long long)g * a.c.page_size];
   };
+  auto load_v = [&](const Where& w, Raw<D, NG>& r) INLINE {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) load_words(r.v[t], a.c.v_codes + (w.row0[t] + w.off[t]) * (D / 2), v_lane);
+  };
+  auto load = [&](const Where& w, Raw<D, NG>& r) INLINE {
+    load_k(w, r);
+    load_v(w, r);
+  };
   // CAREFUL: the block has tokens that are not there or not seen by every column, the scores are capped, or V's scales are
   // brought near 1.  Without it the block is straight code but for the one branch on the references; false: nothing has been
-  // done, the block needs care.
-  auto compute_as = [&](auto careful, int n0, bool there0, bool there1, const Raw<D, NG>& r) INLINE -> bool {
+  // done, the block needs care.  after_k() is called when K's registers are free.
+  auto compute_as = [&](auto careful, int n0, bool there0, bool there1, const Raw<D, NG>& r, auto after_k) INLINE -> bool {
     constexpr bool CAREFUL = decltype(careful)::value;
     // ---- the block's widest V scale; the parameters of tokens that are not there may hold anything
     uint32_t param[NG];
@@ -313,6 +318,7 @@ __global__ __launch_bounds__(256, KV4_WAVES(D)) void kv4_attn_kernel(AttnArgs a,
         }
       }
     }
+    after_k();
     if (CAREFUL && a.soft_cap > 0.f) {
 #pragma unroll
       for (int cb = 0; cb < CB; ++cb)
@@ -402,17 +408,17 @@ __global__ __launch_bounds__(256, KV4_WAVES(D)) void kv4_attn_kernel(AttnArgs a,
         sc[cb][i] = exp2_fast(__builtin_fmaf(sc[cb][i], x_mul[cb], -m[cb]));      // P from here on
         l[cb] += sc[cb][i];
       }
-    // ---- O^T += V^T . P^T, group by group: value = scale (code - 8) + (low + 8 scale)
+    // ---- O^T += V^T . P^T, group by group
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-      float sv[8], zc[8];
+      float sv[8], low[8];
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const u32x4 vp = *(const u32x4*)&params[1][g][16 * t + 4 * lg];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           sv[4 * t + i] = scale_of<IS_BF16>(vp[i]);
-          zc[4 * t + i] = __builtin_fmaf(8.f, sv[4 * t + i], low_of<IS_BF16>(vp[i]));
+          low[4 * t + i] = low_of<IS_BF16>(vp[i]);
         }
       }
       if (CAREFUL) {
@@ -426,7 +432,7 @@ __global__ __launch_bounds__(256, KV4_WAVES(D)) void kv4_attn_kernel(AttnArgs a,
         for (int i = 0; i < 8; i += 2) {
           float s2[2], c2[2];
 #pragma unroll
-          for (int k = 0; k < 2; ++k) s2[k] = sc[cb][i + k] * sv[i + k], c2[k] = sc[cb][i + k] * zc[i + k];
+          for (int k = 0; k < 2; ++k) s2[k] = sc[cb][i + k] * sv[i + k], c2[k] = sc[cb][i + k] * low[i + k];
           if (CAREFUL) {                      // 0 times the NaN of a token that only other columns see
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
@@ -469,39 +475,56 @@ __global__ __launch_bounds__(256, KV4_WAVES(D)) void kv4_attn_kernel(AttnArgs a,
     return true;
   };
   // A wave's blocks are 128 tokens apart.  RING of them are in flight: while one is multiplied the next ones are on their way,
-  // and the pages of the one behind them are looked up.    Plain blocks first; from
-  // the first one that needs care on, all of them get it.
+  // and the pages of the one behind them are looked up.  With RING 1 the next block's K is fetched into the registers of this
+  // one's as soon as the scores are there, and V after the products: where two column blocks need the registers.  Plain blocks
+  // first; from the first one that needs care on, all of them get it.
   int n0 = start + 32 * wave;
   if (n0 < end) {
     fetch_q();
     constexpr int RING = KV4_RING(D, CB);
     Raw<D, NG> ring[RING];
     bool there[RING];
-#pragma unroll
-    for (int i = 0; i < RING - 1; ++i) {
-      const Where w = lookup(n0 + 128 * i);
-      load(w, ring[i]);
-      there[i] = w.there[0] && w.there[1];
-    }
-    there[RING - 1] = false;
-    Where ahead = lookup(n0 + 128 * (RING - 1));
-    prepare_q();
+    auto nothing = [] {};
     const int plain_end = a.soft_cap > 0.f ? 0 : min(full, end);
-    auto plain = [&](auto slot) INLINE -> bool {
-      constexpr int I = decltype(slot)::value, AHEAD = (I + RING - 1) % RING;
-      if (n0 + 32 > plain_end || !there[I]) return false;
-      load(ahead, ring[AHEAD]);               // (behind the last block: the last tile's page once more)
-      there[AHEAD] = ahead.there[0] && ahead.there[1];
-      ahead = lookup(n0 + 128 * RING);
-      if (!compute_as(std::false_type{}, n0, true, true, ring[I])) return false;
-      n0 += 128;
-      return true;
-    };
-    for (;;) {
-      if (!plain(std::integral_constant<int, 0>{})) break;
-      if (!plain(std::integral_constant<int, 1>{})) break;
-      if constexpr (RING > 2) {
-        if (!plain(std::integral_constant<int, 2>{})) break;
+    if constexpr (RING == 1) {
+      Where w = lookup(n0);
+      load(w, ring[0]);
+      there[0] = w.there[0] && w.there[1];
+      w = lookup(n0 + 128);
+      prepare_q();
+      while (n0 + 32 <= plain_end && there[0]) {
+        if (!compute_as(std::false_type{}, n0, true, true, ring[0], [&]() INLINE { load_k(w, ring[0]); })) break;
+        load_v(w, ring[0]);                   // (behind the last block: the last tile's page once more)
+        there[0] = w.there[0] && w.there[1];
+        w = lookup(n0 + 256);
+        n0 += 128;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < RING - 1; ++i) {
+        const Where w = lookup(n0 + 128 * i);
+        load(w, ring[i]);
+        there[i] = w.there[0] && w.there[1];
+      }
+      there[RING - 1] = false;
+      Where ahead = lookup(n0 + 128 * (RING - 1));
+      prepare_q();
+      auto plain = [&](auto slot) INLINE -> bool {
+        constexpr int I = decltype(slot)::value, AHEAD = (I + RING - 1) % RING;
+        if (n0 + 32 > plain_end || !there[I]) return false;
+        load(ahead, ring[AHEAD]);
+        there[AHEAD] = ahead.there[0] && ahead.there[1];
+        ahead = lookup(n0 + 128 * RING);
+        if (!compute_as(std::false_type{}, n0, true, true, ring[I], nothing)) return false;
+        n0 += 128;
+        return true;
+      };
+      for (;;) {
+        if (!plain(std::integral_constant<int, 0>{})) break;
+        if (!plain(std::integral_constant<int, 1>{})) break;
+        if constexpr (RING > 2) {
+          if (!plain(std::integral_constant<int, 2>{})) break;
+        }
       }
     }
     if (n0 < end) {
@@ -514,7 +537,7 @@ __global__ __launch_bounds__(256, KV4_WAVES(D)) void kv4_attn_kernel(AttnArgs a,
         load(w, next);
         const bool next0 = w.there[0], next1 = w.there[1];
         w = lookup(n0 + 256);
-        compute_as(std::true_type{}, n0, there0, there1, r);
+        compute_as(std::true_type{}, n0, there0, there1, r, nothing);
         n0 += 128;
         if (n0 >= end) break;
         r = next, there0 = next0, there1 = next1;
