@@ -109,8 +109,24 @@ __device__ __forceinline__ void load_words(uint32_t (&dst)[N], const uint8_t* ba
   }
 }
 
-// CB blocks of sixteen columns share what a wave unpacks.
-template <bool IS_BF16, int D, int G, int CB>
+// The larger of an op's two sides over the sixteen lanes of a row; every lane gets it.
+template <class Op>
+__device__ __forceinline__ float over_row(float v, Op op) {
+  auto with = [&](int moved) { v = op(v, __builtin_bit_cast(float, moved)); };
+  with(__builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0xb1, 0xf, 0xf, true));
+  with(__builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x4e, 0xf, 0xf, true));
+  with(__builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x141, 0xf, 0xf, true));
+  with(__builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x140, 0xf, 0xf, true));
+  return v;
+}
+
+// R = 0: CB blocks of sixteen columns share what a wave unpacks; scores as S^T[token, column].
+//
+// R = 1, 2: at most 4 R columns (a decode step of grouped heads).  S^T would leave three quarters or half of every register idle,
+// and all the work per score is done on registers.  Here it is S[column, token]: Q is the first operand, its columns spread
+// over the rows 4 g + i, i < R, so that lane group g holds R columns of sixteen tokens - R registers a tile where S^T has four,
+// and one token's parameters a lane where it has four's.  P goes to the second product through LDS.  Everything else is the same.
+template <bool IS_BF16, int D, int G, int CB, int R = 0>
 __global__ __launch_bounds__(256, KV4_WAVES(D)) void kv4_attn_kernel(AttnArgs a, const int* __restrict__ block_table,
                                                                         const int* __restrict__ kv_len) {
   constexpr int KS = D / 32;            // MFMA steps over the head dim = dwords of a lane per K row
@@ -122,29 +138,33 @@ __global__ __launch_bounds__(256, KV4_WAVES(D)) void kv4_attn_kernel(AttnArgs a,
   constexpr float WIDE = 0x1p3f, NARROW = 0x1p-9f;      // V scales that are taken as they are
   constexpr float AT = 6.f, MOST = 14.f;  // log2 of the largest P: where a new reference puts it, and where it may grow to
   constexpr int DC = D < 128 ? D : 128; // channels merged at a time
+  constexpr int W = R > 0 ? R : CB;     // columns of which a lane holds scores
+  static_assert(R == 0 || CB == 1, "");
   __shared__ float s_m[4][16], s_l[4][16];
   __shared__ __attribute__((aligned(16))) float s_o[4][16][DC + 4];
   __shared__ __attribute__((aligned(16))) uint32_t s_params[4][2][NG][32];
+  __shared__ __attribute__((aligned(16))) uint16_t s_p[R > 0 ? 4 : 1][NG][IS_BF16 ? 1 : 2][R > 0 ? 4 * R : 1][32];
 
   const int kvh = blockIdx.x, split = blockIdx.y;       // (kv heads first: what shares a cache line's XCD shares its L2)
   const int z = a.first + (int)blockIdx.z;
   const int cblk = a.batch == 1 ? z : z / a.batch, b = z - cblk * a.batch;
   const int group = a.group, columns = group * a.S;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, lg = lane >> 4;
-  const int col0 = cblk * 16 * CB;
+  constexpr int COLUMNS = R > 0 ? 4 * R : 16 * CB;
+  const int col0 = cblk * COLUMNS;
 
   // tokens: a column sees [0, limit), the workgroup's columns [0, len), none of them misses one below `full`
   const long long room = (long long)a.max_pages * a.c.page_size;
   const int L = (int)min((long long)max(kv_len[b], 0), room);
   const bool one = a.S == 1;                  // (columns are heads: no division by a variable on the way to the first load)
-  const int s_first = one ? 0 : col0 / group, s_last = one ? 0 : min(col0 + 16 * CB - 1, columns - 1) / group;
+  const int s_first = one ? 0 : col0 / group, s_last = one ? 0 : min(col0 + COLUMNS - 1, columns - 1) / group;
   const int len = max(0, a.causal ? L - a.S + s_last + 1 : L);
   const int full = a.causal ? L - a.S + s_first + 1 : L;
   const int per = a.splits == 1 ? len : ((len + a.splits - 1) / a.splits + 127) & ~127;
   const int start = (int)min((long long)split * per, (long long)len), end = min(len, start + per);
   if (a.splits > 1 && start >= end) {         // (the merge does not look at the sums of a split without tokens)
     const int col = col0 + (int)threadIdx.x;
-    if (threadIdx.x < 16 * CB && col < columns)
+    if (threadIdx.x < COLUMNS && col < columns)
       a.partial_lse[(((long long)b * a.S + (one ? 0 : col / group)) * a.q_heads + kvh * group + (one ? col : col % group)) * a.splits +
                     split] = -INFINITY;
     return;
@@ -152,18 +172,27 @@ __global__ __launch_bounds__(256, KV4_WAVES(D)) void kv4_attn_kernel(AttnArgs a,
 
   // Q as fp16: bf16 rows are brought near 2^8 by a power of two per column, which loses nothing that a score could show
   // (numbers 2^-32 of the column's largest).  A negative scale turns Q's sign, so that larger scores are larger weights.
-  int limit[CB];
+  int limit[W];
   u32x4 q[CB][KS];
-  float qsum[CB][NG], qk[CB];
+  float qsum[W][NG], qk[W];
   f32x4 c0[CB][NG];                           // what the accumulators start at
   u32x4 raw[CB][KS];
   auto fetch_q = [&]() INLINE {
 #pragma unroll
     for (int cb = 0; cb < CB; ++cb) {
-      const int col = col0 + cb * 16 + li;
-      const bool col_ok = col < columns;
+      // the column of this lane's operand row, and of its scores
+      const int col = R > 0 ? col0 + (li >> 2) * R + (li & 3) : col0 + cb * 16 + li;
+      const bool col_ok = col < columns && (R == 0 || (li & 3) < R);
       const int row_s = one || !col_ok ? 0 : col / group, head = kvh * group + (col_ok ? col - row_s * group : 0);
-      limit[cb] = !col_ok ? 0 : a.causal ? L - a.S + row_s + 1 : L;
+      if constexpr (R == 0) {
+        limit[cb] = !col_ok ? 0 : a.causal ? L - a.S + row_s + 1 : L;
+      } else {
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+          const int mine = col0 + lg * R + i;
+          limit[i] = mine >= columns ? 0 : a.causal && !one ? L - a.S + mine / group + 1 : L;
+        }
+      }
       const uint16_t* qp = a.q + b * a.q_sb + row_s * a.q_ss + head * a.q_sh + lg * 8;
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
@@ -192,7 +221,13 @@ __global__ __launch_bounds__(256, KV4_WAVES(D)) void kv4_attn_kernel(AttnArgs a,
         mul = sign * __builtin_bit_cast(float, (uint32_t)(127 + 8 - e) << 23);
         back = __builtin_bit_cast(float, (uint32_t)(127 - 8 + e) << 23);
       }
-      qk[cb] = fmaxf(lead * back, 1e-37f);    // (never 0: a masked score is -inf, and stays that)
+      const float factor = fmaxf(lead * back, 1e-37f);      // (never 0: a masked score is -inf, and stays that)
+      if constexpr (R == 0) {
+        qk[cb] = factor;
+      } else {
+#pragma unroll
+        for (int i = 0; i < R; ++i) qk[i] = __shfl(factor, 4 * lg + i);
+      }
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
         float sum0 = 0.f, sum1 = 0.f;         // of the channels that unpack as 1024 + code, and as 64 + code
@@ -209,23 +244,41 @@ __global__ __launch_bounds__(256, KV4_WAVES(D)) void kv4_attn_kernel(AttnArgs a,
         sum0 += __shfl_xor(sum0, 32);
         sum1 += __shfl_xor(sum1, 16);
         sum1 += __shfl_xor(sum1, 32);
-        qsum[cb][g] = sum0 + sum1;
         const float c = -1024.f * sum0 - 64.f * sum1;
-        c0[cb][g] = f32x4{c, c, c, c};
+        if constexpr (R == 0) {
+          qsum[cb][g] = sum0 + sum1;
+          c0[cb][g] = f32x4{c, c, c, c};
+        } else {
+          c0[cb][g] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int i = 0; i < R; ++i) qsum[i][g] = __shfl(sum0 + sum1, 4 * lg + i), c0[cb][g][i] = __shfl(c, 4 * lg + i);
+        }
       }
     }
   };
 
-  float m[CB], l[CB], corr[CB][NG], vs[NG];
+  float m[W], l[W], corr[W][NG], vs[NG];
   f32x4 o[CB][NT];
 #pragma unroll
-  for (int cb = 0; cb < CB; ++cb) {
-    m[cb] = NONE, l[cb] = 0.f;
+  for (int cb = 0; cb < CB; ++cb)
 #pragma unroll
     for (int j = 0; j < NT; ++j) o[cb][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int g = 0; g < NG; ++g) corr[cb][g] = 0.f;
+  for (int i = 0; i < W; ++i) {
+    m[i] = NONE, l[i] = 0.f;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) corr[i][g] = 0.f;
   }
+  // a value of column li's score lane, for R > 0 (R registers of lane group li / R)
+  auto of_column = [&](const float (&v)[W]) INLINE -> float {
+    const int from = 16 * ((li / (R > 0 ? R : 1)) & 3);
+    float r = __shfl(v[0], from);
+    if constexpr (R == 2) {
+      const float other = __shfl(v[W - 1], from);
+      r = li & 1 ? other : r;
+    }
+    return r;
+  };
 #pragma unroll
   for (int g = 0; g < NG; ++g) vs[g] = 1.f;
   bool scaled = false;
@@ -269,27 +322,65 @@ __global__ __launch_bounds__(256, KV4_WAVES(D)) void kv4_attn_kernel(AttnArgs a,
     load_k(w, r);
     load_v(w, r);
   };
-  // CAREFUL: the block has tokens that are not there or not seen by every column, the scores are capped, or V's scales are
-  // brought near 1.  Without it the block is straight code but for the one branch on the references; false: nothing has been
-  // done, the block needs care.  after_k() is called when K's registers are free.
-  auto compute_as = [&](auto careful, int n0, bool there0, bool there1, const Raw<D, NG>& r, auto after_k) INLINE -> bool {
+  // V scales far from 1 are brought there by a power of two per group, the same for all columns; `widest` becomes the widest
+  // after that.  false: they are far from 1, and the block is not treated as one that needs care.
+  auto rescale = [&](auto careful, const uint32_t (&param)[NG], float (&ratio)[NG], float& widest) INLINE -> bool {
     constexpr bool CAREFUL = decltype(careful)::value;
-    // ---- the block's widest V scale; the parameters of tokens that are not there may hold anything
-    uint32_t param[NG];
-    float widest = 0x1p-20f;
+    bool off = false;
+    if (!CAREFUL) {
 #pragma unroll
-    for (int g = 0; g < NG; ++g) param[g] = r.params[g];
-    if (CAREFUL) {
-      const bool live = (lane & 16 ? there1 : there0) && n0 + (lane & 31) < end;
-#pragma unroll
-      for (int g = 0; g < NG; ++g) param[g] = live ? param[g] : 0u;
+      for (int g = 0; g < NG; ++g) {
+        const float w = max_upper_half(fmaxf(0.f, scale_of<IS_BF16>(param[g])));
+        off |= w > WIDE || (w > 0.f && w < NARROW);
+      }
+      if (off) return false;
     }
+    widest = 0x1p-20f;
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-      params[lane >> 5][g][lane & 31] = param[g];
-      widest = fmaxf(widest, CAREFUL ? scale_of<IS_BF16>(param[g]) * vs[g] : scale_of<IS_BF16>(param[g]));
+      ratio[g] = 1.f;
+      const float w = max_upper_half(fmaxf(0.f, scale_of<IS_BF16>(param[g]) * vs[g]));
+      if (CAREFUL && (w > WIDE || (w > 0.f && w < NARROW))) {
+        const int have = (int)(__builtin_bit_cast(uint32_t, vs[g]) >> 23) - 127;
+        int e = (int)(__builtin_bit_cast(uint32_t, w) >> 23) - 127;
+        e = min(max(e, -60), 60);           // (what is further off takes several blocks to arrive)
+        e = min(max(e, have - 120), have + 120);
+        ratio[g] = __builtin_bit_cast(float, (uint32_t)(127 - e) << 23);
+        vs[g] *= ratio[g];
+      }
+      off |= vs[g] != 1.f;
+      widest = fmaxf(widest, w * ratio[g]);
     }
-    widest = max_upper_half(widest);
+    scaled |= off;
+    return true;
+  };
+  // O^T += V^T . P^T for the channels of group g
+  auto multiply_v = [&](int g, const Raw<D, NG>& r, const u32x4 (&hi)[CB], const u32x4 (&lo)[CB]) INLINE {
+#pragma unroll
+    for (int j = g * GT; j < (g + 1) * GT; ++j) {
+      const int h = j / 4, n = j % 4;
+      uint32_t w[4] = {r.v[0][2 * h], r.v[0][2 * h + 1], r.v[1][2 * h], r.v[1][2 * h + 1]};
+      if (n >= 2) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] >>= 8;
+      }
+      const u32x4 v = n & 1 ? u32x4{u.odd(w[0]), u.odd(w[1]), u.odd(w[2]), u.odd(w[3])}
+                            : u32x4{u.even(w[0]), u.even(w[1]), u.even(w[2]), u.even(w[3])};
+#pragma unroll
+      for (int cb = 0; cb < CB; ++cb) {
+        o[cb][j] = mfma(n & 1 ? neg1 : neg0, hi[cb], o[cb][j]);
+        o[cb][j] = mfma(v, hi[cb], o[cb][j]);
+        if constexpr (!IS_BF16) {
+          o[cb][j] = mfma(n & 1 ? neg1 : neg0, lo[cb], o[cb][j]);
+          o[cb][j] = mfma(v, lo[cb], o[cb][j]);
+        }
+      }
+    }
+  };
+  // the rest of a block, its parameters in LDS
+  auto wide_ = [&](auto careful, int n0, bool there0, bool there1, const Raw<D, NG>& r, const uint32_t (&param)[NG], float widest,
+                   auto after_k) INLINE -> bool {
+    constexpr bool CAREFUL = decltype(careful)::value;
     // ---- scores of token n0 + 16 t + 4 lg + i, column li of each block: sum(q value), still to be times qk
     float sc[CB][8];
 #pragma unroll
@@ -354,34 +445,8 @@ __global__ __launch_bounds__(256, KV4_WAVES(D)) void kv4_attn_kernel(AttnArgs a,
       raise |= __builtin_fmaf(top, x_mul[cb], wide) > m[cb] + MOST;
     }
     if (__any(raise)) {
-      // scales far from 1 are brought there by a power of two per group, the same for all columns
       float ratio[NG];
-      bool off = false;
-      if (!CAREFUL) {
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          const float w = max_upper_half(fmaxf(0.f, scale_of<IS_BF16>(param[g])));
-          off |= w > WIDE || (w > 0.f && w < NARROW);
-        }
-        if (off) return false;
-      }
-      widest = 0x1p-20f;
-#pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        ratio[g] = 1.f;
-        const float w = max_upper_half(fmaxf(0.f, scale_of<IS_BF16>(param[g]) * vs[g]));
-        if (CAREFUL && (w > WIDE || (w > 0.f && w < NARROW))) {
-          const int have = (int)(__builtin_bit_cast(uint32_t, vs[g]) >> 23) - 127;
-          int e = (int)(__builtin_bit_cast(uint32_t, w) >> 23) - 127;
-          e = min(max(e, -60), 60);           // (what is further off takes several blocks to arrive)
-          e = min(max(e, have - 120), have + 120);
-          ratio[g] = __builtin_bit_cast(float, (uint32_t)(127 - e) << 23);
-          vs[g] *= ratio[g];
-        }
-        off |= vs[g] != 1.f;
-        widest = fmaxf(widest, w * ratio[g]);
-      }
-      scaled |= off;
+      if (!rescale(careful, param, ratio, widest)) return false;
       const float now = log2_fast(widest);
 #pragma unroll
       for (int cb = 0; cb < CB; ++cb) {
@@ -451,28 +516,142 @@ __global__ __launch_bounds__(256, KV4_WAVES(D)) void kv4_attn_kernel(AttnArgs a,
           }
         }
       }
+      multiply_v(g, r, hi, lo);
+    }
+    return true;
+  };
+  auto narrow = [&](auto careful, int n0, bool there0, bool there1, const Raw<D, NG>& r, const uint32_t (&param)[NG], float widest,
+                    auto after_k) INLINE -> bool {
+    constexpr bool CAREFUL = decltype(careful)::value;
+    // ---- scores of token n0 + 16 t + li, column lg R + i
+    float sc[2][W];
 #pragma unroll
-      for (int j = g * GT; j < (g + 1) * GT; ++j) {
-        const int h = j / 4, n = j % 4;
-        uint32_t w[4] = {r.v[0][2 * h], r.v[0][2 * h + 1], r.v[1][2 * h], r.v[1][2 * h + 1]};
-        if (n >= 2) {
+    for (int t = 0; t < 2; ++t) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) w[i] >>= 8;
+      for (int g = 0; g < NG; ++g) {
+        const uint32_t kp = params[0][g][16 * t + li];
+        f32x4 acc = c0[0][g];
+#pragma unroll
+        for (int s = g * GS; s < (g + 1) * GS; ++s) {
+          const uint32_t w = r.k[t][s], w8 = w >> 8;
+          acc = mfma(q[0][s], u32x4{u.even(w), u.odd(w), u.even(w8), u.odd(w8)}, acc);
         }
-        const u32x4 v = n & 1 ? u32x4{u.odd(w[0]), u.odd(w[1]), u.odd(w[2]), u.odd(w[3])}
-                              : u32x4{u.even(w[0]), u.even(w[1]), u.even(w[2]), u.even(w[3])};
+        const float s = scale_of<IS_BF16>(kp), low = low_of<IS_BF16>(kp);
 #pragma unroll
-        for (int cb = 0; cb < CB; ++cb) {
-          o[cb][j] = mfma(n & 1 ? neg1 : neg0, hi[cb], o[cb][j]);
-          o[cb][j] = mfma(v, hi[cb], o[cb][j]);
-          if constexpr (!IS_BF16) {
-            o[cb][j] = mfma(n & 1 ? neg1 : neg0, lo[cb], o[cb][j]);
-            o[cb][j] = mfma(v, lo[cb], o[cb][j]);
-          }
+        for (int i = 0; i < W; ++i) {
+          const float first = g == 0 ? low * qsum[i][g] : __builtin_fmaf(low, qsum[i][g], sc[t][i]);
+          sc[t][i] = __builtin_fmaf(s, acc[i], first);
         }
       }
     }
+    after_k();
+    if (CAREFUL && a.soft_cap > 0.f) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < W; ++i) {         // as above
+          const float e = exp2_fast(2.f * LOG2E * qk[i] * sc[t][i]);
+          sc[t][i] = a.soft_cap * LOG2E * (1.f - 2.f * __builtin_amdgcn_rcpf(e + 1.f));
+        }
+    }
+    float x_mul[W];
+    bool seen[2][W];
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      x_mul[i] = CAREFUL && a.soft_cap > 0.f ? 1.f : qk[i];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        seen[t][i] = !CAREFUL || ((t ? there1 : there0) && n0 + 16 * t + li < min(limit[i], end));
+        if (CAREFUL) sc[t][i] = seen[t][i] ? sc[t][i] : -INFINITY;
+      }
+    }
+    const float wide = log2_fast(widest);
+    bool raise = false;
+#pragma unroll
+    for (int i = 0; i < W; ++i) raise |= __builtin_fmaf(fmaxf(sc[0][i], sc[1][i]), x_mul[i], wide) > m[i] + MOST;
+    if (__any(raise)) {
+      float ratio[NG];
+      if (!rescale(careful, param, ratio, widest)) return false;
+      const float now = log2_fast(widest);
+      float f[W];
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        const float top = over_row(fmaxf(sc[0][i], sc[1][i]), [](float a, float b) { return fmaxf(a, b); });
+        const float at = __builtin_fmaf(top, x_mul[i], now);
+        const float to = at > m[i] + MOST ? at - AT : m[i];
+        f[i] = exp2_fast(m[i] - to);
+        m[i] = to;
+        l[i] *= f[i];
+#pragma unroll
+        for (int g = 0; g < NG; ++g) corr[i][g] *= f[i];
+      }
+      const float mine = of_column(f);
+#pragma unroll
+      for (int j = 0; j < NT; ++j) o[0][j] *= mine * ratio[j / GT];
+    }
+#pragma unroll
+    for (int i = 0; i < W; ++i)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        sc[t][i] = exp2_fast(__builtin_fmaf(sc[t][i], x_mul[i], -m[i]));        // P from here on
+        l[i] += sc[t][i];
+      }
+    // P to the order in which V's tokens are contracted: token 4 g + k of tile t is element 8 g + 4 t + k
+    uint16_t(*const ps)[IS_BF16 ? 1 : 2][R > 0 ? 4 * R : 1][32] = s_p[R > 0 ? wave : 0];
+    const int put = (li >> 2) * 8 + (li & 3), column = li & (4 * W - 1);
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const uint32_t vp = params[1][g][16 * t + li];
+        float sv = scale_of<IS_BF16>(vp);
+        const float low = low_of<IS_BF16>(vp);
+        if (CAREFUL) sv *= vs[g];
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+          float s1 = sc[t][i] * sv, c1 = sc[t][i] * low;
+          if (CAREFUL) s1 = seen[t][i] ? s1 : 0.f, c1 = seen[t][i] ? c1 : 0.f;
+          corr[i][g] += c1;
+          const _Float16 h = (_Float16)s1;
+          ps[g][0][lg * W + i][put + 4 * t] = __builtin_bit_cast(uint16_t, h);
+          if constexpr (!IS_BF16) ps[g][1][lg * W + i][put + 4 * t] = __builtin_bit_cast(uint16_t, (_Float16)(s1 - (float)h));
+        }
+      }
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      u32x4 hi[CB], lo[CB];
+      hi[0] = *(const u32x4*)&ps[g][0][column][8 * lg];
+      if constexpr (!IS_BF16) lo[0] = *(const u32x4*)&ps[g][1][column][8 * lg];
+      multiply_v(g, r, hi, lo);
+    }
     return true;
+  };
+  // CAREFUL: the block has tokens that are not there or not seen by every column, the scores are capped, or V's scales are
+  // brought near 1.  Without it the block is straight code but for the one branch on the references; false: nothing has been
+  // done, the block needs care.  after_k() is called when K's registers are free.
+  auto compute_as = [&](auto careful, int n0, bool there0, bool there1, const Raw<D, NG>& r, auto after_k) INLINE -> bool {
+    constexpr bool CAREFUL = decltype(careful)::value;
+    // ---- the block's widest V scale; the parameters of tokens that are not there may hold anything
+    uint32_t param[NG];
+    float widest = 0x1p-20f;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) param[g] = r.params[g];
+    if (CAREFUL) {
+      const bool live = (lane & 16 ? there1 : there0) && n0 + (lane & 31) < end;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) param[g] = live ? param[g] : 0u;
+    }
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      params[lane >> 5][g][lane & 31] = param[g];
+      widest = fmaxf(widest, CAREFUL ? scale_of<IS_BF16>(param[g]) * vs[g] : scale_of<IS_BF16>(param[g]));
+    }
+    widest = max_upper_half(widest);
+    if constexpr (R > 0) {
+      return narrow(careful, n0, there0, there1, r, param, widest, after_k);
+    } else {
+      return wide_(careful, n0, there0, there1, r, param, widest, after_k);
+    }
   };
   // A wave's blocks are 128 tokens apart.  RING of them are in flight: while one is multiplied the next ones are on their way,
   // and the pages of the one behind them are looked up.  With RING 1 the next block's K is fetched into the registers of this
@@ -548,15 +727,33 @@ __global__ __launch_bounds__(256, KV4_WAVES(D)) void kv4_attn_kernel(AttnArgs a,
   // ---- merge: one column's sums are spread over the four lane groups, then over the four waves
 #pragma unroll
   for (int cb = 0; cb < CB; ++cb) {
-    l[cb] += __shfl_xor(l[cb], 16);
-    l[cb] += __shfl_xor(l[cb], 32);
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      corr[cb][g] += __shfl_xor(corr[cb][g], 16);
-      corr[cb][g] += __shfl_xor(corr[cb][g], 32);
-    }
+    float low_sum[NG];                        // of column li
     if (cb) __syncthreads();
-    if (lg == 0) s_m[wave][li] = m[cb], s_l[wave][li] = l[cb];
+    if constexpr (R == 0) {
+      l[cb] += __shfl_xor(l[cb], 16);
+      l[cb] += __shfl_xor(l[cb], 32);
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        low_sum[g] = corr[cb][g] + __shfl_xor(corr[cb][g], 16);
+        low_sum[g] += __shfl_xor(low_sum[g], 32);
+      }
+      if (lg == 0) s_m[wave][li] = m[cb], s_l[wave][li] = l[cb];
+    } else {
+      auto add = [](float a, float b) { return a + b; };
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        l[i] = over_row(l[i], add);
+        if (li == 0) s_m[wave][lg * W + i] = m[i], s_l[wave][lg * W + i] = l[i];
+      }
+      if (lg == 0 && li >= 4 * W) s_m[wave][li] = NONE, s_l[wave][li] = 0.f;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        float v[W];
+#pragma unroll
+        for (int i = 0; i < W; ++i) v[i] = over_row(corr[i][g], add);
+        low_sum[g] = of_column(v);
+      }
+    }
     __syncthreads();
     // thread (column mc, part): channels part * 4 + 64 i of that column
     const int mc = threadIdx.x >> 4, part = threadIdx.x & 15;
@@ -581,11 +778,11 @@ __global__ __launch_bounds__(256, KV4_WAVES(D)) void kv4_attn_kernel(AttnArgs a,
         f32x4 v = o[cb][j];
         const float undo = 1.f / vs[j / GT];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = __builtin_fmaf(v[i], undo, corr[cb][j / GT]);
+        for (int i = 0; i < 4; ++i) v[i] = __builtin_fmaf(v[i], undo, low_sum[j / GT]);
         *(f32x4*)&s_o[wave][li][(j - d0 / 16) * 16 + 4 * lg] = v;
       }
       __syncthreads();
-      if (mcol < columns) {
+      if (mcol < columns && mc < COLUMNS) {
 #pragma unroll
         for (int i = 0; i < DC / 64; ++i) {
           const int ch = part * 4 + 64 * i;
@@ -605,7 +802,7 @@ __global__ __launch_bounds__(256, KV4_WAVES(D)) void kv4_attn_kernel(AttnArgs a,
         }
       }
     }
-    if (mcol < columns && part == 0) {
+    if (mcol < columns && mc < COLUMNS && part == 0) {
       if (a.splits > 1) a.partial_lse[row * a.splits + split] = lse;
       else if (a.out_mode == 2) ((float*)a.out)[row * (D + 1) + D] = lse * LN2;
     }
@@ -707,8 +904,8 @@ TDIST_API int tdist_kv4_attn(const void* k_codes, const void* v_codes, const voi
   TDIST_REQUIRE(q && table && kv_len && out, "null argument");
   TDIST_REQUIRE(((uintptr_t)q & 15) == 0 && ((uintptr_t)out & 7) == 0 && ((q_sb | q_ss | q_sh) & 7) == 0,
                 "q rows must keep 16-byte alignment");
-  const long long columns = (long long)(q_heads / kv_heads) * S, per_group = columns > 16 && head_dim <= 128 ? 2 : 1;
-  const long long blocks = (columns + 16 * per_group - 1) / (16 * per_group) * batch;
+  const long long columns = (long long)(q_heads / kv_heads) * S, per_group = columns <= 4 ? 4 : columns <= 8 ? 8 : columns > 16 && head_dim <= 128 ? 32 : 16;
+  const long long blocks = (columns + per_group - 1) / per_group * batch;
   TDIST_REQUIRE(blocks < (1ll << 31) && columns < (1ll << 30) && (long long)batch * S * q_heads < (1ll << 31), "too many query rows");
   a.q = (const uint16_t*)q, a.partial = partial, a.out = out;
   a.page_tiles = page_size / 16;
@@ -726,9 +923,11 @@ TDIST_API int tdist_kv4_attn(const void* k_codes, const void* v_codes, const voi
     constexpr bool BF = decltype(bf)::value;
     constexpr int D = decltype(d)::value, G = decltype(g)::value;
     if constexpr (D <= 128) {
-      if (per_group == 2) return launch(kv4_attn_kernel<BF, D, G, 2>);
+      if (per_group == 32) return launch(kv4_attn_kernel<BF, D, G, 2>);
     }
-    launch(kv4_attn_kernel<BF, D, G, 1>);
+    if (per_group == 4) launch(kv4_attn_kernel<BF, D, G, 1, 1>);
+    else if (per_group == 8) launch(kv4_attn_kernel<BF, D, G, 1, 2>);
+    else launch(kv4_attn_kernel<BF, D, G, 1>);
   });
   TDIST_REQUIRE(ok, "head_dim 64 / 128 / 256 with groups of 32 / 64 / 128 channels (at most head_dim)");
   TDIST_HIP_TRY(hipGetLastError());
