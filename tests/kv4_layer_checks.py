@@ -49,7 +49,7 @@ def attention_layer(device, dtype):
         rows = [kv4._load_reference(cache, torch.full_like(at, b), at, table)[1:] for b in range(B)]
         want, _ = oracle.attention(queries[0], [k for k, _ in rows], [v for _, v in rows], D ** -0.5)
         got = out.view(B, S, Hq, D).double().cpu()
-        assert ((got - want).abs() <= oracle.bounds(want, dtype, float(rows[0][1].abs().max()))).all()
+        assert ((got - want).abs() <= oracle.bounds(want, dtype, float(rows[0][1].abs().max()), dtype)).all()
         # the 16-bit cache's rows, rounded by the definition: a norm that rounds the other way in 64 bits may move a code by one,
         # or a group's scale and low by a rounding (two of 16 bits, 16 steps of the scale's: less than a step together)
         for b in range(B):

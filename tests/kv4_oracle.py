@@ -76,11 +76,19 @@ def filled(gen, lens, kv_heads, D, group, page, dtype=torch.bfloat16, device="cp
     return cache, table, [k[b, :n] for b, n in enumerate(lens)], [v[b, :n] for b, n in enumerate(lens)]
 
 
-def bounds(ref: torch.Tensor, dtype, v_max: float) -> torch.Tensor:
-    """How far an output may be from its 64-bit value: half a step of its type (eps / 2, relative), and what 32-bit scores and
-    a 16-significant-bit P leave.  A score is a chain of D / 32 MFMA accumulations and a few fp32 operations on magnitudes of
-    at most 31 sum|q| (about 31 * 0.8 * 256 = 6350 codes for unit q of 256 channels): at most 8 * 2^-24 * 6350 = 3.1e-3 codes,
-    times a scale of at most 1 and 1 / sqrt(256) = 2e-4 of a nat at the very worst.  An error e of every weight moves the
-    output by at most 2 e max|v| = 4e-4 max|v| < 2^-11 max|v|; P's 2^-17 and the exponentials' 2^-22 are small beside it."""
+def bounds(ref: torch.Tensor, dtype, v_max, cache_dtype=torch.bfloat16, scores: float = 1.0) -> torch.Tensor:
+    """How far an output may be from its 64-bit value: half a step of its type (eps / 2, relative), and what the scores and the
+    weights leave.  ``v_max``: the largest |V|, a number or one per channel; ``scores``: scale times size of q, over 1 / sqrt(D).
+
+    Weights.  P * scale is one fp16 number where the cache is bf16: half a step, 2^-11 of the weight, times a code's 15 * scale,
+    a group's range of at most 2 v_max: 2^-10 v_max (a remainder in a second number for fp16 caches: 2^-21).
+
+    Scores.  codes are summed with 1024 added to half of them, in fp32: the accumulator passes through about 1024 times the
+    signed sum of a group's even channels of q, for `rows` 1024 * sqrt(64) * 1.1 = 9e3 in groups of 128, and is rounded
+    some 8 times in each of 4 products: 2^-24 / sqrt(3) * 9e3 * sqrt(32) = 1.8e-3 codes, times a scale of 0.5 and 1 / sqrt(128)
+    that is 8e-5 of a nat, independent from token to token (one standard deviation).  Errors e of two weights p and 1 - p move
+    the output by p (1 - p) (e1 - e2) (v1 - v2) <= 1 / 4 * sqrt(2) * 8e-5 * 2 v_max = 5.7e-5 v_max, more tokens average it:
+    2^-11 v_max are more than eight deviations."""
     half = torch.finfo(dtype).eps / 2
-    return half * ref.abs() + 2.0 ** -11 * v_max
+    weights = 2.0 ** -10 if cache_dtype == torch.bfloat16 else 2.0 ** -21
+    return half * ref.abs() + (scores * 2.0 ** -11 + weights) * v_max

@@ -1,21 +1,29 @@
 // GQA attention of the last tokens of each sequence over a 4-bit KV cache (format and layout: tdist/kv4.hpp).
 //
-// One workgroup of four waves takes one (sequence, KV head, block of sixteen query columns, KV split); a column is one
-// (new token, query head) of the `group` heads that share the KV head.  A wave walks 32-token blocks with a softmax state
-// of its own; the four states are merged through LDS, the splits by a second launch.
+// One workgroup of four waves takes one (sequence, KV head, block of query columns, KV split); a column is one (new token,
+// query head) of the `group` heads that share the KV head.  A wave walks 32-token blocks, 128 tokens apart, with a softmax
+// state of its own; the four states are merged through LDS, the splits by a second launch.
 //
-//   S^T[token, column] = K . Q^T.  A dword of K codes becomes four registers of two 16-bit numbers 16 + code (the code
-//   is put into the significand of 16.0: a shift and one and-or each), which is what a 16x16x32 MFMA takes.  The
-//   accumulator starts at -16 sum(q) of the group, so what comes out is sum(q code), and with a token's scale and low
+//   S^T[token, column] = K . Q^T.  A dword of K codes becomes four registers of two fp16 numbers, 1024 + code or 64 + code: the
+//   code is put into the significand, one and-or for two codes and one shift for eight.  They are exact, and what a 16x16x32
+//   MFMA takes.  The accumulator starts at -1024 and -64 times the sums of q that the offsets add, so what comes out is
+//   sum(q code), and with a token's scale and low
 //       s = scale * sum(q code) + low * sum(q).
-//   O^T[channel, column] = V^T . P^T.  The scale belongs to a token, the axis that is summed: it goes into P.  P * scale is
-//   split into two bf16 numbers (high and low part, 16 significant bits together) and multiplied twice: a single 8-bit
-//   rounding of P would be as large as the rounding of the result.  The 16 of 16 + code and low come off at the end:
-//       O = sum(p scale (16 + code)) + sum(p (low - 16 scale)).
-//   The 32 tokens of a block are contracted in the order in which the S^T accumulators hold them, which is how the V
-//   codes are stored, so neither side moves between lanes.
-// The running maximum is only raised (and the sums rescaled) when a score exceeds it by 2^8: P up to 256 costs nothing
-// in floating point, and the cross-lane maximum leaves the loop.
+//   O^T[channel, column] = V^T . P^T.  The scale belongs to a token, the axis that is summed: it goes into P, and P * scale is
+//   rounded to fp16.  A step of that, 2^-11 of a weight, is an eighth of the bf16 result's own; for fp16 caches, whose result
+//   has steps of 2^-11 too, the remainder is a second fp16 number.  A product of the same P with -1024 or -64 takes the
+//   offsets off in the accumulator, where they and the code have met the same rounded weight.  sum(p low) is kept beside.
+//   The 32 tokens of a block are contracted in the order in which the S^T accumulators hold them, which is how the V codes
+//   are stored, so neither side moves between lanes.
+// The reference m of the exponentials is raised only when a P * scale would pass 2^14 (fp16 ends at 2^16), and then put where
+// the largest is 2^6: the cross-lane maximum leaves the loop, and a weight keeps all its bits down to 2^-20 of the largest
+// (2^-8 in a group of 2^-12 of the widest scale; groups further apart, or far from 1, get a power of two each).
+//
+// What bounds it: many sequences, the bytes of the cache (64 x 4096 tokens, 8 heads of 128: 286 MB in 58 us, 4.9 TB/s, a copy's
+// rate on the same card); one long sequence of 131072, those and the two launches' start and end (151 MB in 35 .. 37 us,
+// 4.1 .. 4.3 TB/s); a few tokens, the launches (6.5 us); many columns, the vector instructions of unpacking and softmax (1024
+// new tokens over 16384, 266 GFLOP: 511 us, 520 TFLOP/s, against 1203 of a large bf16 matrix product).  bf16 high and low
+// parts of 16 + code, what this began with, took 103 us for the first of these.
 #include <algorithm>
 
 #include "tdist/kv4.hpp"
@@ -42,12 +50,10 @@ struct AttnArgs {
 typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 
-#ifndef KV4_WAVES
-#define KV4_WAVES(D) 2
-#endif
-#ifndef KV4_RING
-#define KV4_RING(D, CB) (CB == 2 || D == 256 ? 1 : 3)
-#endif
+// Blocks a wave has in flight.  Three where the registers hold them (131072 tokens: 37.5 us); one where two column blocks or
+// heads of 256 channels need the registers (chunk of 1024 511 us against 531 with two, heads of 256 50.3 against 53.9).
+constexpr int ring_of(int D, int CB) { return CB == 2 || D == 256 ? 1 : 3; }
+
 #define INLINE __attribute__((always_inline))     // (lambdas: a call would put what they capture into memory)
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -120,15 +126,18 @@ __device__ __forceinline__ float over_row(float v, Op op) {
   return v;
 }
 
-// R = 0: CB blocks of sixteen columns share what a wave unpacks; scores as S^T[token, column].
+// R = 0: CB blocks of sixteen columns share what a wave unpacks; scores as S^T[token, column].  Two blocks where there are more
+// than sixteen columns (chunk of 1024: 1007 us with one, 532 with two and the loop as straight code); for heads of 256 the
+// second block's sums do not fit the registers, and one is faster.
 //
 // R = 1, 2: at most 4 R columns (a decode step of grouped heads).  S^T would leave three quarters or half of every register idle,
 // and all the work per score is done on registers.  Here it is S[column, token]: Q is the first operand, its columns spread
 // over the rows 4 g + i, i < R, so that lane group g holds R columns of sixteen tokens - R registers a tile where S^T has four,
 // and one token's parameters a lane where it has four's.  P goes to the second product through LDS.  Everything else is the same.
+// 131072 tokens, four heads to a KV head: 37.5 us with it, 39.4 without (another card 35.4); 512 tokens 6.5 and 6.8.
 template <bool IS_BF16, int D, int G, int CB, int R = 0>
-__global__ __launch_bounds__(256, KV4_WAVES(D)) void kv4_attn_kernel(AttnArgs a, const int* __restrict__ block_table,
-                                                                        const int* __restrict__ kv_len) {
+__global__ __launch_bounds__(256, 2) void kv4_attn_kernel(AttnArgs a, const int* __restrict__ block_table,
+                                                           const int* __restrict__ kv_len) {
   constexpr int KS = D / 32;            // MFMA steps over the head dim = dwords of a lane per K row
   constexpr int NT = D / 16;            // 16-channel tiles of V
   constexpr int NG = D / G;
@@ -221,7 +230,7 @@ __global__ __launch_bounds__(256, KV4_WAVES(D)) void kv4_attn_kernel(AttnArgs a,
         mul = sign * __builtin_bit_cast(float, (uint32_t)(127 + 8 - e) << 23);
         back = __builtin_bit_cast(float, (uint32_t)(127 - 8 + e) << 23);
       }
-      const float factor = fmaxf(lead * back, 1e-37f);      // (never 0: a masked score is -inf, and stays that)
+      const float factor = fminf(fmaxf(lead * back, 1e-37f), 1e37f);     // (a masked score is -inf, a 0 is 0: they stay that)
       if constexpr (R == 0) {
         qk[cb] = factor;
       } else {
@@ -377,9 +386,9 @@ __global__ __launch_bounds__(256, KV4_WAVES(D)) void kv4_attn_kernel(AttnArgs a,
       }
     }
   };
-  // the rest of a block, its parameters in LDS
-  auto wide_ = [&](auto careful, int n0, bool there0, bool there1, const Raw<D, NG>& r, const uint32_t (&param)[NG], float widest,
-                   auto after_k) INLINE -> bool {
+  // the rest of a block, its parameters in LDS (R = 0)
+  auto by_columns = [&](auto careful, int n0, bool there0, bool there1, const Raw<D, NG>& r, const uint32_t (&param)[NG],
+                        float widest, auto after_k) INLINE -> bool {
     constexpr bool CAREFUL = decltype(careful)::value;
     // ---- scores of token n0 + 16 t + 4 lg + i, column li of each block: sum(q value), still to be times qk
     float sc[CB][8];
@@ -520,8 +529,9 @@ __global__ __launch_bounds__(256, KV4_WAVES(D)) void kv4_attn_kernel(AttnArgs a,
     }
     return true;
   };
-  auto narrow = [&](auto careful, int n0, bool there0, bool there1, const Raw<D, NG>& r, const uint32_t (&param)[NG], float widest,
-                    auto after_k) INLINE -> bool {
+  // the same for R > 0
+  auto by_tokens = [&](auto careful, int n0, bool there0, bool there1, const Raw<D, NG>& r, const uint32_t (&param)[NG],
+                       float widest, auto after_k) INLINE -> bool {
     constexpr bool CAREFUL = decltype(careful)::value;
     // ---- scores of token n0 + 16 t + li, column lg R + i
     float sc[2][W];
@@ -648,9 +658,9 @@ __global__ __launch_bounds__(256, KV4_WAVES(D)) void kv4_attn_kernel(AttnArgs a,
     }
     widest = max_upper_half(widest);
     if constexpr (R > 0) {
-      return narrow(careful, n0, there0, there1, r, param, widest, after_k);
+      return by_tokens(careful, n0, there0, there1, r, param, widest, after_k);
     } else {
-      return wide_(careful, n0, there0, there1, r, param, widest, after_k);
+      return by_columns(careful, n0, there0, there1, r, param, widest, after_k);
     }
   };
   // A wave's blocks are 128 tokens apart.  RING of them are in flight: while one is multiplied the next ones are on their way,
@@ -660,7 +670,7 @@ __global__ __launch_bounds__(256, KV4_WAVES(D)) void kv4_attn_kernel(AttnArgs a,
   int n0 = start + 32 * wave;
   if (n0 < end) {
     fetch_q();
-    constexpr int RING = KV4_RING(D, CB);
+    constexpr int RING = ring_of(D, CB);
     Raw<D, NG> ring[RING];
     bool there[RING];
     auto nothing = [] {};
@@ -904,7 +914,8 @@ TDIST_API int tdist_kv4_attn(const void* k_codes, const void* v_codes, const voi
   TDIST_REQUIRE(q && table && kv_len && out, "null argument");
   TDIST_REQUIRE(((uintptr_t)q & 15) == 0 && ((uintptr_t)out & 7) == 0 && ((q_sb | q_ss | q_sh) & 7) == 0,
                 "q rows must keep 16-byte alignment");
-  const long long columns = (long long)(q_heads / kv_heads) * S, per_group = columns <= 4 ? 4 : columns <= 8 ? 8 : columns > 16 && head_dim <= 128 ? 32 : 16;
+  const long long columns = (long long)(q_heads / kv_heads) * S;
+  const long long per_group = columns <= 4 ? 4 : columns <= 8 ? 8 : columns > 16 && head_dim <= 128 ? 32 : 16;
   const long long blocks = (columns + per_group - 1) / per_group * batch;
   TDIST_REQUIRE(blocks < (1ll << 31) && columns < (1ll << 30) && (long long)batch * S * q_heads < (1ll << 31), "too many query rows");
   a.q = (const uint16_t*)q, a.partial = partial, a.out = out;
