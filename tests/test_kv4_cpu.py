@@ -281,7 +281,7 @@ def test_argument_types_of_the_native_calls_match_the_sources():
 
     from triton_distributed_gh_amd import build
 
-    source = "".join((build.CSRC / "ops" / f).read_text() for f in ("kv4.hip", "kv4_attn.hip"))
+    source = "".join((build.CSRC / "ops" / f).read_text() for f in ("kv4.hip", "kv4_attn.hip", "kv4_chunk.hip"))
     for name, signature in kv4._SIGNATURES.items():
         args = re.search(rf"TDIST_API int {name}\((.*?)\) \{{", source, re.S).group(1).split(",")
         kinds = ["p" if "*" in a else "q" if "long long" in a else "f" if "float" in a else "i" for a in args]

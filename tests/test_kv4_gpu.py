@@ -288,6 +288,81 @@ def test_values_far_from_one(Hq, H, S, D, group, dtype):
         _check(got[..., :D], want, got[..., D], lse, torch.float32, v_max, dtype)
 
 
+CHUNKS = [
+    # lens, S, Hq, Hkv, D, group, page, splits
+    ([64], 64, 1, 1, 128, 64, 16, 1),                       # a prompt of its own
+    ([300, 70, 0, 129], 70, 4, 2, 128, 64, 16, 1),          # ragged; one shorter than its queries, one that is not there
+    ([777], 40, 14, 2, 128, 32, 48, 3),                     # a second block of columns that is nearly empty
+    ([1500], 300, 2, 2, 128, 128, 64, 2),
+    ([513, 1], 96, 4, 4, 64, 32, 16, 2),
+    ([400], 260, 8, 4, 64, 64, 1040, 1),
+    ([333, 900], 33, 8, 2, 256, 32, 16, 2),
+    ([450], 200, 2, 1, 256, 64, 32, 1),
+    ([2000], 65, 1, 1, 256, 128, 16, 5),
+    ([90], 80, 4, 1, 128, 64, 16, 40),                      # more splits than there is to split
+]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lens,S,Hq,H,D,group,page,splits", CHUNKS)
+def test_many_columns_against_the_definition(lens, S, Hq, H, D, group, page, splits, dtype):
+    """In a chunk's values V is rounded to the fp16 that the bits of P are, too: 2^-11 of a value and of a weight, and K's
+    rounding of 2^-11 moves a score by 2^-11 / sqrt(3) |q| |k| / sqrt(D) = 3e-4 of a nat (one deviation, |q|, |k| = sqrt(D)):
+    by the two-token bound 1 / 4 * sqrt(2) * 3e-4 * 2 v_max = 2.1e-4 v_max, three deviations 6.4e-4."""
+    gen = _gen(sum(lens) + S)
+    cache, table, ks, vs = oracle.filled(gen, lens, H, D, group, page, dtype, "cuda", room=max(lens) + 40)
+    q = oracle.rows(gen, len(lens), S, Hq, D, dtype=dtype, device="cuda")
+    keys, values = [oracle.held(x, group) for x in ks], [oracle.held(x, group) for x in vs]
+    v_max = max(float(x.abs().max()) if x.numel() else 0.0 for x in values)
+    n = int32(lens, "cuda")
+    for causal in (True, False):
+        want, lse = oracle.attention(q, keys, values, D ** -0.5, causal=causal)
+        out = kv4.gqa_fwd_kv4(q, cache, n, table, kv_split=splits, causal=causal)
+        full = kv4.gqa_fwd_kv4(q, cache, n, table, kv_split=splits, causal=causal, return_lse=True)
+        torch.cuda.synchronize()
+        _check(out, want, None, None, dtype, v_max, scores=3.0)
+        _check(full[..., :D], want, full[..., D], lse, torch.float32, v_max, scores=3.0)
+        assert torch.equal(out, kv4.gqa_fwd_kv4(q, cache, n, table, kv_split=splits, causal=causal))
+
+
+@pytest.mark.parametrize("D,group", [(64, 64), (128, 32), (128, 128), (256, 64)])
+@pytest.mark.parametrize("splits", [1, 3])
+def test_chunks_with_blocks_that_fp16_does_not_reach(D, group, splits):
+    """A few tokens with a large K, with tiny K, with tiny and large V, a NaN and a page that is none: these blocks go the other
+    way, the rest does not, and the columns of both are right."""
+    gen = _gen(45)
+    lens, S, H, Hq, page = [600] * 6, 100, 2, 4, 16
+    for what in range(6):
+        cache, table, ks, vs = oracle.filled(gen, [600], H, D, group, page, torch.bfloat16, "cuda")
+        k, v, there = ks[0].clone(), vs[0].clone(), torch.ones(600, dtype=torch.bool)
+        if what == 0:
+            k[37, 1, 3] = 2.0 ** 16
+        elif what == 1:
+            k[64:128] *= 2.0 ** -12
+        elif what == 2:
+            v[192:256] *= 2.0 ** -14
+        elif what == 3:
+            v[590:] *= 2.0 ** 17
+        elif what == 4:
+            k[555, 0, 0] = math.nan
+        kv4.kv4_append(k[None], v[None], cache, int32([0], "cuda"), table)
+        if what == 5:
+            table[0, 20] = -1
+            there[320:336] = False
+        q = oracle.rows(gen, 1, S, Hq, D, device="cuda")
+        if what == 0:
+            q *= 2.0 ** -10                 # (scores of a few nats)
+        keys, values = [oracle.held(k, group)], [oracle.held(v, group)]
+        want, lse = oracle.attention(q, keys, values, D ** -0.5, there=[there])
+        got = kv4.gqa_fwd_kv4(q, cache, int32([600], "cuda"), table, kv_split=splits, return_lse=True)
+        torch.cuda.synchronize()
+        if what == 4:                       # a query that sees the NaN, of either of its KV head's, is NaN
+            assert got[0, 55:, :2].isnan().all() and got[0, :55].isfinite().all() and got[0, :, 2:].isfinite().all()
+            want[0, 55:, :2], lse[0, 55:, :2] = 0.0, 0.0
+            got[0, 55:, :2] = 0.0
+        _check(got[..., :D], want, got[..., D], lse, torch.float32, float(values[0].abs().max()), scores=3.0)
+
+
 @pytest.mark.parametrize("scale,soft_cap", [(-0.11, 0.0), (0.3, 7.0), (-0.3, 7.0), (0.0, 0.0), (0.0, 5.0), (0.1, 1e-30)])
 @pytest.mark.parametrize("Hq,H,S,D,group", SHAPES)
 def test_scales_and_caps(Hq, H, S, D, group, scale, soft_cap):

@@ -61,7 +61,7 @@ if os.environ.get("TDIST_EXTRA_HIPCC_FLAGS"):
     # e.g. -DTDIST_EXP_...=1 for an A/B build of one experiment (objects are keyed by their flags)
     HIPCC_FLAGS += os.environ["TDIST_EXTRA_HIPCC_FLAGS"].split()
 # sources that need IEEE arithmetic (a stored code depends on a quotient; infinities and NaN reach the kernels)
-SOURCE_FLAGS = {"kv4": ["-fno-fast-math"], "kv4_attn": ["-fno-fast-math"]}
+SOURCE_FLAGS = {"kv4": ["-fno-fast-math"], "kv4_attn": ["-fno-fast-math"], "kv4_chunk": ["-fno-fast-math"]}
 HOST_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-pthread", f"-I{CSRC / 'include'}"]
 
 

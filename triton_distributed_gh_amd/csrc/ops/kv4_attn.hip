@@ -44,6 +44,8 @@ struct AttnArgs {
   uint32_t page_magic;      // and floor(2^32 / page_tiles) + 1 (0: one tile a page)
   int batch, S, q_heads, group, splits, causal, out_mode;
   int first;                // of this launch's (column block, sequence) pairs
+  const int* flags;         // where given: [blocks of flag_columns * batch, splits, kv_heads], 0: another kernel has done it
+  int flag_columns;
   float scale, soft_cap;
 };
 
@@ -161,6 +163,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_kernel(AttnArgs a, const int*
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, lg = lane >> 4;
   constexpr int COLUMNS = R > 0 ? 4 * R : 16 * CB;
   const int col0 = cblk * COLUMNS;
+  if (a.flags && !a.flags[(((long long)(col0 / a.flag_columns) * a.batch + b) * a.splits + split) * gridDim.x + kvh]) return;
 
   // tokens: a column sees [0, limit), the workgroup's columns [0, len), none of them misses one below `full`
   const long long room = (long long)a.max_pages * a.c.page_size;
@@ -169,7 +172,9 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_kernel(AttnArgs a, const int*
   const int s_first = one ? 0 : col0 / group, s_last = one ? 0 : min(col0 + COLUMNS - 1, columns - 1) / group;
   const int len = max(0, a.causal ? L - a.S + s_last + 1 : L);
   const int full = a.causal ? L - a.S + s_first + 1 : L;
-  const int per = a.splits == 1 ? len : ((len + a.splits - 1) / a.splits + 127) & ~127;
+  int whole = len;                            // what is split: with flags, what the flagged block of columns sees
+  if (a.flags && a.causal) whole = max(0, L - a.S + min((col0 / a.flag_columns + 1) * a.flag_columns - 1, columns - 1) / group + 1);
+  const int per = a.splits == 1 ? whole : ((whole + a.splits - 1) / a.splits + 127) & ~127;
   const int start = (int)min((long long)split * per, (long long)len), end = min(len, start + per);
   if (a.splits > 1 && start >= end) {         // (the merge does not look at the sums of a split without tokens)
     const int col = col0 + (int)threadIdx.x;
@@ -819,6 +824,8 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_kernel(AttnArgs a, const int*
   }
 }
 
+constexpr int FEW_SPLITS = 8;
+
 // One workgroup merges the splits of one row.  D / 4 lanes hold a split's sums, so 1024 / D splits are read at a time; eight
 // rounds of loads are issued before the first is used (64 splits of 128 channels: one trip to memory).
 template <bool IS_BF16, int D>
@@ -878,6 +885,44 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(const float* __restrict_
     ((float*)out)[row * (D + 1) + D] = sum != 0.f ? (top + log2_fast(sum)) * 0.6931471805599453f : -INFINITY;
 }
 
+// The same for few splits: D / 4 lanes take a row, and a workgroup 1024 / D rows.  32768 rows of 2 splits, 128 channels: a
+// workgroup each takes 50 us.
+template <bool IS_BF16, int D>
+__global__ __launch_bounds__(256) void kv4_merge_few_kernel(const float* __restrict__ partial, const float* __restrict__ lse, int splits,
+                                                            long long rows, void* __restrict__ out, int out_mode) {
+  constexpr int LANES = D / 4, AT_ONCE = FEW_SPLITS;
+  const long long row = (long long)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+  if (row >= rows) return;
+  const int c = threadIdx.x % LANES * 4;
+  f32x4 v[AT_ONCE];
+  float w[AT_ONCE], top = -INFINITY, sum = 0.f;
+#pragma unroll
+  for (int s = 0; s < AT_ONCE; ++s) {
+    w[s] = s < splits ? lse[row * splits + s] : -INFINITY;
+    if (s < splits) v[s] = *(const f32x4*)(partial + (row * splits + s) * D + c);
+    top = fmaxf(top, w[s]);
+  }
+  if (top == -INFINITY) top = 0.f;        // no split has a token (or what they have is NaN, which the weights keep)
+  f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int s = 0; s < AT_ONCE; ++s) {
+    w[s] = exp2_fast(w[s] - top);
+    sum += w[s];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) acc[k] += w[s] != 0.f ? w[s] * v[s][k] : 0.f;    // (a split without tokens has written no sums)
+  }
+  acc *= sum != 0.f ? 1.f / sum : 0.f;
+  if (out_mode == 2) {
+    float* to = (float*)out + row * (D + 1);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) to[c + k] = acc[k];
+    if (c == 0) to[D] = sum != 0.f ? (top + log2_fast(sum)) * 0.6931471805599453f : -INFINITY;
+  } else {
+    *(uint2*)((uint16_t*)out + row * D + c) =
+        uint2{to16<IS_BF16>(acc[0]) | to16<IS_BF16>(acc[1]) << 16, to16<IS_BF16>(acc[2]) | to16<IS_BF16>(acc[3]) << 16};
+  }
+}
+
 template <class Fn>
 bool dispatch(int dtype, int D, int G, Fn&& fn) {
   auto typed = [&](auto d, auto g) {
@@ -897,11 +942,12 @@ bool dispatch(int dtype, int D, int G, Fn&& fn) {
 
 // partial (splits > 1): batch * S * q_heads * splits * (head_dim + 1) floats.
 // out_mode 1: out [batch, S, q_heads, D] in q's type; 2: fp32 [batch, S, q_heads, D + 1], natural-log LSE last.
+// flags (or null): what tdist_kv4_chunk, run before with the same arguments, has left undone; only that is done here, and the merge.
 TDIST_API int tdist_kv4_attn(const void* k_codes, const void* v_codes, const void* k_params, const void* v_params, int pages,
                              int kv_heads, int page_size, int head_dim, int group, const void* q, long long q_sb, long long q_ss,
                              long long q_sh, const int* table, int table_stride, int max_pages, const int* kv_len, float* partial,
                              void* out, int batch, int S, int q_heads, int splits, int causal, int out_mode, float scale,
-                             float soft_cap, int dtype, void* stream) {
+                             float soft_cap, int dtype, const int* flags, int flag_columns, void* stream) {
   AttnArgs a;
   a.c = Cache{(uint8_t*)k_codes, (uint8_t*)v_codes, (uint32_t*)k_params, (uint32_t*)v_params, pages, kv_heads, page_size};
   TDIST_REQUIRE(k_codes && v_codes && k_params && v_params && pages > 0 && kv_heads > 0 && page_size > 0 && page_size % 16 == 0 &&
@@ -909,6 +955,7 @@ TDIST_API int tdist_kv4_attn(const void* k_codes, const void* v_codes, const voi
                 "a 4-bit cache needs four 16-byte aligned tensors, pages of a multiple of 16 tokens");
   TDIST_REQUIRE(batch >= 0 && S >= 0 && q_heads > 0 && q_heads % kv_heads == 0 && max_pages >= 0, "bad head counts");
   TDIST_REQUIRE(splits >= 1 && splits <= 65535 && (splits == 1 || partial), "splits need their partial rows");
+  TDIST_REQUIRE(!flags || (flag_columns > 0 && flag_columns % 32 == 0), "flags are for blocks of a multiple of 32 columns");
   TDIST_REQUIRE((out_mode == 1 || out_mode == 2) && (dtype == 0 || dtype == 1), "out_mode must be 1 or 2, dtype 0 (bf16) or 1 (fp16)");
   if (batch == 0 || S == 0) return 0;
   TDIST_REQUIRE(q && table && kv_len && out, "null argument");
@@ -924,7 +971,7 @@ TDIST_API int tdist_kv4_attn(const void* k_codes, const void* v_codes, const voi
   a.partial_lse = partial ? partial + (long long)batch * S * q_heads * splits * head_dim : nullptr;
   a.q_sb = q_sb, a.q_ss = q_ss, a.q_sh = q_sh, a.table_stride = table_stride, a.max_pages = max_pages;
   a.batch = batch, a.S = S, a.q_heads = q_heads, a.group = q_heads / kv_heads, a.splits = splits, a.causal = causal, a.out_mode = out_mode;
-  a.scale = scale, a.soft_cap = soft_cap;
+  a.scale = scale, a.soft_cap = soft_cap, a.flags = flags, a.flag_columns = flag_columns;
   const bool ok = dispatch(dtype, head_dim, group, [&](auto bf, auto d, auto g) {
     auto launch = [&](auto kernel) {
       for (a.first = 0; a.first < blocks; a.first += 65535)       // (the limit of a grid's third dimension)
@@ -945,6 +992,12 @@ TDIST_API int tdist_kv4_attn(const void* k_codes, const void* v_codes, const voi
   if (splits == 1) return 0;
   const long long rows = (long long)batch * S * q_heads;
   dispatch(dtype, head_dim, group, [&](auto bf, auto d, auto) {
+    constexpr int per_block = 1024 / decltype(d)::value;
+    if (splits <= FEW_SPLITS) {
+      hipLaunchKernelGGL((kv4_merge_few_kernel<decltype(bf)::value, decltype(d)::value>), dim3((unsigned)((rows + per_block - 1) / per_block)),
+                         dim3(256), 0, (hipStream_t)stream, a.partial, a.partial_lse, splits, rows, out, out_mode);
+      return;
+    }
     hipLaunchKernelGGL((kv4_merge_kernel<decltype(bf)::value, decltype(d)::value>), dim3((unsigned)rows), dim3(256), 0,
                        (hipStream_t)stream, a.partial, a.partial_lse, splits, out, out_mode);
   });

@@ -34,6 +34,9 @@ from .. import _lib
 
 HEAD_DIMS = (64, 128, 256)
 GROUPS = (32, 64, 128)
+# columns (new tokens times query heads of a KV head) from which csrc/ops/kv4_chunk.hip runs first, and its workgroups' columns
+CHUNK_FROM = 64
+CHUNK_COLUMNS = {64: 256, 128: 256, 256: 128}
 
 # argument types of the native calls (p pointer, i int, q long long, f float), so that plain integers can be passed; the
 # stream comes last everywhere
@@ -42,7 +45,8 @@ _SIGNATURES = {
     "tdist_kv4_append": _CACHE_ARGS + "pp" + "qqqqqq" + "ppp" + "iiiii" + "p",
     "tdist_kv4_qkv_prep": _CACHE_ARGS + "pqqppffpppq" + "pppp" + "iiiii" + "p",
     "tdist_kv4_read": _CACHE_ARGS + "pii" + "pp" + "iq" + "pp" + "qqqq" + "i" + "p",
-    "tdist_kv4_attn": _CACHE_ARGS + "pqqq" + "pii" + "ppp" + "iiiiii" + "ff" + "i" + "p",
+    "tdist_kv4_attn": _CACHE_ARGS + "pqqq" + "pii" + "ppp" + "iiiiii" + "ff" + "ipi" + "p",
+    "tdist_kv4_chunk": _CACHE_ARGS + "pqqq" + "pii" + "ppp" + "iiiiii" + "f" + "ipi" + "p",
 }
 _CTYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "q": ctypes.c_longlong, "f": ctypes.c_float}
 
@@ -399,13 +403,17 @@ def attend_reference(q, cache: Int4KVCache, kv_lens, block_table, scale, soft_ca
     return out, lse
 
 
-def auto_kv_splits(batch: int, kv_heads: int, columns: int, head_dim: int, capacity: int, num_cus: int = 256) -> int:
+def auto_kv_splits(batch: int, kv_heads: int, columns: int, head_dim: int, capacity: int, num_cus: int = 256,
+                   chunk: bool = False) -> int:
     """KV splits of a launch: ``columns`` = new tokens times query heads of a KV head, ``capacity`` = tokens of a sequence's pages.
 
     One round of the chip: a CU holds two workgroups, and a third round of nothing but start-up costs more than it gives.
     Measured (32 / 8 heads of 128, groups of 64, microseconds): 131072 tokens of one sequence 43.2 / 36.4 / 41.2 with 32 / 64 / 96
     splits; 16 x 4096 26.3 / 23.2 / 27.1 with 2 / 4 / 8; 64 x 4096 55.3 / 64.8 with 1 / 2.  At least 128 tokens each: 512 tokens
     9.8 / 8.8 with 2 / 4, 2048 tokens 9.8 / 8.9 with 8 / 16; beyond sixteen splits 256: 8192 tokens 10.3 / 11.0 with 32 / 64."""
+    if chunk:
+        groups = batch * kv_heads * (-(-columns // CHUNK_COLUMNS[head_dim]))
+        return max(1, min(num_cus // max(1, groups), capacity // 256, 64))
     per_group = 32 if columns > 16 and head_dim <= 128 else 16          # columns of a workgroup
     groups = batch * kv_heads * (-(-columns // per_group))
     most = min(capacity // 128, max(16, capacity // 256), 64)
@@ -438,14 +446,21 @@ def gqa_fwd_kv4(q: torch.Tensor, cache: Int4KVCache, kv_lens: torch.Tensor, bloc
         out = torch.cat([out, lse.unsqueeze(-1)], -1) if return_lse else out.to(q.dtype)
         return out.squeeze(1) if flat else out
     q4 = _rows(q4)
-    splits = int(kv_split) if kv_split > 0 else auto_kv_splits(batch, cache.kv_heads, Hq // cache.kv_heads * S, D,
-                                                               block_table.shape[1] * cache.page_size)
+    columns = Hq // cache.kv_heads * S
+    chunk = columns >= CHUNK_FROM and soft_cap == 0
+    splits = int(kv_split) if kv_split > 0 else auto_kv_splits(batch, cache.kv_heads, columns, D, block_table.shape[1] * cache.page_size,
+                                                               chunk=chunk)
     out = torch.empty((batch, S, Hq, D + 1), dtype=torch.float32, device=q.device) if return_lse else \
         torch.empty_like(q4, memory_format=torch.contiguous_format)
     part = torch.empty(batch * S * Hq * splits * (D + 1), dtype=torch.float32, device=q.device) if splits > 1 else None
-    _launch("tdist_kv4_attn", cache.device, *cache._native, q4.data_ptr(), *q4.stride()[:3], block_table.data_ptr(),
-            block_table.stride(0), block_table.shape[1], kv_lens.data_ptr(), _ptr(part), out.data_ptr(), batch, S, Hq, splits,
-            1 if causal else 0, 2 if return_lse else 1, scale, soft_cap, _dt(cache.dtype))
+    call = (*cache._native, q4.data_ptr(), *q4.stride()[:3], block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
+            kv_lens.data_ptr(), _ptr(part), out.data_ptr(), batch, S, Hq, splits, 1 if causal else 0, 2 if return_lse else 1, scale)
+    flags, at_once = None, 0
+    if chunk:
+        at_once = CHUNK_COLUMNS[D]
+        flags = torch.empty(-(-columns // at_once) * batch * splits * cache.kv_heads, dtype=torch.int32, device=q.device)
+        _launch("tdist_kv4_chunk", cache.device, *call, _dt(cache.dtype), flags.data_ptr(), at_once)
+    _launch("tdist_kv4_attn", cache.device, *call, soft_cap, _dt(cache.dtype), _ptr(flags), at_once)
     return out.squeeze(1) if flat else out
 
 
