@@ -288,6 +288,12 @@ def test_values_far_from_one(Hq, H, S, D, group, dtype):
         _check(got[..., :D], want, got[..., D], lse, torch.float32, v_max, dtype)
 
 
+@pytest.fixture
+def chunks(monkeypatch):
+    """Many columns go to the kernel for them however short the sequences are."""
+    monkeypatch.setattr(kv4, "takes_chunks", lambda *a: a[2] >= 32 and a[5] == 0)
+
+
 CHUNKS = [
     # lens, S, Hq, Hkv, D, group, page, splits
     ([64], 64, 1, 1, 128, 64, 16, 1),                       # a prompt of its own
@@ -305,7 +311,7 @@ CHUNKS = [
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("lens,S,Hq,H,D,group,page,splits", CHUNKS)
-def test_many_columns_against_the_definition(lens, S, Hq, H, D, group, page, splits, dtype):
+def test_many_columns_against_the_definition(lens, S, Hq, H, D, group, page, splits, dtype, chunks):
     """In a chunk's values V is rounded to the fp16 that the bits of P are, too: 2^-11 of a value and of a weight, and K's
     rounding of 2^-11 moves a score by 2^-11 / sqrt(3) |q| |k| / sqrt(D) = 3e-4 of a nat (one deviation, |q|, |k| = sqrt(D)):
     by the two-token bound 1 / 4 * sqrt(2) * 3e-4 * 2 v_max = 2.1e-4 v_max, three deviations 6.4e-4."""
@@ -327,11 +333,11 @@ def test_many_columns_against_the_definition(lens, S, Hq, H, D, group, page, spl
 
 @pytest.mark.parametrize("D,group", [(64, 64), (128, 32), (128, 128), (256, 64)])
 @pytest.mark.parametrize("splits", [1, 3])
-def test_chunks_with_blocks_that_fp16_does_not_reach(D, group, splits):
+def test_chunks_with_blocks_that_fp16_does_not_reach(D, group, splits, chunks):
     """A few tokens with a large K, with tiny K, with tiny and large V, a NaN and a page that is none: these blocks go the other
     way, the rest does not, and the columns of both are right."""
     gen = _gen(45)
-    lens, S, H, Hq, page = [600] * 6, 100, 2, 4, 16
+    S, H, Hq, page = 100, 2, 4, 16
     for what in range(6):
         cache, table, ks, vs = oracle.filled(gen, [600], H, D, group, page, torch.bfloat16, "cuda")
         k, v, there = ks[0].clone(), vs[0].clone(), torch.ones(600, dtype=torch.bool)
@@ -361,6 +367,69 @@ def test_chunks_with_blocks_that_fp16_does_not_reach(D, group, splits):
             want[0, 55:, :2], lse[0, 55:, :2] = 0.0, 0.0
             got[0, 55:, :2] = 0.0
         _check(got[..., :D], want, got[..., D], lse, torch.float32, float(values[0].abs().max()), scores=3.0)
+
+
+@pytest.mark.parametrize("scale", [-0.11, 0.0, 0.3])
+def test_chunks_at_other_scales_strides_and_streams(scale, chunks):
+    gen = _gen(46)
+    lens, S, H, Hq, D, group, page = [333, 70], 40, 2, 8, 128, 64, 32
+    cache, table, ks, vs = oracle.filled(gen, lens, H, D, group, page, torch.bfloat16, "cuda")
+    q = oracle.rows(gen, 2, S + 3, Hq + 2, D, device="cuda")[:, 2:S + 2, 1:Hq + 1]
+    keys, values = [oracle.held(x, group) for x in ks], [oracle.held(x, group) for x in vs]
+    want, lse = oracle.attention(q, keys, values, scale)
+    n = int32(lens, "cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        there = kv4.gqa_fwd_kv4(q, cache, n, table, scale=scale, return_lse=True, kv_split=2)
+    here = kv4.gqa_fwd_kv4(q, cache, n, table, scale=scale, return_lse=True, kv_split=2)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    assert torch.equal(here, there)
+    _check(here[..., :D], want, here[..., D], lse, torch.float32, max(float(x.abs().max()) for x in values),
+           scores=3.0 * max(1.0, abs(scale) * D ** 0.5))
+
+
+def test_chunks_replay_from_a_graph(chunks):
+    """A flagged block and a plain one, replayed with other queries and another cache behind the same addresses."""
+    gen = _gen(47)
+    lens, S, H, Hq, D, group, page = [500, 300], 80, 1, 4, 128, 32, 16
+    cache, table, ks, vs = oracle.filled(gen, lens, H, D, group, page, torch.bfloat16, "cuda")
+    n, q = int32(lens, "cuda"), oracle.rows(gen, 2, S, Hq, D, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        kv4.gqa_fwd_kv4(q, cache, n, table, kv_split=2)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            out = kv4.gqa_fwd_kv4(q, cache, n, table, kv_split=2)
+    torch.cuda.current_stream().wait_stream(side)
+    for i in range(5):
+        q.copy_(oracle.rows(gen, 2, S, Hq, D, device="cuda"))
+        k = oracle.rows(gen, 2, 64, H, D, device="cuda")
+        if i % 2:
+            k[0] *= 2.0 ** 17
+        kv4.kv4_append(k, k, cache, int32([100 * (i % 3), 64 * (i % 4)], "cuda"), table)
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = kv4.gqa_fwd_kv4(q, cache, n, table, kv_split=2)
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager)
+
+
+def test_large_chunks_and_small_ones_agree(monkeypatch):
+    """The same call by either kernel, at a size where it is the other one's: each is within its bounds of the definition."""
+    gen = _gen(48)
+    S, H, Hq, D, group, page, L = 70, 8, 32, 128, 64, 64, 16000
+    cache, table, ks, vs = oracle.filled(gen, [L], H, D, group, page, torch.bfloat16, "cuda")
+    q, n = oracle.rows(gen, 1, S, Hq, D, device="cuda"), int32([L], "cuda")
+    assert kv4.takes_chunks(1, H, S * Hq // H, D, table.shape[1] * page)
+    one = kv4.gqa_fwd_kv4(q, cache, n, table, return_lse=True)
+    monkeypatch.setattr(kv4, "takes_chunks", lambda *a: False)
+    other = kv4.gqa_fwd_kv4(q, cache, n, table, return_lse=True)
+    torch.cuda.synchronize()
+    v_max = float(vs[0].abs().max())
+    _check(one[..., :D], other[..., :D].double().cpu(), one[..., D], other[..., D].double().cpu(), torch.float32, v_max, scores=4.0)
 
 
 @pytest.mark.parametrize("scale,soft_cap", [(-0.11, 0.0), (0.3, 7.0), (-0.3, 7.0), (0.0, 0.0), (0.0, 5.0), (0.1, 1e-30)])

@@ -22,8 +22,8 @@
 // What bounds it: many sequences, the bytes of the cache (64 x 4096 tokens, 8 heads of 128: 286 MB in 58 us, 4.9 TB/s, a copy's
 // rate on the same card); one long sequence of 131072, those and the two launches' start and end (151 MB in 35 .. 37 us,
 // 4.1 .. 4.3 TB/s); a few tokens, the launches (6.5 us); many columns, the vector instructions of unpacking and softmax (1024
-// new tokens over 16384, 266 GFLOP: 511 us, 520 TFLOP/s, against 1203 of a large bf16 matrix product).  bf16 high and low
-// parts of 16 + code, what this began with, took 103 us for the first of these.
+// new tokens over 16384, 266 GFLOP: 511 us, 520 TFLOP/s; kv4_chunk.hip takes 312 and gets such calls).  bf16 high and low parts
+// of 16 + code, what this began with, took 103 us for the first of these.
 #include <algorithm>
 
 #include "tdist/kv4.hpp"
@@ -885,8 +885,8 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(const float* __restrict_
     ((float*)out)[row * (D + 1) + D] = sum != 0.f ? (top + log2_fast(sum)) * 0.6931471805599453f : -INFINITY;
 }
 
-// The same for few splits: D / 4 lanes take a row, and a workgroup 1024 / D rows.  32768 rows of 2 splits, 128 channels: a
-// workgroup each takes 50 us.
+// The same for few splits: D / 4 lanes take a row, a workgroup 1024 / D rows, and all splits are read at once.  32768 rows of 2
+// splits, 128 channels: 8.4 us (42 MB, 5.0 TB/s) where a workgroup for each row takes 50.
 template <bool IS_BF16, int D>
 __global__ __launch_bounds__(256) void kv4_merge_few_kernel(const float* __restrict__ partial, const float* __restrict__ lse, int splits,
                                                             long long rows, void* __restrict__ out, int out_mode) {

@@ -14,6 +14,13 @@
 // fp16 does not reach as far as bf16: a block of tokens whose values come to 2^15 or whose largest one is under 2^-6 (K) or
 // 2^-9 (V), a NaN in a scale and a page that is none are for the other kernel.  Whoever meets one says so in `flags`, one int per
 // workgroup, written by every launch; the other kernel runs behind this one and takes just the flagged workgroups' columns.
+//
+// What bounds it: 1024 new tokens over 16384, 32 / 8 heads of 128 (266 GFLOP): 312 .. 350 us in all, 760 .. 850 TFLOP/s where a
+// large bf16 matrix product reaches 1203; the other kernel takes 511.  Of a SIMD's cycles its matrix unit has 37 %, vector
+// instructions 48 % - a third of them unpacking, a fifth the exponentials - and two waves hardly overlap the two.  Eight waves
+// with one set of buffers against twice four: 346 and 367 us (with half the columns for a workgroup, unpacking costs twice as
+// much); scores of the next 32 tokens made ahead of time from a third buffer: 348, and 99 for 77 where heads of 256 then need
+// shorter blocks; all 64 tokens' scores at once spill registers.
 #include <algorithm>
 
 #include "tdist/kv4.hpp"
@@ -26,9 +33,6 @@ typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
 typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
-#ifndef EARLY
-#define EARLY 4
-#endif
 #define INLINE __attribute__((always_inline))     // (lambdas: a call would put what they capture into memory)
 
 struct ChunkArgs {
@@ -72,6 +76,7 @@ struct Unpack {
   }
 };
 
+constexpr int WAVES = 8;                // of a workgroup
 template <int D>
 constexpr int column_blocks() { return D <= 128 ? 2 : 1; }          // of sixteen, per wave: what its registers hold
 template <int D, int NW>
@@ -411,12 +416,10 @@ __global__ __launch_bounds__(NW * 64, 2) void kv4_chunk_kernel(ChunkArgs a, cons
       next = lookup(n0 + 3 * TOK);
     };
     // what all columns see, then the rest
-    const bool early = wave < EARLY;
     for (; n0 + TOK <= plain_end; n0 += TOK, buf ^= 1) {
-      if (early) ahead();
+      ahead();
       compute(std::false_type{}, buf, 0, n0);
       compute(std::false_type{}, buf, 1, n0 + 32);
-      if (!early) ahead();
       __syncthreads();
     }
     for (; n0 < end; n0 += TOK, buf ^= 1) {
@@ -476,9 +479,6 @@ bool dispatch(int dtype, int D, int G, Fn&& fn) {
 #undef TDIST_KV4_CASE
   return false;
 }
-#ifndef NWAVES
-#define NWAVES(D) 8
-#endif
 
 }  // namespace
 
@@ -512,7 +512,7 @@ TDIST_API int tdist_kv4_chunk(const void* k_codes, const void* v_codes, const vo
   a.scale = scale;
   bool same = true;
   const bool ok = dispatch(dtype, head_dim, group, [&](auto bf, auto d, auto g) {
-    constexpr int D = decltype(d)::value, NW = NWAVES(D);
+    constexpr int D = decltype(d)::value, NW = WAVES;
     constexpr int per_group = columns_of<D, NW>();
     same = flag_columns == per_group;
     if (!same) return;

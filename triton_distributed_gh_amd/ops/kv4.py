@@ -34,9 +34,10 @@ from .. import _lib
 
 HEAD_DIMS = (64, 128, 256)
 GROUPS = (32, 64, 128)
-# columns (new tokens times query heads of a KV head) from which csrc/ops/kv4_chunk.hip runs first, and its workgroups' columns
-CHUNK_FROM = 64
+# columns (new tokens times query heads of a KV head) of a workgroup of csrc/ops/kv4_chunk.hip, and the products of columns and
+# cached tokens from which a launch goes there
 CHUNK_COLUMNS = {64: 256, 128: 256, 256: 128}
+CHUNK_WORK = {64: 1 << 25, 128: 1 << 25, 256: 1 << 23}
 
 # argument types of the native calls (p pointer, i int, q long long, f float), so that plain integers can be passed; the
 # stream comes last everywhere
@@ -403,6 +404,15 @@ def attend_reference(q, cache: Int4KVCache, kv_lens, block_table, scale, soft_ca
     return out, lse
 
 
+def takes_chunks(batch: int, kv_heads: int, columns: int, head_dim: int, capacity: int, soft_cap: float = 0.0) -> bool:
+    """Whether a launch goes to csrc/ops/kv4_chunk.hip, which unpacks for many columns at once, and only what that leaves to
+    csrc/ops/kv4_attn.hip.  Measured (four query heads to a KV head, microseconds there / here): one sequence of 16384, 8 heads of
+    128: 128 columns 40 / 34, 256 46 / 50, 1024 98 / 147; of 4096: 512 columns 43 / 35, 1024 49 / 51, 2048 66 / 78; of 1024: 2048
+    columns 39 / 27; 4 x 2048: 256 columns 38 / 36, 1024 65 / 84; 4 heads of 256: 2048: 512 columns 30 / 29, 1024 36 / 40."""
+    work = batch * kv_heads * columns * capacity
+    return soft_cap == 0 and 2 * columns > CHUNK_COLUMNS[head_dim] and work >= CHUNK_WORK[head_dim]
+
+
 def auto_kv_splits(batch: int, kv_heads: int, columns: int, head_dim: int, capacity: int, num_cus: int = 256,
                    chunk: bool = False) -> int:
     """KV splits of a launch: ``columns`` = new tokens times query heads of a KV head, ``capacity`` = tokens of a sequence's pages.
@@ -410,7 +420,10 @@ def auto_kv_splits(batch: int, kv_heads: int, columns: int, head_dim: int, capac
     One round of the chip: a CU holds two workgroups, and a third round of nothing but start-up costs more than it gives.
     Measured (32 / 8 heads of 128, groups of 64, microseconds): 131072 tokens of one sequence 43.2 / 36.4 / 41.2 with 32 / 64 / 96
     splits; 16 x 4096 26.3 / 23.2 / 27.1 with 2 / 4 / 8; 64 x 4096 55.3 / 64.8 with 1 / 2.  At least 128 tokens each: 512 tokens
-    9.8 / 8.8 with 2 / 4, 2048 tokens 9.8 / 8.9 with 8 / 16; beyond sixteen splits 256: 8192 tokens 10.3 / 11.0 with 32 / 64."""
+    9.8 / 8.8 with 2 / 4, 2048 tokens 9.8 / 8.9 with 8 / 16; beyond sixteen splits 256: 8192 tokens 10.3 / 11.0 with 32 / 64.
+
+    ``chunk``: of a launch that `takes_chunks`; one workgroup fills a CU there (1024 new tokens over 16384: 613 / 356 / 443 with 1 /
+    2 / 3; 256 over 16384 126 / 106 / 128 with 6 / 8 / 16)."""
     if chunk:
         groups = batch * kv_heads * (-(-columns // CHUNK_COLUMNS[head_dim]))
         return max(1, min(num_cus // max(1, groups), capacity // 256, 64))
@@ -447,9 +460,9 @@ def gqa_fwd_kv4(q: torch.Tensor, cache: Int4KVCache, kv_lens: torch.Tensor, bloc
         return out.squeeze(1) if flat else out
     q4 = _rows(q4)
     columns = Hq // cache.kv_heads * S
-    chunk = columns >= CHUNK_FROM and soft_cap == 0
-    splits = int(kv_split) if kv_split > 0 else auto_kv_splits(batch, cache.kv_heads, columns, D, block_table.shape[1] * cache.page_size,
-                                                               chunk=chunk)
+    room = block_table.shape[1] * cache.page_size
+    chunk = takes_chunks(batch, cache.kv_heads, columns, D, room, soft_cap)
+    splits = int(kv_split) if kv_split > 0 else auto_kv_splits(batch, cache.kv_heads, columns, D, room, chunk=chunk)
     out = torch.empty((batch, S, Hq, D + 1), dtype=torch.float32, device=q.device) if return_lse else \
         torch.empty_like(q4, memory_format=torch.contiguous_format)
     part = torch.empty(batch * S * Hq * splits * (D + 1), dtype=torch.float32, device=q.device) if splits > 1 else None
