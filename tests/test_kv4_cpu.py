@@ -315,3 +315,53 @@ def test_facade_serves_the_operators():
     from triton_dist.models.kv_cache import KV4_Cache  # noqa: F401
 
     assert facade is kv4
+
+
+def test_a_table_without_pages_is_empty_sequences():
+    _no_pages("cpu")
+
+
+def _no_pages(device):
+    gen = _gen(51)
+    cache = kv4.Int4KVCache.alloc(2, 16, 2, 64, group=32, device=device)
+    table = torch.zeros(3, 0, dtype=torch.int32, device=device)
+    rows = oracle.rows(gen, 3, 2, 2, 64, device=device)
+    kv4.kv4_append(rows, rows, cache, int32([0, 1, 5], device), table)
+    assert not cache.k_params.any() and not cache.v_codes.any()
+    out = kv4.gqa_fwd_kv4(rows, cache, int32([2, 9, 0], device), table, return_lse=True)
+    assert not out[..., :64].any() and (out[..., 64] == -math.inf).all()
+    k, v = kv4.kv4_read(cache, table, int32([0, 1, 2, 4], device), 4)
+    assert not k.any() and not v.any()
+
+
+def test_projection_refuses_to_write_over_the_offsets_it_reads():
+    cache = kv4.Int4KVCache.alloc(4, 16, 1, 64, group=32)
+    table, n = torch.zeros(2, 2, dtype=torch.int32), torch.zeros(3, dtype=torch.int32)
+    qkv, rope = torch.zeros(2, 1, 3 * 64, dtype=torch.bfloat16), torch.ones(8, 32)
+    pos = torch.zeros(2, 1, dtype=torch.int64)
+    for total in (n[:2], n[1:]):
+        with pytest.raises(ValueError, match="share memory"):
+            kv4.kv4_qkv_prep(qkv, None, None, 0.0, 0.0, pos, rope, rope, cache, n[:2], total, table, 1)
+    kv4.kv4_qkv_prep(qkv, None, None, 0.0, 0.0, pos, rope, rope, cache, n[:2], int32([0, 0]), table, 1)
+
+
+def test_tables_of_more_than_2_to_the_30_tokens_are_refused():
+    cache = kv4.Int4KVCache.alloc(1, 1 << 20, 1, 64, group=64)
+    q = torch.zeros(1, 1, 64, dtype=torch.bfloat16)
+    table = torch.full((1, 1025), -1, dtype=torch.int32)
+    with pytest.raises(ValueError, match="2\\^30"):
+        kv4.gqa_fwd_kv4(q, cache, int32([1]), table)
+    kv4.gqa_fwd_kv4(q, cache, int32([1]), table[:, :1024])
+
+
+@pytest.mark.parametrize("head_dim", [64, 128, 256])
+def test_split_and_chunk_rules_stay_within_their_launches(head_dim):
+    for batch in (0, 1, 7, 64, 70000):
+        for columns in (0, 1, 5, 100, 1000, 1 << 20):
+            for capacity in (0, 16, 500, 4096, 1 << 30):
+                for chunk in (False, True):
+                    splits = kv4.auto_kv_splits(batch, 8, columns, head_dim, capacity, chunk=chunk)
+                    assert 1 <= splits <= 64 and (splits == 1 or capacity // splits >= 128)
+                assert not kv4.takes_chunks(batch, 8, columns, head_dim, capacity, 1.0)
+    assert not kv4.takes_chunks(64, 8, 16, head_dim, 1 << 20)
+    assert kv4.takes_chunks(1, 8, 4096, head_dim, 16384)

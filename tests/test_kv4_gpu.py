@@ -518,6 +518,12 @@ def test_masked_nan_reaches_the_query_that_sees_it_alone():
         assert out[0, :2].isfinite().all() and out[0, 2].isnan().all()
 
 
+def test_a_table_without_pages_is_empty_sequences():
+    from test_kv4_cpu import _no_pages
+
+    _no_pages("cuda")
+
+
 def test_bad_pages_inside_a_sequence():
     gen = _gen(24)
     H, Hq, D, group, page = 2, 4, 64, 32, 16

@@ -494,11 +494,12 @@ TDIST_API int tdist_kv4_chunk(const void* k_codes, const void* v_codes, const vo
   TDIST_REQUIRE(k_codes && v_codes && k_params && v_params && pages > 0 && kv_heads > 0 && page_size > 0 && page_size % 16 == 0 &&
                     (((uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k_params | (uintptr_t)v_params) & 15) == 0,
                 "a 4-bit cache needs four 16-byte aligned tensors, pages of a multiple of 16 tokens");
-  TDIST_REQUIRE(batch >= 0 && S >= 0 && q_heads > 0 && q_heads % kv_heads == 0 && max_pages >= 0, "bad head counts");
+  TDIST_REQUIRE(batch >= 0 && S >= 0 && q_heads > 0 && q_heads % kv_heads == 0 && max_pages >= 0 &&
+                    (long long)max_pages * page_size <= (1ll << 30), "bad head counts, or more than 2^30 tokens in a row of the table");
   TDIST_REQUIRE(splits >= 1 && splits <= 65535 && (splits == 1 || partial), "splits need their partial rows");
   TDIST_REQUIRE((out_mode == 1 || out_mode == 2) && (dtype == 0 || dtype == 1), "out_mode must be 1 or 2, dtype 0 (bf16) or 1 (fp16)");
   if (batch == 0 || S == 0) return 0;
-  TDIST_REQUIRE(q && table && kv_len && out && flags, "null argument");
+  TDIST_REQUIRE(q && (table || max_pages == 0) && kv_len && out && flags, "null argument");
   TDIST_REQUIRE(((uintptr_t)q & 15) == 0 && ((uintptr_t)out & 7) == 0 && ((q_sb | q_ss | q_sh) & 7) == 0,
                 "q rows must keep 16-byte alignment");
   const long long columns = (long long)(q_heads / kv_heads) * S;

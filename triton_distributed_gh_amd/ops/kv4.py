@@ -144,8 +144,8 @@ def _check_data(cache: Int4KVCache, **rows: torch.Tensor) -> None:
 def _check_index(cache: Int4KVCache, batch: int, block_table: torch.Tensor, **counts: Optional[torch.Tensor]) -> None:
     if not (block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[0] == batch
             and (block_table.shape[1] <= 1 or block_table.stride(1) == 1) and block_table.device == cache.device
-            and block_table.shape[1] * cache.page_size < 2 ** 31):
-        raise ValueError(f"block_table must be int32 [{batch}, max_pages] with contiguous rows of less than 2^31 tokens on "
+            and block_table.shape[1] * cache.page_size <= 2 ** 30):
+        raise ValueError(f"block_table must be int32 [{batch}, max_pages] with contiguous rows of at most 2^30 tokens on "
                          f"{cache.device}")
     for name, t in counts.items():
         if t is None:
@@ -299,6 +299,8 @@ def kv4_qkv_prep(qkv: torch.Tensor, q_w: Optional[torch.Tensor], k_w: Optional[t
                 and t.device == cache.device and t.shape == cos.shape):
             raise ValueError(f"cos / sin must be contiguous fp32 [positions, {D // 2}] on {cache.device}")
     _check_index(cache, batch, block_table, kv_offset=kv_offset, total_out=total_out)
+    if abs(total_out.data_ptr() - kv_offset.data_ptr()) < 4 * batch:
+        raise ValueError("total_out is written while kv_offset is read: they must not share memory")
     if batch == 0 or S == 0:
         total_out.copy_(kv_offset)
         return qkv.new_empty(batch, S, num_q_heads, D)
