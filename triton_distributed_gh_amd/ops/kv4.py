@@ -55,7 +55,7 @@ _CTYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "q": ctypes.c_longlong, "f":
 def _launch(name: str, device: torch.device, *args) -> None:
     """One native call on the current stream of ``device``.  (A decode step makes a few of these per layer: a token's worth of
     work on the GPU is shorter than a careless call, so streams and pointers are passed as plain integers.)"""
-    if device.index != torch.cuda.current_device():
+    if device.index != torch._C._cuda_getDevice():
         with torch.cuda.device(device):
             return _launch(name, device, *args)
     fn = getattr(_lib.hip(), name)
@@ -133,7 +133,7 @@ def _dt(dtype: torch.dtype) -> int:
 
 def _check_data(cache: Int4KVCache, **rows: torch.Tensor) -> None:
     for name, t in rows.items():
-        if t.dtype != cache.dtype:
+        if t.dtype is not cache.dtype:
             raise TypeError(f"{name} must be {cache.dtype} like the cache, got {t.dtype}")
         if t.device != cache.device:
             raise ValueError(f"{name} is on {t.device}, the cache on {cache.device}")
@@ -141,19 +141,18 @@ def _check_data(cache: Int4KVCache, **rows: torch.Tensor) -> None:
             raise RuntimeError(f"a 4-bit cache has no gradient: {name} requires one (detach it, or run under torch.no_grad())")
 
 
-def _check_index(cache: Int4KVCache, batch: int, block_table: torch.Tensor, **counts: Optional[torch.Tensor]) -> None:
-    if not (block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[0] == batch
-            and (block_table.shape[1] <= 1 or block_table.stride(1) == 1) and block_table.device == cache.device
-            and block_table.shape[1] * cache.page_size <= 2 ** 30):
-        raise ValueError(f"block_table must be int32 [{batch}, max_pages] with contiguous rows of at most 2^30 tokens on "
-                         f"{cache.device}")
-    for name, t in counts.items():
-        if t is None:
-            continue
-        n = batch + 1 if name == "cu_seqlens" else batch
-        if not (t.dtype == torch.int32 and t.dim() == 1 and t.shape[0] == n and (n <= 1 or t.stride(0) == 1)
-                and t.device == cache.device):
-            raise ValueError(f"{name} must be contiguous int32 [{n}] on {cache.device}")
+def _check_table(cache: Int4KVCache, batch: int, table: torch.Tensor) -> int:
+    """The pages of a row of the table."""
+    if table.dim() == 2 and table.dtype is torch.int32 and table.size(0) == batch and table.device == cache.device:
+        pages = table.size(1)
+        if (pages <= 1 or table.stride(1) == 1) and pages * cache.page_size <= 2 ** 30:
+            return pages
+    raise ValueError(f"block_table must be int32 [{batch}, max_pages] with contiguous rows of at most 2^30 tokens on {cache.device}")
+
+
+def _check_counts(cache: Int4KVCache, n: int, name: str, t: torch.Tensor) -> None:
+    if not (t.dtype is torch.int32 and t.dim() == 1 and t.numel() == n and t.is_contiguous() and t.device == cache.device):
+        raise ValueError(f"{name} must be contiguous int32 [{n}] on {cache.device}")
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
@@ -255,7 +254,10 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, cache: Int4KVCache, kv_offset: 
         raise ValueError(f"k and v must be [batch, S, {cache.kv_heads}, {cache.head_dim}], got {tuple(k.shape)} and {tuple(v.shape)}")
     batch, S = k.shape[:2]
     _check_data(cache, k=k, v=v)
-    _check_index(cache, batch, block_table, kv_offset=kv_offset, new_lens=new_lens)
+    pages = _check_table(cache, batch, block_table)
+    _check_counts(cache, batch, "kv_offset", kv_offset)
+    if new_lens is not None:
+        _check_counts(cache, batch, "new_lens", new_lens)
     if batch == 0 or S == 0:
         return
     if not k.is_cuda:
@@ -267,7 +269,7 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, cache: Int4KVCache, kv_offset: 
         return
     k, v = _rows(k), _rows(v)
     _launch("tdist_kv4_append", cache.device, *cache._native, k.data_ptr(), v.data_ptr(), *k.stride()[:3], *v.stride()[:3],
-            kv_offset.data_ptr(), _ptr(new_lens), block_table.data_ptr(), block_table.stride(0), block_table.shape[1], batch, S,
+            kv_offset.data_ptr(), _ptr(new_lens), block_table.data_ptr(), block_table.stride(0), pages, batch, S,
             _dt(cache.dtype))
 
 
@@ -298,7 +300,9 @@ def kv4_qkv_prep(qkv: torch.Tensor, q_w: Optional[torch.Tensor], k_w: Optional[t
         if not (t.dtype == torch.float32 and t.dim() == 2 and t.shape[1] == D // 2 and t.shape[0] > 0 and t.is_contiguous()
                 and t.device == cache.device and t.shape == cos.shape):
             raise ValueError(f"cos / sin must be contiguous fp32 [positions, {D // 2}] on {cache.device}")
-    _check_index(cache, batch, block_table, kv_offset=kv_offset, total_out=total_out)
+    pages = _check_table(cache, batch, block_table)
+    _check_counts(cache, batch, "kv_offset", kv_offset)
+    _check_counts(cache, batch, "total_out", total_out)
     if abs(total_out.data_ptr() - kv_offset.data_ptr()) < 4 * batch:
         raise ValueError("total_out is written while kv_offset is read: they must not share memory")
     if batch == 0 or S == 0:
@@ -326,7 +330,7 @@ def kv4_qkv_prep(qkv: torch.Tensor, q_w: Optional[torch.Tensor], k_w: Optional[t
     q = torch.empty((batch, S, num_q_heads, D), dtype=qkv.dtype, device=qkv.device)
     _launch("tdist_kv4_qkv_prep", cache.device, *cache._native, qkv.data_ptr(), *qkv.stride()[:2], _ptr(q_w), _ptr(k_w), q_eps,
             k_eps, pos.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0], q.data_ptr(), kv_offset.data_ptr(),
-            total_out.data_ptr(), block_table.data_ptr(), block_table.stride(0), block_table.shape[1], batch, S, num_q_heads)
+            total_out.data_ptr(), block_table.data_ptr(), block_table.stride(0), pages, batch, S, num_q_heads)
     return q
 
 
@@ -340,14 +344,16 @@ def kv4_read(cache: Int4KVCache, block_table: torch.Tensor, cu_seqlens: torch.Te
     Returns (k, v) ``[total, kv_heads, head_dim]`` - what ``flash_attn_varlen_fwd`` takes.  Rows that no sequence covers are
     left as they were (``out``) or unset; tokens without a page come out as zeros.  A finite value that its group's rounded
     scale carries beyond the type's largest number comes out as that number."""
-    batch = block_table.shape[0] if block_table.dim() == 2 else -1
-    _check_index(cache, batch, block_table, cu_seqlens=cu_seqlens, starts=starts)
+    batch = block_table.size(0) if block_table.dim() == 2 else -1
+    pages = _check_table(cache, batch, block_table)
+    _check_counts(cache, batch + 1, "cu_seqlens", cu_seqlens)
+    if starts is not None:
+        _check_counts(cache, batch, "starts", starts)
     if not 0 <= total < 2 ** 31:
         raise ValueError(f"total must be a row count, got {total}")
     shape = (int(total), cache.kv_heads, cache.head_dim)
     if out is None:
-        k = torch.empty(shape, dtype=cache.dtype, device=cache.device)
-        v = torch.empty_like(k)
+        k, v = cache.k_params.new_empty(shape), cache.k_params.new_empty(shape)
     else:
         k, v = out
         _check_data(cache, k_out=k, v_out=v)
@@ -367,7 +373,7 @@ def kv4_read(cache: Int4KVCache, block_table: torch.Tensor, cu_seqlens: torch.Te
         most = torch.finfo(cache.dtype).max
         k[r], v[r] = kk.clamp(max=most).to(cache.dtype), vv.clamp(max=most).to(cache.dtype)
         return k, v
-    _launch("tdist_kv4_read", cache.device, *cache._native, block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
+    _launch("tdist_kv4_read", cache.device, *cache._native, block_table.data_ptr(), block_table.stride(0), pages,
             cu_seqlens.data_ptr(), _ptr(starts), batch, int(total), k.data_ptr(), v.data_ptr(), *k.stride()[:2], *v.stride()[:2],
             _dt(cache.dtype))
     return k, v
@@ -450,7 +456,8 @@ def gqa_fwd_kv4(q: torch.Tensor, cache: Int4KVCache, kv_lens: torch.Tensor, bloc
         raise ValueError(f"q must be [batch, S, heads, {cache.head_dim}] with a multiple of {cache.kv_heads} heads, got {tuple(q.shape)}")
     batch, S, Hq, D = q4.shape
     _check_data(cache, q=q)
-    _check_index(cache, batch, block_table, kv_lens=kv_lens)
+    pages = _check_table(cache, batch, block_table)
+    _check_counts(cache, batch, "kv_lens", kv_lens)
     scale = D ** -0.5 if scale is None else float(scale)
     if not (math.isfinite(scale) and math.isfinite(soft_cap) and soft_cap >= 0):
         raise ValueError(f"scale must be finite, soft_cap 0 (off) or positive, got {scale} and {soft_cap}")
@@ -462,13 +469,13 @@ def gqa_fwd_kv4(q: torch.Tensor, cache: Int4KVCache, kv_lens: torch.Tensor, bloc
         return out.squeeze(1) if flat else out
     q4 = _rows(q4)
     columns = Hq // cache.kv_heads * S
-    room = block_table.shape[1] * cache.page_size
+    room = pages * cache.page_size
     chunk = takes_chunks(batch, cache.kv_heads, columns, D, room, soft_cap)
     splits = int(kv_split) if kv_split > 0 else auto_kv_splits(batch, cache.kv_heads, columns, D, room, chunk=chunk)
     out = torch.empty((batch, S, Hq, D + 1), dtype=torch.float32, device=q.device) if return_lse else \
         torch.empty_like(q4, memory_format=torch.contiguous_format)
     part = torch.empty(batch * S * Hq * splits * (D + 1), dtype=torch.float32, device=q.device) if splits > 1 else None
-    call = (*cache._native, q4.data_ptr(), *q4.stride()[:3], block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
+    call = (*cache._native, q4.data_ptr(), *q4.stride()[:3], block_table.data_ptr(), block_table.stride(0), pages,
             kv_lens.data_ptr(), _ptr(part), out.data_ptr(), batch, S, Hq, splits, 1 if causal else 0, 2 if return_lse else 1, scale)
     flags, at_once = None, 0
     if chunk:
