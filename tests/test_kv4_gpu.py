@@ -338,15 +338,18 @@ def test_chunks_with_blocks_that_fp16_does_not_reach(D, group, splits, chunks):
     way, the rest does not, and the columns of both are right."""
     gen = _gen(45)
     S, H, Hq, page = 100, 2, 4, 16
-    for what in range(6):
+    for what in range(7):
         cache, table, ks, vs = oracle.filled(gen, [600], H, D, group, page, torch.bfloat16, "cuda")
         k, v, there = ks[0].clone(), vs[0].clone(), torch.ones(600, dtype=torch.bool)
         if what == 0:
             k[37, 1, 3] = 2.0 ** 16
         elif what == 1:
-            k[64:128] *= 2.0 ** -12
+            k[64:128] *= 2.0 ** -17
         elif what == 2:
-            v[192:256] *= 2.0 ** -14
+            v[192:256] *= 2.0 ** -18
+        elif what == 6:                     # (small, but not for the other kernel)
+            k[64:128] *= 2.0 ** -10
+            v[192:256] *= 2.0 ** -11
         elif what == 3:
             v[590:] *= 2.0 ** 17
         elif what == 4:

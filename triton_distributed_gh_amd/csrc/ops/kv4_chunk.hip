@@ -11,16 +11,18 @@
 // weight cancels where that weight is nearly all of the sum.  Values rounded to fp16 are within 2^-11 of themselves, as near as
 // `kv4_read` brings them for fp16 caches and eight times as near as for bf16.  The reference m moves as in kv4_attn.hip.
 //
-// fp16 does not reach as far as bf16: a block of tokens whose values come to 2^15 or whose largest one is under 2^-6 (K) or
-// 2^-9 (V), a NaN in a scale and a page that is none are for the other kernel.  Whoever meets one says so in `flags`, one int per
-// workgroup, written by every launch; the other kernel runs behind this one and takes just the flagged workgroups' columns.
+// fp16 does not reach as far as bf16: values of 2^15, sixteen tokens' groups of K or thirty-two's of V whose largest value is
+// under 2^-11 and not 0 (fp16's smallest numbers are 2^-25 off at most, 2^-14 of it from there on), a NaN in a scale and a page
+// that is none are for the other kernel.  Whoever meets one says so in `flags`, one int per workgroup, written by every launch;
+// the other kernel runs behind this one and takes just the flagged workgroups' columns.
 //
-// What bounds it: 1024 new tokens over 16384, 32 / 8 heads of 128 (266 GFLOP): 312 .. 350 us in all, 760 .. 850 TFLOP/s where a
+// What bounds it: 1024 new tokens over 16384, 32 / 8 heads of 128 (266 GFLOP): 306 .. 312 us in all, 850 .. 870 TFLOP/s where a
 // large bf16 matrix product reaches 1203; the other kernel takes 511.  Of a SIMD's cycles its matrix unit has 37 %, vector
-// instructions 48 % - a third of them unpacking, a fifth the exponentials - and two waves hardly overlap the two.  Eight waves
-// with one set of buffers against twice four: 346 and 367 us (with half the columns for a workgroup, unpacking costs twice as
-// much); scores of the next 32 tokens made ahead of time from a third buffer: 348, and 99 for 77 where heads of 256 then need
-// shorter blocks; all 64 tokens' scores at once spill registers.
+// instructions 48 %, and two waves hardly overlap the two.  Timing-only builds of 349 us (launches apart from each other): 279
+// without the unpacking, 294 without V's way back from LDS, 311 with half of the second product, 334 without the exponentials.
+// Eight waves with one set of buffers against twice four: 346 and 367 us (with half the columns for a workgroup, unpacking costs
+// twice as much); scores of the next 32 tokens made ahead of time from a third buffer: 348, and 99 for 77 where heads of 256 then
+// need shorter blocks; all 64 tokens' scores at once spill registers; operands read ahead of the references 346.
 #include <algorithm>
 
 #include "tdist/kv4.hpp"
@@ -98,7 +100,7 @@ __global__ __launch_bounds__(NW * 64, 2) void kv4_chunk_kernel(ChunkArgs a, cons
   constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
   constexpr float NONE = -1e30f;        // the reference before the first token
   constexpr float AT = 6.f, MOST = 14.f;  // log2 of the largest P: where a new reference puts it, and where it may grow to
-  constexpr float FAR = 0x1p15f, NEAR_K = 0x1p-6f, NEAR_V = 0x1p-9f;
+  constexpr float FAR = 0x1p15f, NEAR = 0x1p-11f;
   __shared__ __attribute__((aligned(16))) u32x4 s_k[2][4][KS][64];
   __shared__ __attribute__((aligned(16))) u32x4 s_v[2][2][NT][64];
   __shared__ int s_bad;
@@ -267,7 +269,7 @@ __global__ __launch_bounds__(NW * 64, 2) void kv4_chunk_kernel(ChunkArgs a, cons
     for (int g = 0; g < KG; ++g) {
       const float s = scale_of<IS_BF16>(r.kp[g]), l = low_of<IS_BF16>(r.kp[g]);
       const float size = __builtin_fmaf(15.f, s, fabsf(l));
-      const bool far = !(size < FAR), near = !__any(size >= NEAR_K) & size > 0.f;
+      const bool far = !(size < FAR), near = !__any(size >= NEAR) & size > 0.f;
       bad |= far | near;
       scale[g] = both(s, s), low[g] = both(l, l);
     }
@@ -300,7 +302,7 @@ __global__ __launch_bounds__(NW * 64, 2) void kv4_chunk_kernel(ChunkArgs a, cons
             }
             sv[g][k] = both(s[0], s[1]), lv[g][k] = both(l[0], l[1]);
           }
-          const bool near = !__any(top >= NEAR_V) & top > 0.f;
+          const bool near = !__any(top >= NEAR) & top > 0.f;
           bad |= !fine | near;
         }
         const u32x2 v0 = r.v[n][0], v1 = r.v[n][1];
