@@ -187,15 +187,29 @@ def test_projection_writes_the_bits_of_the_cpu_path(D, group, B, S, norm):
     assert (a == b).float().mean() > 0.999
 
 
-def _check(got, want, lse_got, lse, dtype, v_max, cache_dtype=torch.bfloat16, scores=1.0):
+def _fp16_keys(q, keys, scale):
+    """What rounding K to fp16 (2^-11 of each value at most) can do to a score of q [B, S, Hq, D] over lists of [L, Hkv, D]."""
+    worst = 0.0
+    for x, k in zip(q.double().abs().cpu(), keys):
+        k = k.abs().nan_to_num(0.0).transpose(0, 1)                            # [Hkv, L, D]
+        x = x.transpose(0, 1).reshape(k.shape[0], -1, k.shape[2])               # [Hkv, heads and tokens, D]
+        if k.numel():
+            worst = max(worst, float((x @ k.transpose(1, 2)).max()))
+    return 2.0 ** -11 * abs(scale) * worst
+
+
+def _check(got, want, lse_got, lse, dtype, v_max, cache_dtype=torch.bfloat16, scores=1.0, rounded=None):
+    """``rounded``: K and V are fp16 numbers on the way, which moves a score by that at most: an LSE by as much, an output,
+    sum of p_i e_i (v_i - out), by 2 v_max as much, and by V's own 2^-11."""
     assert torch.equal(got.isnan().cpu(), want.isnan())
     off = (got.double().cpu() - want).abs()
-    assert (off <= oracle.bounds(want, dtype, v_max, cache_dtype, scores)).all(), off.max()
+    extra = 0.0 if rounded is None else 2 * rounded + 2.0 ** -11
+    assert (off <= oracle.bounds(want, dtype, v_max, cache_dtype, scores) + extra * v_max).all(), off.max()
     if lse_got is not None:
         assert torch.equal(lse_got.cpu() == -math.inf, lse == -math.inf)
         fine = lse != -math.inf
         # a score's 8e-5 six times over, and the half step of an fp32 LSE that is not near 1
-        assert ((lse_got.double().cpu() - lse)[fine].abs() <= scores * 5e-4 + 2.0 ** -24 * lse[fine].abs()).all()
+        assert ((lse_got.double().cpu() - lse)[fine].abs() <= scores * 5e-4 + (rounded or 0.0) + 2.0 ** -24 * lse[fine].abs()).all()
 
 
 ATTEND = [
@@ -312,9 +326,6 @@ CHUNKS = [
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("lens,S,Hq,H,D,group,page,splits", CHUNKS)
 def test_many_columns_against_the_definition(lens, S, Hq, H, D, group, page, splits, dtype, chunks):
-    """In a chunk's values V is rounded to the fp16 that the bits of P are, too: 2^-11 of a value and of a weight, and K's
-    rounding of 2^-11 moves a score by 2^-11 / sqrt(3) |q| |k| / sqrt(D) = 3e-4 of a nat (one deviation, |q|, |k| = sqrt(D)):
-    by the two-token bound 1 / 4 * sqrt(2) * 3e-4 * 2 v_max = 2.1e-4 v_max, three deviations 6.4e-4."""
     gen = _gen(sum(lens) + S)
     cache, table, ks, vs = oracle.filled(gen, lens, H, D, group, page, dtype, "cuda", room=max(lens) + 40)
     q = oracle.rows(gen, len(lens), S, Hq, D, dtype=dtype, device="cuda")
@@ -326,8 +337,9 @@ def test_many_columns_against_the_definition(lens, S, Hq, H, D, group, page, spl
         out = kv4.gqa_fwd_kv4(q, cache, n, table, kv_split=splits, causal=causal)
         full = kv4.gqa_fwd_kv4(q, cache, n, table, kv_split=splits, causal=causal, return_lse=True)
         torch.cuda.synchronize()
-        _check(out, want, None, None, dtype, v_max, scores=3.0)
-        _check(full[..., :D], want, full[..., D], lse, torch.float32, v_max, scores=3.0)
+        e = _fp16_keys(q, keys, D ** -0.5)
+        _check(out, want, None, None, dtype, v_max, rounded=e)
+        _check(full[..., :D], want, full[..., D], lse, torch.float32, v_max, rounded=e)
         assert torch.equal(out, kv4.gqa_fwd_kv4(q, cache, n, table, kv_split=splits, causal=causal))
 
 
@@ -369,7 +381,8 @@ def test_chunks_with_blocks_that_fp16_does_not_reach(D, group, splits, chunks):
             assert got[0, 55:, :2].isnan().all() and got[0, :55].isfinite().all() and got[0, :, 2:].isfinite().all()
             want[0, 55:, :2], lse[0, 55:, :2] = 0.0, 0.0
             got[0, 55:, :2] = 0.0
-        _check(got[..., :D], want, got[..., D], lse, torch.float32, float(values[0].abs().max()), scores=3.0)
+        _check(got[..., :D], want, got[..., D], lse, torch.float32, float(values[0].nan_to_num(0.0).abs().max()),
+               rounded=_fp16_keys(q, keys, D ** -0.5))
 
 
 @pytest.mark.parametrize("scale", [-0.11, 0.0, 0.3])
@@ -390,7 +403,7 @@ def test_chunks_at_other_scales_strides_and_streams(scale, chunks):
     torch.cuda.synchronize()
     assert torch.equal(here, there)
     _check(here[..., :D], want, here[..., D], lse, torch.float32, max(float(x.abs().max()) for x in values),
-           scores=3.0 * max(1.0, abs(scale) * D ** 0.5))
+           scores=max(1.0, abs(scale) * D ** 0.5), rounded=_fp16_keys(q, keys, scale))
 
 
 def test_chunks_replay_from_a_graph(chunks):
@@ -432,7 +445,8 @@ def test_large_chunks_and_small_ones_agree(monkeypatch):
     other = kv4.gqa_fwd_kv4(q, cache, n, table, return_lse=True)
     torch.cuda.synchronize()
     v_max = float(vs[0].abs().max())
-    _check(one[..., :D], other[..., :D].double().cpu(), one[..., D], other[..., D].double().cpu(), torch.float32, v_max, scores=4.0)
+    _check(one[..., :D], other[..., :D].double().cpu(), one[..., D], other[..., D].double().cpu(), torch.float32, v_max, scores=2.0,
+           rounded=_fp16_keys(q, [oracle.held(ks[0], group)], D ** -0.5))
 
 
 @pytest.mark.parametrize("scale,soft_cap", [(-0.11, 0.0), (0.3, 7.0), (-0.3, 7.0), (0.0, 0.0), (0.0, 5.0), (0.1, 1e-30)])
