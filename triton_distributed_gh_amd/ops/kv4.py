@@ -157,8 +157,10 @@ def _check_counts(cache: Int4KVCache, n: int, name: str, t: torch.Tensor) -> Non
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
     """``x`` itself where the kernels can take its rows 16 bytes at a time, else a contiguous copy."""
-    *outer, last = x.stride()
-    if last == 1 and x.data_ptr() % 16 == 0 and not any(s % 8 for s in outer):
+    strides, bits = x.stride(), 0
+    for s in strides[:-1]:
+        bits |= s
+    if strides[-1] == 1 and bits % 8 == 0 and x.data_ptr() % 16 == 0:
         return x
     return x.clone(memory_format=torch.contiguous_format)
 
@@ -296,10 +298,10 @@ def kv4_qkv_prep(qkv: torch.Tensor, q_w: Optional[torch.Tensor], k_w: Optional[t
                 raise ValueError(f"norm weights are contiguous [{D}]")
     if not (position_ids.shape == (batch, S) and position_ids.device == cache.device):
         raise ValueError(f"position_ids must be [{batch}, {S}] on {cache.device}")
-    for t in (cos, sin):
-        if not (t.dtype == torch.float32 and t.dim() == 2 and t.shape[1] == D // 2 and t.shape[0] > 0 and t.is_contiguous()
-                and t.device == cache.device and t.shape == cos.shape):
-            raise ValueError(f"cos / sin must be contiguous fp32 [positions, {D // 2}] on {cache.device}")
+    if not (cos.dtype is torch.float32 and sin.dtype is torch.float32 and cos.dim() == 2 and cos.size(1) == D // 2 and cos.size(0) > 0
+            and cos.shape == sin.shape and cos.is_contiguous() and sin.is_contiguous() and cos.device == cache.device
+            and sin.device == cache.device):
+        raise ValueError(f"cos / sin must be contiguous fp32 [positions, {D // 2}] on {cache.device}")
     pages = _check_table(cache, batch, block_table)
     _check_counts(cache, batch, "kv_offset", kv_offset)
     _check_counts(cache, batch, "total_out", total_out)
@@ -308,7 +310,9 @@ def kv4_qkv_prep(qkv: torch.Tensor, q_w: Optional[torch.Tensor], k_w: Optional[t
     if batch == 0 or S == 0:
         total_out.copy_(kv_offset)
         return qkv.new_empty(batch, S, num_q_heads, D)
-    pos = position_ids.to(torch.int64).contiguous()
+    pos = position_ids
+    if pos.dtype is not torch.int64 or not pos.is_contiguous():
+        pos = pos.to(torch.int64).contiguous()
     if not qkv.is_cuda:
         q, k, v = qkv.unflatten(-1, (-1, D)).split([num_q_heads, Hkv, Hkv], 2)
         at = pos.clamp(0, cos.shape[0] - 1)
@@ -326,8 +330,8 @@ def kv4_qkv_prep(qkv: torch.Tensor, q_w: Optional[torch.Tensor], k_w: Optional[t
         total_out.copy_(kv_offset + S)
         return q
     qkv = _rows(qkv)
-    q_w, k_w = (w if w is None else _rows(w) for w in (q_w, k_w))
-    q = torch.empty((batch, S, num_q_heads, D), dtype=qkv.dtype, device=qkv.device)
+    q_w, k_w = (w if w is None or w.data_ptr() % 16 == 0 else w.clone() for w in (q_w, k_w))
+    q = qkv.new_empty((batch, S, num_q_heads, D))
     _launch("tdist_kv4_qkv_prep", cache.device, *cache._native, qkv.data_ptr(), *qkv.stride()[:2], _ptr(q_w), _ptr(k_w), q_eps,
             k_eps, pos.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0], q.data_ptr(), kv_offset.data_ptr(),
             total_out.data_ptr(), block_table.data_ptr(), block_table.stride(0), pages, batch, S, num_q_heads)
