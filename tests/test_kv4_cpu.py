@@ -365,3 +365,18 @@ def test_split_and_chunk_rules_stay_within_their_launches(head_dim):
                 assert not kv4.takes_chunks(batch, 8, columns, head_dim, capacity, 1.0)
     assert not kv4.takes_chunks(64, 8, 16, head_dim, 1 << 20)
     assert kv4.takes_chunks(1, 8, 4096, head_dim, 16384)
+
+
+def test_copies_of_a_cache_have_their_own_memory():
+    import copy
+    import pickle
+
+    gen = _gen(52)
+    cache, table, _, _ = oracle.filled(gen, [20], 2, 64, 32, 16)
+    before = cache.k_codes.clone()
+    for twin in (copy.deepcopy(cache), pickle.loads(pickle.dumps(cache))):
+        tensors = (twin.k_codes, twin.v_codes, twin.k_params, twin.v_params)
+        assert twin._native[:4] == tuple(t.data_ptr() for t in tensors) and twin._native[4:] == cache._native[4:]
+        rows = oracle.rows(gen, 1, 20, 2, 64)
+        kv4.kv4_append(rows, rows, twin, int32([0]), table)
+        assert torch.equal(cache.k_codes, before) and not torch.equal(twin.k_codes, before)

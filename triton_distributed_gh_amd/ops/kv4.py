@@ -80,7 +80,8 @@ class Int4KVCache:
     """One layer's pages.  The four tensors are packed as csrc/include/tdist/kv4.hpp describes; ``kv4_read`` gives the values.
 
     ``k_codes [pages, kv_heads, page_size, head_dim / 2]`` and ``v_codes [pages, kv_heads, page_size / 4, 2 * head_dim]`` uint8,
-    ``k_params`` / ``v_params [pages, kv_heads, head_dim / group, page_size, 2]`` (scale, low) in ``dtype``."""
+    ``k_params`` / ``v_params [pages, kv_heads, head_dim / group, page_size, 2]`` (scale, low) in ``dtype``.  Checked once, here:
+    the tensors keep their memory as long as the cache is used (their contents may change, by whatever means)."""
 
     k_codes: torch.Tensor
     v_codes: torch.Tensor
@@ -109,6 +110,9 @@ class Int4KVCache:
         for name, value in dict(num_pages=P, kv_heads=H, page_size=S, head_dim=D, group=G, dtype=kp.dtype, device=k.device,
                                 _native=native).items():
             object.__setattr__(self, name, value)
+
+    def __reduce__(self):       # (copies and pickles are caches of their own tensors)
+        return Int4KVCache, (self.k_codes, self.v_codes, self.k_params, self.v_params)
 
     @classmethod
     def alloc(cls, num_pages: int, page_size: int, kv_heads: int, head_dim: int, group: int = 64, dtype=torch.bfloat16,
