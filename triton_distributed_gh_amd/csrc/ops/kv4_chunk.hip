@@ -16,7 +16,7 @@
 // that is none are for the other kernel.  Whoever meets one says so in `flags`, one int per workgroup, written by every launch;
 // the other kernel runs behind this one and takes just the flagged workgroups' columns.
 //
-// What bounds it: 1024 new tokens over 16384, 32 / 8 heads of 128 (266 GFLOP): 306 .. 312 us in all, 850 .. 870 TFLOP/s where a
+// What bounds it: 1024 new tokens over 16384, 32 / 8 heads of 128 (266 GFLOP): 301 .. 312 us in all, 850 .. 880 TFLOP/s where a
 // large bf16 matrix product reaches 1203; the other kernel takes 511.  Of a SIMD's cycles its matrix unit has 37 %, vector
 // instructions 48 %, and two waves hardly overlap the two.  Timing-only builds of 349 us (launches apart from each other): 279
 // without the unpacking, 294 without V's way back from LDS, 311 with half of the second product, 334 without the exponentials.

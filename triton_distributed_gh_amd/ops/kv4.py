@@ -434,9 +434,10 @@ def auto_kv_splits(batch: int, kv_heads: int, columns: int, head_dim: int, capac
     """KV splits of a launch: ``columns`` = new tokens times query heads of a KV head, ``capacity`` = tokens of a sequence's pages.
 
     One round of the chip: a CU holds two workgroups, and a third round of nothing but start-up costs more than it gives.
-    Measured (32 / 8 heads of 128, groups of 64, microseconds): 131072 tokens of one sequence 43.2 / 36.4 / 41.2 with 32 / 64 / 96
-    splits; 16 x 4096 26.3 / 23.2 / 27.1 with 2 / 4 / 8; 64 x 4096 55.3 / 64.8 with 1 / 2.  At least 128 tokens each: 512 tokens
-    9.8 / 8.8 with 2 / 4, 2048 tokens 9.8 / 8.9 with 8 / 16; beyond sixteen splits 256: 8192 tokens 10.3 / 11.0 with 32 / 64.
+    Measured (32 / 8 heads of 128, groups of 64, microseconds): 131072 tokens of one sequence 38.2 / 35.6 / 42.2 with 32 / 64 / 96
+    splits; 16 x 4096 23.1 / 20.3 / 24.7 with 2 / 4 / 8; 64 x 4096 55.9 / 61.9 with 1 / 2.  At least 128 tokens each: 2048 tokens 9.5 /
+    8.9 with 8 / 16; beyond sixteen splits 256: 8192 tokens 10.3 / 11.0 with 32 / 64.  Up to 512 tokens in one piece: 256 tokens
+    6.8 / 8.3 with 1 / 2, 512 8.5 / 8.6 with 1 / 4 (640: 9.3 / 8.6 with 1 / 6), and one launch instead of two on the host, 11 / 15.
 
     ``chunk``: of a launch that `takes_chunks`; one workgroup fills a CU there (1024 new tokens over 16384: 613 / 356 / 443 with 1 /
     2 / 3; 256 over 16384 126 / 106 / 128 with 6 / 8 / 16)."""
@@ -445,7 +446,7 @@ def auto_kv_splits(batch: int, kv_heads: int, columns: int, head_dim: int, capac
         return max(1, min(num_cus // max(1, groups), capacity // 256, 64))
     per_group = 32 if columns > 16 and head_dim <= 128 else 16          # columns of a workgroup
     groups = batch * kv_heads * (-(-columns // per_group))
-    most = min(capacity // 128, max(16, capacity // 256), 64)
+    most = 1 if capacity <= 512 else min(capacity // 128, max(16, capacity // 256), 64)
     return max(1, min(2 * num_cus // max(1, groups), most))
 
 
