@@ -852,13 +852,15 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(const float* __restrict_
     for (int s = s0 + lane; s < min(splits, s0 + AT_ONCE * ROUNDS); s += 64) peak = fmaxf(peak, l[s]);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) peak = fmaxf(peak, __shfl_xor(peak, o));
-    if (peak == -INFINITY) peak = 0.f;    // no split has a token (or what they have is NaN, which the weights keep)
-    const float f = exp2_fast(top - peak);
+    // As long as no split has had a token (or only NaN, which the weights keep), what is subtracted is 0, but `top` stays where
+    // it is: a 0 kept there would be the reference of all later passes, however far below it their sums are.
+    const float from = peak == -INFINITY ? 0.f : peak;
+    const float f = exp2_fast(top - from);
     sum *= f;
     acc *= f;
 #pragma unroll
     for (int i = 0; i < ROUNDS; ++i) {
-      const float w = exp2_fast(mine[i] - peak);
+      const float w = exp2_fast(mine[i] - from);
       sum += w;
 #pragma unroll
       for (int k = 0; k < 4; ++k) acc[k] += w != 0.f ? w * v[i][k] : 0.f;      // (a split without tokens has written no sums)
