@@ -380,3 +380,19 @@ def test_copies_of_a_cache_have_their_own_memory():
         rows = oracle.rows(gen, 1, 20, 2, 64)
         kv4.kv4_append(rows, rows, twin, int32([0]), table)
         assert torch.equal(cache.k_codes, before) and not torch.equal(twin.k_codes, before)
+
+
+def test_tables_whose_rows_are_2_to_the_31_entries_apart_are_refused():
+    """The kernels take a row's distance in 32 bits: a longer one would be cut, and the rows looked for elsewhere."""
+    cache = kv4.Int4KVCache.alloc(4, 16, 2, 64, group=32, device="meta")
+    rows, cu = torch.zeros(2, 1, 2, 64, dtype=torch.bfloat16, device="meta"), int32([0, 1, 2], "meta")
+    n = int32([1, 1], "meta")
+    far = torch.empty_strided((2, 2), (2 ** 31, 1), dtype=torch.int32, device="meta")
+    for call in (lambda: kv4.kv4_append(rows, rows, cache, n, far), lambda: kv4.kv4_read(cache, far, cu, 2),
+                 lambda: kv4.gqa_fwd_kv4(rows, cache, n, far),
+                 lambda: kv4.kv4_qkv_prep(rows.view(2, 1, 128).repeat(1, 1, 3), None, None, 0.0, 0.0, n.long().view(2, 1),
+                                          torch.zeros(8, 32, device="meta"), torch.zeros(8, 32, device="meta"), cache, n, n.clone(), far, 2)):
+        with pytest.raises(ValueError, match="2\\^31 entries"):
+            call()
+    near = torch.empty_strided((2, 2), (2 ** 31 - 1, 1), dtype=torch.int32, device="meta")
+    assert kv4._check_table(cache, 2, near) == 2

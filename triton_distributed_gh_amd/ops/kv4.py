@@ -149,9 +149,10 @@ def _check_table(cache: Int4KVCache, batch: int, table: torch.Tensor) -> int:
     """The pages of a row of the table."""
     if table.dim() == 2 and table.dtype is torch.int32 and table.size(0) == batch and table.device == cache.device:
         pages = table.size(1)
-        if (pages <= 1 or table.stride(1) == 1) and pages * cache.page_size <= 2 ** 30:
+        if (pages <= 1 or table.stride(1) == 1) and pages * cache.page_size <= 2 ** 30 and table.stride(0) < 2 ** 31:
             return pages
-    raise ValueError(f"block_table must be int32 [{batch}, max_pages] with contiguous rows of at most 2^30 tokens on {cache.device}")
+    raise ValueError(f"block_table must be int32 [{batch}, max_pages] with contiguous rows of at most 2^30 tokens, less than 2^31 entries "
+                     f"apart, on {cache.device}")
 
 
 def _check_counts(cache: Int4KVCache, n: int, name: str, t: torch.Tensor) -> None:
