@@ -54,3 +54,182 @@ def test_splits_without_any_token_are_an_empty_row():
     got = kv4.gqa_fwd_kv4(q, cache, int32([128 * 70], "cuda"), table, kv_split=70, return_lse=True)
     torch.cuda.synchronize()
     assert (got[..., :128] == 0).all() and (got[..., 128] == -math.inf).all()
+
+
+# ---- many columns ---------------------------------------------------------------------------------------------------
+@pytest.fixture
+def chunks(monkeypatch):
+    monkeypatch.setattr(kv4, "takes_chunks", lambda *a: a[2] >= 32 and a[5] == 0)
+
+
+def _first_rows(D, group, size, q_size, k_size, rows):
+    """A prompt of 96 tokens, the first ``rows`` of them with V of ``size`` and K of ``k_size``; (out [96, Hq, D], lse) and what
+    is exact."""
+    gen = _gen(D + group)
+    L, H, Hq, page = 96, 1, 2, 16
+    table, pages = oracle.table_for(1, L, page, gen, device="cuda")
+    cache = kv4.Int4KVCache.alloc(pages, page, H, D, group=group, device="cuda")
+    k, v = oracle.rows(gen, L, H, D), oracle.rows(gen, L, H, D)
+    k[:rows] *= k_size
+    v[:rows] *= size
+    kv4.kv4_append(k[None].cuda(), v[None].cuda(), cache, int32([0], "cuda"), table)
+    q = oracle.rows(gen, 1, L, Hq, D, device="cuda") * q_size
+    got = kv4.gqa_fwd_kv4(q, cache, int32([L], "cuda"), table, return_lse=True)
+    torch.cuda.synchronize()
+    keys, values = oracle.held(k, group), oracle.held(v, group)
+    want, lse = oracle.attention(q[:, :rows], [keys[:rows]], [values[:rows]], D ** -0.5)
+    return got[0, :rows].double().cpu(), want[0], lse[0], values[:rows]
+
+
+@pytest.mark.parametrize("size", [1e-2, 1e-3, 1e-4, 1e-5, 1e-6, 0.0])
+@pytest.mark.parametrize("D,group", [(64, 64), (128, 32), (128, 128), (256, 64)])
+def test_rows_that_see_small_values_alone(D, group, size, chunks):
+    """The first rows of a prompt see tokens whose V is far smaller than that of the tokens beside them, which they do not see:
+    what comes out is as near, measured by their own size, as for any other row.
+
+    Row 0 sees one token, and no weight is rounded in its result: a value is an fp16 number at most 2^-11 of itself off or, at the
+    smallest size that is taken so, 17 halves of fp16's last step (15 from the scale, one from low, one from the result) of a group
+    no smaller than 2^-9: 17 * 2^-25 / 2^-9 < 2^-11.9 of the group's 15 scale + |low| <= 3 max |v|.  Where codes are multiplied instead, P
+    times scale is an fp16 number: 2^-11 of 15 scale.  Together under 2^-11 |v| + 2^-11 * 3 max |v| <= 2^-9 max |v| of its group."""
+    got, want, lse, values = _first_rows(D, group, size, 1.0, 1.0, 3)
+    top = values.abs().unflatten(-1, (-1, group)).amax(-1).repeat_interleave(group, -1)     # [rows, H, D]
+    off = (got[0, :, :D] - want[0]).abs()
+    assert (off <= 2.0 ** -9 * top[0]).all(), float((off / top[0].clamp(min=1e-30)).max())
+    # rows 1 and 2: the weights' own errors too, on what their tokens hold (2^-11 of a weight, and 2^-11 for the scores)
+    for r in (1, 2):
+        off = (got[r, :, :D] - want[r]).abs()
+        assert (off <= (2.0 ** -9 + 2.0 ** -10 + 2.0 ** -11) * top[:r + 1].amax(0)).all()
+
+
+@pytest.mark.parametrize("k_size,q_size", [(2.0 ** -20, 2.0 ** 20), (2.0 ** -14, 2.0 ** 14), (2.0 ** -12, 2.0 ** 8), (2.0 ** -20, 1.0)])
+@pytest.mark.parametrize("D,group", [(64, 64), (128, 32), (128, 128), (256, 64)])
+def test_rows_that_see_small_keys_alone(D, group, k_size, q_size, chunks):
+    """The same for K, with queries that are large enough for scores of a few nats from such keys."""
+    got, want, lse, values = _first_rows(D, group, 1.0, q_size, k_size, 12)
+    scores = max(1.0, k_size * q_size)
+    off = (got[..., :D] - want).abs()
+    # K as fp16 numbers: 2^-11 of a score's terms (|q| |k| summed, about 8 nats here at scores of 1) at most, on either side of
+    # a weight; then the bounds of the weights and the scores
+    assert (off <= oracle.bounds(want, torch.float32, float(values.abs().max()), scores=scores) + 2.0 ** -11 * 8 * 2 * float(values.abs().max())).all()
+    assert ((got[..., D] - lse).abs() <= scores * 5e-4 + 2.0 ** -11 * 8).all()
+
+
+def _flags(q, cache, lens, table, splits, scale):
+    """What csrc/ops/kv4_chunk.hip leaves to the other kernel: [column blocks, batch, splits, KV heads]."""
+    batch, S, Hq, D = q.shape
+    at_once = kv4.CHUNK_COLUMNS[D]
+    blocks = -(-(Hq // cache.kv_heads * S) // at_once)
+    flags = torch.full((blocks, batch, splits, cache.kv_heads), 7, dtype=torch.int32, device="cuda")
+    part = torch.empty(batch * S * Hq * splits * (D + 1), dtype=torch.float32, device="cuda")
+    out = torch.empty(batch, S, Hq, D + 1, dtype=torch.float32, device="cuda")
+    args = [*cache._native, q.data_ptr(), *q.stride()[:3], table.data_ptr(), table.stride(0), table.shape[1], lens.data_ptr(),
+            part.data_ptr(), out.data_ptr(), batch, S, Hq, splits, 1, 2, scale]
+    kv4._launch("tdist_kv4_chunk", cache.device, *args, 0, flags.data_ptr(), at_once)
+    torch.cuda.synchronize()
+    return flags.cpu()
+
+
+@pytest.mark.parametrize("D,group", [(64, 64), (128, 32), (128, 128), (256, 64)])
+def test_what_goes_to_the_other_kernel(D, group):
+    """Exactly the splits and heads that hold something fp16 values do not reach are flagged; small values that they do reach, and
+    small keys under ordinary queries, are not."""
+    S, H, Hq, page, splits, L = 50, 2, 4, 16, 3, 600            # splits: tokens 0 .. 255, 256 .. 511, 512 .. 599
+    cases = [
+        ("nothing", None, []),
+        ("small V", lambda k, v, q: v[192:256].mul_(2.0 ** -11), []),
+        ("small K", lambda k, v, q: k[64:128].mul_(2.0 ** -17), []),
+        ("small K of one token", lambda k, v, q: k[70].mul_(2.0 ** -17), []),
+        ("V of zero", lambda k, v, q: v[0].zero_(), []),
+        ("large K", lambda k, v, q: k[37, 1, 3].fill_(2.0 ** 16), [(0, 1)]),
+        ("large V", lambda k, v, q: v[590:, 0].mul_(2.0 ** 17), [(2, 0)]),
+        ("tiny V of one token", lambda k, v, q: v[300, 1].mul_(2.0 ** -24), [(1, 1)]),
+        ("tiny V", lambda k, v, q: v[192:320].mul_(2.0 ** -24), [(0, 0), (0, 1), (1, 0), (1, 1)]),
+        ("a NaN", lambda k, v, q: k[555, 0, 0].fill_(math.nan), [(2, 0)]),
+        ("large queries, small K", lambda k, v, q: (q.mul_(2.0 ** 14), k[255, 0].mul_(2.0 ** -14)), [(0, 0)]),
+        ("a page that is none", "page", [(1, 0), (1, 1)]),
+    ]
+    for name, change, wanted in cases:
+        gen = _gen(45)
+        cache, table, ks, vs = oracle.filled(gen, [L], H, D, group, page, torch.bfloat16, "cuda")
+        k, v, q = ks[0].clone(), vs[0].clone(), oracle.rows(gen, 1, S, Hq, D, device="cuda")
+        if change == "page":
+            table[0, 20] = -1
+        elif change is not None:
+            change(k, v, q)
+            kv4.kv4_append(k[None], v[None], cache, int32([0], "cuda"), table)
+        flags = _flags(q, cache, int32([L], "cuda"), table, splits, D ** -0.5)
+        expect = torch.zeros_like(flags)
+        for split, head in wanted:
+            expect[:, 0, split, head] = 1
+        assert torch.equal(flags, expect), (name, flags.tolist())
+
+
+CHUNKS = [
+    # lens, S, Hq, Hkv, D, group, page, splits
+    ([64], 64, 1, 1, 128, 64, 16, 1),
+    ([300, 70, 0, 129], 70, 4, 2, 128, 64, 16, 1),
+    ([777], 40, 14, 2, 128, 32, 48, 3),
+    ([2000], 65, 2, 1, 128, 128, 64, 2),
+    ([513, 1], 96, 4, 4, 64, 32, 16, 2),
+    ([400], 150, 8, 4, 64, 64, 1040, 1),
+    ([333, 900], 33, 8, 2, 256, 32, 16, 2),
+    ([2000], 65, 1, 1, 256, 128, 16, 5),
+]
+
+
+def _fp16_rows(x, group, boost):
+    """What the chunk kernel makes of rows: fp16(scale * code + low) from fp16 scale and low, all of them times ``boost``."""
+    code, scale, low = kv4.quantise_reference(x.cpu(), group)
+    s, w = ((t.double() * boost).half().double().repeat_interleave(group, -1) for t in (scale, low))
+    return (code.double() * s + w).half().double() / boost
+
+
+def _attention(q, keys, values, scale, causal):
+    """fp64 (out, lse, sum of p |v - out|, largest sum of |q| |k| scale)."""
+    B, S, Hq, D = q.shape
+    out, spread = torch.zeros(B, S, Hq, D, dtype=torch.float64), torch.zeros(B, S, Hq, D, dtype=torch.float64)
+    lse, terms = torch.full((B, S, Hq), -math.inf, dtype=torch.float64), 0.0
+    q = q.double().cpu()
+    for b in range(B):
+        L, H = keys[b].shape[:2]
+        for s in range(S):
+            n = max(0, min(L, L - S + s + 1)) if causal else L
+            if n == 0:
+                continue
+            for h in range(Hq):
+                k, v = keys[b][:n, h // (Hq // H)], values[b][:n, h // (Hq // H)]
+                x = k @ q[b, s, h] * scale
+                p = torch.softmax(x, 0)
+                out[b, s, h] = p @ v
+                spread[b, s, h] = p @ (v - out[b, s, h]).abs()
+                lse[b, s, h] = torch.logsumexp(x, 0)
+                terms = max(terms, float((k.abs() @ q[b, s, h].abs()).max()) * abs(scale))
+    return out, lse, spread, terms
+
+
+@pytest.mark.parametrize("lens,S,Hq,H,D,group,page,splits", CHUNKS)
+def test_many_columns_against_values_as_they_are_held(lens, S, Hq, H, D, group, page, splits, chunks):
+    """Against fp64 over K and V as the kernel holds them, so that their rounding is not part of the tolerance.
+
+    What is left: P is one fp16 number, and the sum that divides is of the same numbers: e_i <= 2^-11 moves the output by sum p_i e_i
+    (v_i - out).  A score is summed in fp32 over D / 32 <= 8 products of 32 terms: 2^-24 each of their absolute sum, 2^-21 together and
+    for two weights' difference twice, twice more for Q in log2 units and the exponential's argument: 2^-18 of the terms.  The sums over
+    tokens are in fp32: 64 tokens at a time, 2^-24 each, under 2^-18 of the largest V.  The smallest weights, 2^-25 off next to a largest
+    of 2^6 at least, are 2000 * 2^-31 < 2^-20 together."""
+    gen = _gen(sum(lens) + S)
+    cache, table, ks, vs = oracle.filled(gen, lens, H, D, group, page, torch.bfloat16, "cuda", room=max(lens) + 40)
+    q = oracle.rows(gen, len(lens), S, Hq, D, device="cuda")
+    keys, values = [_fp16_rows(x, group, 1.0) for x in ks], [_fp16_rows(x, group, 128.0) for x in vs]
+    v_max = max(float(x.abs().max()) for x in values if x.numel())
+    n = int32(lens, "cuda")
+    for causal in (True, False):
+        want, lse, spread, terms = _attention(q, keys, values, D ** -0.5, causal)
+        full = kv4.gqa_fwd_kv4(q, cache, n, table, kv_split=splits, causal=causal, return_lse=True).double().cpu()
+        out = kv4.gqa_fwd_kv4(q, cache, n, table, kv_split=splits, causal=causal).double().cpu()
+        tol = (2.0 ** -11 + 2.0 ** -18 * terms) * spread + (2.0 ** -18 + 2.0 ** -20) * v_max
+        off = (full[..., :D] - want).abs()
+        assert (off <= tol).all(), float((off / tol.clamp(min=1e-12)).max())
+        assert ((out - want).abs() <= tol + 2.0 ** -8 * (want.abs() + tol)).all()
+        fine = lse != -math.inf
+        assert torch.equal(full[..., D] == -math.inf, ~fine)
+        assert ((full[..., D] - lse)[fine].abs() <= 2.0 ** -11 + 2.0 ** -18 * terms + 2.0 ** -22 * lse[fine].abs() + 2.0 ** -20).all()

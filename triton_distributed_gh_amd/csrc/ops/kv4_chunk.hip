@@ -9,12 +9,19 @@
 //   S^T[token, column] = K . Q^T,   P = exp2(scale log2(e) s - m) in fp16,   O^T[channel, column] = V^T . P^T,
 // and the sums of P come out of one more product with ones, of the same rounded P that O is made of: what rounding does to a
 // weight cancels where that weight is nearly all of the sum.  Values rounded to fp16 are within 2^-11 of themselves, as near as
-// `kv4_read` brings them for fp16 caches and eight times as near as for bf16.  The reference m moves as in kv4_attn.hip.
+// `kv4_read` brings them for fp16 caches and eight times as near as for bf16 (but for small ones, see below).  The reference m moves as in kv4_attn.hip.
 //
-// fp16 does not reach as far as bf16: values of 2^15, sixteen tokens' groups of K or thirty-two's of V whose largest value is
-// under 2^-11 and not 0 (fp16's smallest numbers are 2^-25 off at most, 2^-14 of it from there on), a NaN in a scale and a page
-// that is none are for the other kernel.  Whoever meets one says so in `flags`, one int per workgroup, written by every launch;
-// the other kernel runs behind this one and takes just the flagged workgroups' columns.
+// fp16 does not reach as far as bf16.  Below 2^-14 its numbers are 2^-24 apart, and a value is then off by as much as 17 * 2^-25:
+// a code's 15 times what the scale lost, what low lost, and the result's own rounding.  Whose group is how large against that
+// is asked of every token by itself, as a row may see that token alone.
+//   V: an answer's own size counts.  V is held times 2^7, which puts the numbers of trained models in the middle of fp16's range;
+//      a group of less than 2^-16 and not 0 is flagged (at 2^-9 as it is held, 17 * 2^-25 are 2^-11.9 of it), one of 2^8 too.
+//   K: a score's absolute error counts, the sum of scale |q| times what K is off by.  While that sum is under 2^8 for every column of the
+//      workgroup (about 10 for queries of size 1), 17 * 2^-25 of it are less than 2^-12 of a nat whatever K's size.  Beyond it, groups of
+//      less than 2^-9 and not 0 are flagged; groups of 2^15 always.
+// (A group's size: 15 scale + |low|, one to three times its largest value.)  A NaN in a scale and a page that is none are flagged too.
+// `flags` has one int per workgroup, written by every launch; kv4_attn.hip runs behind this kernel and takes just the flagged
+// workgroups' columns.
 //
 // What bounds it: 1024 new tokens over 16384, 32 / 8 heads of 128 (266 GFLOP): 301 .. 312 us in all, 850 .. 880 TFLOP/s where a
 // large bf16 matrix product reaches 1203; the other kernel takes 511.  Of a SIMD's cycles its matrix unit has 37 %, vector
@@ -100,10 +107,12 @@ __global__ __launch_bounds__(NW * 64, 2) void kv4_chunk_kernel(ChunkArgs a, cons
   constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
   constexpr float NONE = -1e30f;        // the reference before the first token
   constexpr float AT = 6.f, MOST = 14.f;  // log2 of the largest P: where a new reference puts it, and where it may grow to
-  constexpr float FAR = 0x1p15f, NEAR = 0x1p-11f;
+  constexpr float FAR = 0x1p15f, NEAR = 0x1p-9f;        // sizes, as they are held, that are flagged from there on / below
+  constexpr float BOOST = 0x1p7f;       // V is held times that
+  constexpr float WIDE_Q = 0x1p8f;      // sums of scale |q| for which small K is looked for
   __shared__ __attribute__((aligned(16))) u32x4 s_k[2][4][KS][64];
   __shared__ __attribute__((aligned(16))) u32x4 s_v[2][2][NT][64];
-  __shared__ int s_bad;
+  __shared__ int s_bad, s_wide;
 
   const int kvh = blockIdx.x, split = blockIdx.y;
   const int z = a.first + (int)blockIdx.z;
@@ -121,7 +130,8 @@ __global__ __launch_bounds__(NW * 64, 2) void kv4_chunk_kernel(ChunkArgs a, cons
   const int start = (int)min((long long)split * per, (long long)len), end = min(len, start + per);
   const int plain_end = min(end, a.causal ? L - a.S + block0 / group + 1 : L);
   const int most = col0 >= columns ? 0 : min(end, a.causal ? L - a.S + min(col0 + 16 * CB - 1, columns - 1) / group + 1 : L);
-  if (threadIdx.x == 0) s_bad = 0;
+  if (threadIdx.x == 0) s_bad = s_wide = 0;
+  bool wide_q = false;
 
   // Q in fp16: bf16 rows are brought near 2^8 by a power of two per column, which loses nothing that a score could show
   // (numbers 2^-32 of the column's largest).  A negative scale turns Q's sign, so that larger scores are larger weights.
@@ -140,6 +150,14 @@ __global__ __launch_bounds__(NW * 64, 2) void kv4_chunk_kernel(ChunkArgs a, cons
       q[cb][s] = u32x4{0, 0, 0, 0};
       if (col_ok) q[cb][s] = *(const u32x4*)(qp + 32 * s);
     }
+    float all = 0.f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) all += fabsf(from16<IS_BF16>(q[cb][s][i] & 0xffffu)) + fabsf(low_of<IS_BF16>(q[cb][s][i]));
+    all += __shfl_xor(all, 16);
+    all += __shfl_xor(all, 32);
+    wide_q |= !(all * fabsf(a.scale) < WIDE_Q);
     float mul = a.scale < 0.f ? -1.f : 1.f, back = 1.f;
     if (IS_BF16) {
       float top = 0.f;
@@ -249,6 +267,7 @@ __global__ __launch_bounds__(NW * 64, 2) void kv4_chunk_kernel(ChunkArgs a, cons
     }
   };
   const Unpack u;
+  float near_k = 0.f;                   // K below this and not 0 is flagged
   auto unpack = [&](int buf, int n0, Raw& r) INLINE {
     if (n0 + TOK > end) {               // tokens behind the end: zeros, whatever the page holds there
       const bool live = n0 + 16 * k_tile + li < end;
@@ -269,8 +288,7 @@ __global__ __launch_bounds__(NW * 64, 2) void kv4_chunk_kernel(ChunkArgs a, cons
     for (int g = 0; g < KG; ++g) {
       const float s = scale_of<IS_BF16>(r.kp[g]), l = low_of<IS_BF16>(r.kp[g]);
       const float size = __builtin_fmaf(15.f, s, fabsf(l));
-      const bool far = !(size < FAR), near = !__any(size >= NEAR) & size > 0.f;
-      bad |= far | near;
+      bad |= !(size < FAR) | (size < near_k & size > 0.f);
       scale[g] = both(s, s), low[g] = both(l, l);
     }
 #pragma unroll
@@ -287,23 +305,18 @@ __global__ __launch_bounds__(NW * 64, 2) void kv4_chunk_kernel(ChunkArgs a, cons
         f16x2 sv[VG][4], lv[VG][4];     // of tokens 4 lg + 2 (k & 1), + 1 of tile k >> 1
 #pragma unroll
         for (int g = 0; g < VG; ++g) {
-          float top = 0.f;
-          bool fine = true;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             float s[2], l[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               const uint32_t p = r.vp[n][k >> 1][g][2 * (k & 1) + i];
-              s[i] = scale_of<IS_BF16>(p), l[i] = low_of<IS_BF16>(p);
+              s[i] = scale_of<IS_BF16>(p) * BOOST, l[i] = low_of<IS_BF16>(p) * BOOST;
               const float size = __builtin_fmaf(15.f, s[i], fabsf(l[i]));
-              fine &= size < FAR;
-              top = fmaxf(top, size);
+              bad |= !(size < FAR) | (size < NEAR & size > 0.f);
             }
             sv[g][k] = both(s[0], s[1]), lv[g][k] = both(l[0], l[1]);
           }
-          const bool near = !__any(top >= NEAR) & top > 0.f;
-          bad |= !fine | near;
         }
         const u32x2 v0 = r.v[n][0], v1 = r.v[n][1];
         uint32_t w[4] = {v0[0], v0[1], v1[0], v1[1]};
@@ -406,7 +419,10 @@ __global__ __launch_bounds__(NW * 64, 2) void kv4_chunk_kernel(ChunkArgs a, cons
   if (start < end) {
     Raw raw;
     load(lookup(start), raw);
-    __syncthreads();                    // (s_bad)
+    __syncthreads();                    // (s_bad, s_wide are 0)
+    if (__any(wide_q) && lane == 0) s_wide = 1;
+    __syncthreads();
+    near_k = s_wide ? NEAR : 0.f;
     unpack(0, start, raw);
     load(lookup(start + TOK), raw);     // (behind the last block: its last tile's page once more)
     Spots next = lookup(start + 2 * TOK);
@@ -444,7 +460,7 @@ __global__ __launch_bounds__(NW * 64, 2) void kv4_chunk_kernel(ChunkArgs a, cons
     const int col = col0 + cb * 16 + li, row_s = col / group;
     if (col >= columns) continue;
     const long long at = ((long long)b * a.S + row_s) * a.q_heads + kvh * group + col - row_s * group;
-    const float sum = l[cb][0], inv = sum != 0.f ? 1.f / sum : 0.f;
+    const float sum = l[cb][0], inv = sum != 0.f ? 1.f / BOOST / sum : 0.f;
     const float lse = sum != 0.f ? m[cb] + __builtin_amdgcn_logf(sum) : -INFINITY;
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
