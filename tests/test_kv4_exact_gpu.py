@@ -233,3 +233,31 @@ def test_many_columns_against_values_as_they_are_held(lens, S, Hq, H, D, group, 
         fine = lse != -math.inf
         assert torch.equal(full[..., D] == -math.inf, ~fine)
         assert ((full[..., D] - lse)[fine].abs() <= 2.0 ** -11 + 2.0 ** -18 * terms + 2.0 ** -22 * lse[fine].abs() + 2.0 ** -20).all()
+
+
+@pytest.mark.parametrize("D,group", [(64, 32), (128, 64), (256, 128)])
+def test_many_columns_of_a_fp16_cache_are_as_exact_as_few(D, group):
+    """A row that sees one token is its V; a prompt's rows are those of the same call in pieces of few columns.  At a size that is many
+    columns' for bf16: a fp16 result has steps of 2^-11, and what is held in one fp16 number on the way would show.
+
+    Row 0: P times scale is two fp16 numbers (2^-22 of 15 scale), P times low and the sums are fp32: under 2^-19 of 3 max |v|."""
+    gen = _gen(D)
+    S, H, Hq, page = 1536 if D == 256 else 2560, 2, 16, 64
+    assert kv4.takes_chunks(1, H, S * Hq // H, D, S)
+    table, pages = oracle.table_for(1, S, page, gen, device="cuda")
+    cache = kv4.Int4KVCache.alloc(pages, page, H, D, group=group, dtype=torch.float16, device="cuda")
+    k, v = (oracle.rows(gen, 1, S, H, D, dtype=torch.float16, device="cuda") for _ in range(2))
+    kv4.kv4_append(k, v, cache, int32([0], "cuda"), table)
+    q = oracle.rows(gen, 1, S, Hq, D, dtype=torch.float16, device="cuda")
+    got = kv4.gqa_fwd_kv4(q, cache, int32([S], "cuda"), table, return_lse=True)
+    torch.cuda.synchronize()
+    held = oracle.held(v[0, 0], group).repeat_interleave(Hq // H, 0)
+    top = held.abs().unflatten(-1, (-1, group)).amax(-1).repeat_interleave(group, -1)
+    assert ((got[0, 0, :, :D].double().cpu() - held).abs() <= 2.0 ** -17 * top).all()
+    # the same rows, few columns at a time: the same arithmetic but for the splits, whose weights are fp32 (2^-20 at most)
+    for s in (1, 63, 700, S - 1):
+        few = kv4.gqa_fwd_kv4(q[:, s:s + 1], cache, int32([s + 1], "cuda"), table, return_lse=True, kv_split=1)
+        torch.cuda.synchronize()
+        off = (got[0, s].double() - few[0, 0].double()).abs().cpu()
+        assert (off[:, :D] <= 2.0 ** -13 * float(v.abs().max())).all(), float(off[:, :D].max())
+        assert (off[:, D] <= 5e-4).all()

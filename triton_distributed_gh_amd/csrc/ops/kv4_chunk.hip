@@ -8,8 +8,13 @@
 // in the order in which 16x16x32 MFMAs take them, so that a wave then reads its operands as straight 16-byte runs:
 //   S^T[token, column] = K . Q^T,   P = exp2(scale log2(e) s - m) in fp16,   O^T[channel, column] = V^T . P^T,
 // and the sums of P come out of one more product with ones, of the same rounded P that O is made of: what rounding does to a
-// weight cancels where that weight is nearly all of the sum.  Values rounded to fp16 are within 2^-11 of themselves, as near as
-// `kv4_read` brings them for fp16 caches and eight times as near as for bf16 (but for small ones, see below).  The reference m moves as in kv4_attn.hip.
+// weight cancels where that weight is nearly all of the sum.  The reference m moves as in kv4_attn.hip.
+//
+// For bf16 caches: values rounded to fp16 are within 2^-11 of themselves (but for small ones, see below) and a weight within 2^-11,
+// where the result is rounded to 2^-8; 1024 tokens over 16384 are 1.9e-3 off at most with it and with the plain form in 32 bits
+// (relative to a row's norm).  A fp16 result has steps of 2^-11 itself, and these roundings would be most of its error: 5.8e-4
+// for 2.7e-4, three times the scores 1.6e-3 for 2.4e-4, where kv4_attn.hip comes to 2.8e-4 and 2.5e-4.  So fp16 caches stay there, which costs
+// them 740 us where this kernel took 351.
 //
 // fp16 does not reach as far as bf16.  Below 2^-14 its numbers are 2^-24 apart, and a value is then off by as much as 17 * 2^-25:
 // a code's 15 times what the scale lost, what low lost, and the result's own rounding.  Whose group is how large against that
@@ -91,7 +96,7 @@ constexpr int column_blocks() { return D <= 128 ? 2 : 1; }          // of sixtee
 template <int D, int NW>
 constexpr int columns_of() { return 16 * column_blocks<D>() * NW; }
 
-template <bool IS_BF16, int D, int G, int NW>
+template <int D, int G, int NW>
 __global__ __launch_bounds__(NW * 64, 2) void kv4_chunk_kernel(ChunkArgs a, const int* __restrict__ block_table,
                                                                const int* __restrict__ kv_len) {
   constexpr int CB = column_blocks<D>(), COLUMNS = columns_of<D, NW>();
@@ -133,7 +138,7 @@ __global__ __launch_bounds__(NW * 64, 2) void kv4_chunk_kernel(ChunkArgs a, cons
   if (threadIdx.x == 0) s_bad = s_wide = 0;
   bool wide_q = false;
 
-  // Q in fp16: bf16 rows are brought near 2^8 by a power of two per column, which loses nothing that a score could show
+  // Q in fp16: rows are brought near 2^8 by a power of two per column, which loses nothing that a score could show
   // (numbers 2^-32 of the column's largest).  A negative scale turns Q's sign, so that larger scores are larger weights.
   int limit[CB];
   u32x4 q[CB][KS];
@@ -154,32 +159,30 @@ __global__ __launch_bounds__(NW * 64, 2) void kv4_chunk_kernel(ChunkArgs a, cons
 #pragma unroll
     for (int s = 0; s < KS; ++s)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) all += fabsf(from16<IS_BF16>(q[cb][s][i] & 0xffffu)) + fabsf(low_of<IS_BF16>(q[cb][s][i]));
+      for (int i = 0; i < 4; ++i) all += fabsf(from16<true>(q[cb][s][i] & 0xffffu)) + fabsf(low_of<true>(q[cb][s][i]));
     all += __shfl_xor(all, 16);
     all += __shfl_xor(all, 32);
     wide_q |= !(all * fabsf(a.scale) < WIDE_Q);
-    float mul = a.scale < 0.f ? -1.f : 1.f, back = 1.f;
-    if (IS_BF16) {
-      float top = 0.f;
+    float mul = a.scale < 0.f ? -1.f : 1.f;
+    float top = 0.f;
 #pragma unroll
-      for (int s = 0; s < KS; ++s)
+    for (int s = 0; s < KS; ++s)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          top = fmaxf(top, fmaxf(fabsf(from16<IS_BF16>(q[cb][s][i] & 0xffffu)), fabsf(low_of<IS_BF16>(q[cb][s][i]))));
-      top = fmaxf(top, __shfl_xor(top, 16));
-      top = fmaxf(top, __shfl_xor(top, 32));
-      int e = (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127;         // top in [2^e, 2^(e+1))
-      e = e < -100 ? -100 : e > 100 ? 100 : e;
-      mul *= __builtin_bit_cast(float, (uint32_t)(127 + 8 - e) << 23);
-      back = __builtin_bit_cast(float, (uint32_t)(127 - 8 + e) << 23);
-    }
+      for (int i = 0; i < 4; ++i)
+        top = fmaxf(top, fmaxf(fabsf(from16<true>(q[cb][s][i] & 0xffffu)), fabsf(low_of<true>(q[cb][s][i]))));
+    top = fmaxf(top, __shfl_xor(top, 16));
+    top = fmaxf(top, __shfl_xor(top, 32));
+    int e = (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127;           // top in [2^e, 2^(e+1))
+    e = e < -100 ? -100 : e > 100 ? 100 : e;
+    mul *= __builtin_bit_cast(float, (uint32_t)(127 + 8 - e) << 23);
+    const float back = __builtin_bit_cast(float, (uint32_t)(127 - 8 + e) << 23);
     qk[cb] = fminf(fmaxf(fabsf(a.scale * LOG2E) * back, 1e-37f), 1e37f);    // (a masked score is -inf: it stays that)
 #pragma unroll
     for (int s = 0; s < KS; ++s)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        q[cb][s][i] = __builtin_bit_cast(uint32_t, both(from16<IS_BF16>(q[cb][s][i] & 0xffffu) * mul,
-                                                        low_of<IS_BF16>(q[cb][s][i]) * mul));
+        q[cb][s][i] = __builtin_bit_cast(uint32_t, both(from16<true>(q[cb][s][i] & 0xffffu) * mul,
+                                                        low_of<true>(q[cb][s][i]) * mul));
   }
 
   // ---- the codes of 64 tokens on their way: where they are, and what this wave fetches of them
@@ -286,7 +289,7 @@ __global__ __launch_bounds__(NW * 64, 2) void kv4_chunk_kernel(ChunkArgs a, cons
     f16x2 scale[KG], low[KG];
 #pragma unroll
     for (int g = 0; g < KG; ++g) {
-      const float s = scale_of<IS_BF16>(r.kp[g]), l = low_of<IS_BF16>(r.kp[g]);
+      const float s = scale_of<true>(r.kp[g]), l = low_of<true>(r.kp[g]);
       const float size = __builtin_fmaf(15.f, s, fabsf(l));
       bad |= !(size < FAR) | (size < near_k & size > 0.f);
       scale[g] = both(s, s), low[g] = both(l, l);
@@ -311,7 +314,7 @@ __global__ __launch_bounds__(NW * 64, 2) void kv4_chunk_kernel(ChunkArgs a, cons
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               const uint32_t p = r.vp[n][k >> 1][g][2 * (k & 1) + i];
-              s[i] = scale_of<IS_BF16>(p) * BOOST, l[i] = low_of<IS_BF16>(p) * BOOST;
+              s[i] = scale_of<true>(p) * BOOST, l[i] = low_of<true>(p) * BOOST;
               const float size = __builtin_fmaf(15.f, s[i], fabsf(l[i]));
               bad |= !(size < FAR) | (size < NEAR & size > 0.f);
             }
@@ -473,7 +476,7 @@ __global__ __launch_bounds__(NW * 64, 2) void kv4_chunk_kernel(ChunkArgs a, cons
         for (int i = 0; i < 4; ++i) ((float*)a.out)[at * (D + 1) + ch + i] = r[i];
       } else {
         *(u32x2*)((uint16_t*)a.out + at * D + ch) =
-            u32x2{to16<IS_BF16>(r[0]) | to16<IS_BF16>(r[1]) << 16, to16<IS_BF16>(r[2]) | to16<IS_BF16>(r[3]) << 16};
+            u32x2{to16<true>(r[0]) | to16<true>(r[1]) << 16, to16<true>(r[2]) | to16<true>(r[3]) << 16};
       }
     }
     if (lg == 0) {
@@ -484,9 +487,9 @@ __global__ __launch_bounds__(NW * 64, 2) void kv4_chunk_kernel(ChunkArgs a, cons
 }
 
 template <class Fn>
-bool dispatch(int dtype, int D, int G, Fn&& fn) {
+bool dispatch(int D, int G, Fn&& fn) {
   auto typed = [&](auto d, auto g) {
-    if (dtype == 0) fn(std::true_type{}, d, g); else fn(std::false_type{}, d, g);
+    fn(d, g);
     return true;
   };
 #define TDIST_KV4_CASE(DD, GG) \
@@ -500,7 +503,7 @@ bool dispatch(int dtype, int D, int G, Fn&& fn) {
 
 }  // namespace
 
-// The same arguments as tdist_kv4_attn, without a cap.  flags: one int for every (block of columns, sequence, split, KV head),
+// The same arguments as tdist_kv4_attn, for a bf16 cache and without a cap.  flags: one int for every (block of columns, sequence, split, KV head),
 // `flag_columns` columns to a block; tdist_kv4_attn with them, on the same stream, then does what is flagged and the merge.
 TDIST_API int tdist_kv4_chunk(const void* k_codes, const void* v_codes, const void* k_params, const void* v_params, int pages,
                               int kv_heads, int page_size, int head_dim, int group, const void* q, long long q_sb, long long q_ss,
@@ -515,7 +518,7 @@ TDIST_API int tdist_kv4_chunk(const void* k_codes, const void* v_codes, const vo
   TDIST_REQUIRE(batch >= 0 && S >= 0 && q_heads > 0 && q_heads % kv_heads == 0 && max_pages >= 0 &&
                     (long long)max_pages * page_size <= (1ll << 30), "bad head counts, or more than 2^30 tokens in a row of the table");
   TDIST_REQUIRE(splits >= 1 && splits <= 65535 && (splits == 1 || partial), "splits need their partial rows");
-  TDIST_REQUIRE((out_mode == 1 || out_mode == 2) && (dtype == 0 || dtype == 1), "out_mode must be 1 or 2, dtype 0 (bf16) or 1 (fp16)");
+  TDIST_REQUIRE((out_mode == 1 || out_mode == 2) && dtype == 0, "out_mode must be 1 or 2, dtype 0 (bf16)");
   if (batch == 0 || S == 0) return 0;
   TDIST_REQUIRE(q && (table || max_pages == 0) && kv_len && out && flags, "null argument");
   TDIST_REQUIRE(((uintptr_t)q & 15) == 0 && ((uintptr_t)out & 7) == 0 && ((q_sb | q_ss | q_sh) & 7) == 0,
@@ -530,14 +533,14 @@ TDIST_API int tdist_kv4_chunk(const void* k_codes, const void* v_codes, const vo
   a.batch = batch, a.S = S, a.q_heads = q_heads, a.group = q_heads / kv_heads, a.splits = splits, a.causal = causal, a.out_mode = out_mode;
   a.scale = scale;
   bool same = true;
-  const bool ok = dispatch(dtype, head_dim, group, [&](auto bf, auto d, auto g) {
+  const bool ok = dispatch(head_dim, group, [&](auto d, auto g) {
     constexpr int D = decltype(d)::value, NW = WAVES;
     constexpr int per_group = columns_of<D, NW>();
     same = flag_columns == per_group;
     if (!same) return;
     const long long blocks = (columns + per_group - 1) / per_group * batch;
     for (a.first = 0; a.first < blocks; a.first += 65535)       // (the limit of a grid's third dimension)
-      hipLaunchKernelGGL((kv4_chunk_kernel<decltype(bf)::value, D, decltype(g)::value, NW>),
+      hipLaunchKernelGGL((kv4_chunk_kernel<D, decltype(g)::value, NW>),
                          dim3(kv_heads, splits, (unsigned)std::min(65535ll, blocks - a.first)), dim3(NW * 64), 0, (hipStream_t)stream,
                          a, table, kv_len);
   });

@@ -422,8 +422,8 @@ def attend_reference(q, cache: Int4KVCache, kv_lens, block_table, scale, soft_ca
 
 
 def takes_chunks(batch: int, kv_heads: int, columns: int, head_dim: int, capacity: int, soft_cap: float = 0.0) -> bool:
-    """Whether a launch goes to csrc/ops/kv4_chunk.hip, which unpacks for many columns at once, and only what that leaves to
-    csrc/ops/kv4_attn.hip.  Measured (four query heads to a KV head, microseconds there / here): one sequence of 16384, 8 heads of
+    """Whether a launch over a bf16 cache goes to csrc/ops/kv4_chunk.hip, which unpacks for many columns at once, and only what that
+    leaves to csrc/ops/kv4_attn.hip.  (fp16 caches stay with the latter: their results show the former's roundings.)  Measured (four query heads to a KV head, microseconds there / here): one sequence of 16384, 8 heads of
     128: 128 columns 40 / 34, 256 46 / 50, 1024 98 / 147; of 4096: 512 columns 43 / 35, 1024 49 / 51, 2048 66 / 78; of 1024: 2048
     columns 39 / 27; 4 x 2048: 256 columns 38 / 36, 1024 65 / 84; 4 heads of 256: 2048: 512 columns 30 / 29, 1024 36 / 40."""
     work = batch * kv_heads * columns * capacity
@@ -480,7 +480,7 @@ def gqa_fwd_kv4(q: torch.Tensor, cache: Int4KVCache, kv_lens: torch.Tensor, bloc
     q4 = _rows(q4)
     columns = Hq // cache.kv_heads * S
     room = pages * cache.page_size
-    chunk = takes_chunks(batch, cache.kv_heads, columns, D, room, soft_cap)
+    chunk = cache.dtype is torch.bfloat16 and takes_chunks(batch, cache.kv_heads, columns, D, room, soft_cap)
     splits = int(kv_split) if kv_split > 0 else auto_kv_splits(batch, cache.kv_heads, columns, D, room, chunk=chunk)
     out = torch.empty((batch, S, Hq, D + 1), dtype=torch.float32, device=q.device) if return_lse else \
         torch.empty_like(q4, memory_format=torch.contiguous_format)
