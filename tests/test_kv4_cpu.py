@@ -396,3 +396,14 @@ def test_tables_whose_rows_are_2_to_the_31_entries_apart_are_refused():
             call()
     near = torch.empty_strided((2, 2), (2 ** 31 - 1, 1), dtype=torch.int32, device="meta")
     assert kv4._check_table(cache, 2, near) == 2
+
+
+@pytest.mark.parametrize("soft_cap", [1e-60, 1e-39, 2.0, 1e4, 1e7, 1e30, 3e38, 1e60])
+def test_caps_of_any_size(soft_cap):
+    gen = _gen(53)
+    lens, H, D, group, page = [70, 3], 2, 64, 32, 16
+    cache, table, ks, vs = oracle.filled(gen, lens, H, D, group, page)
+    q = oracle.rows(gen, 2, 2, 4, D)
+    got = kv4.gqa_fwd_kv4(q, cache, int32(lens), table, scale=0.1, soft_cap=soft_cap, return_lse=True).double()
+    want, lse = oracle.attention(q, [oracle.held(x, group) for x in ks], [oracle.held(x, group) for x in vs], 0.1, soft_cap)
+    assert (got[..., :D] - want).abs().max() < 1e-4 and (got[..., D] - lse).abs().max() < 1e-4

@@ -6,7 +6,7 @@ import torch
 
 import kv4_oracle as oracle
 from kv4_oracle import int32
-from test_kv4_gpu import _check
+from test_kv4_gpu import SHAPES, _check
 from triton_distributed_gh_amd.ops import kv4
 
 pytestmark = pytest.mark.gpu
@@ -54,6 +54,25 @@ def test_splits_without_any_token_are_an_empty_row():
     got = kv4.gqa_fwd_kv4(q, cache, int32([128 * 70], "cuda"), table, kv_split=70, return_lse=True)
     torch.cuda.synchronize()
     assert (got[..., :128] == 0).all() and (got[..., 128] == -math.inf).all()
+
+
+# ---- soft caps ------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("scale,soft_cap", [(0.1, 1e4), (-0.3, 1e7), (0.1, 1e30), (0.1, 3e38), (0.1, 1e60),
+                                            (0.2, 2.0), (0.1, 1e-39), (0.1, 1e-60)])
+@pytest.mark.parametrize("Hq,H,S,D,group", SHAPES)
+def test_caps_of_any_size(Hq, H, S, D, group, scale, soft_cap):
+    """A cap far above the scores changes nothing; one near them or below bends or flattens them."""
+    gen = _gen(42)
+    lens, page = [333, 40], 16
+    cache, table, ks, vs = oracle.filled(gen, lens, H, D, group, page, torch.bfloat16, "cuda")
+    q = oracle.rows(gen, 2, S, Hq, D, device="cuda")
+    keys, values = [oracle.held(x, group) for x in ks], [oracle.held(x, group) for x in vs]
+    want, lse = oracle.attention(q, keys, values, scale, soft_cap)
+    for splits in (1, 2):
+        got = kv4.gqa_fwd_kv4(q, cache, int32(lens, "cuda"), table, scale=scale, soft_cap=soft_cap, kv_split=splits, return_lse=True)
+        torch.cuda.synchronize()
+        _check(got[..., :D], want, got[..., D], lse, torch.float32, max(float(x.abs().max()) for x in values),
+               scores=max(1.0, abs(scale) * D ** 0.5))
 
 
 # ---- many columns ---------------------------------------------------------------------------------------------------

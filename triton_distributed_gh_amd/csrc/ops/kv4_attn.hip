@@ -46,7 +46,7 @@ struct AttnArgs {
   int first;                // of this launch's (column block, sequence) pairs
   const int* flags;         // where given: [blocks of flag_columns * batch, splits, kv_heads], 0: another kernel has done it
   int flag_columns;
-  float scale, soft_cap;
+  float scale, soft_cap, inv_cap;     // (inv_cap: 1 / soft_cap)
 };
 
 typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
@@ -115,6 +115,16 @@ __device__ __forceinline__ void load_words(uint32_t (&dst)[N], const uint8_t* ba
       for (int j = 0; j < 4; ++j) dst[4 * i + j] = v[j];
     }
   }
+}
+
+// cap tanh(score / cap).  tanh is 1 - 2 / (e^2x + 1), which is off by 2^-24 of 1 however small x is: times a large cap that would
+// be more than the scores themselves.  Up to x = 1 / 4 it is x (1 - x^2 / 3 + 2 x^4 / 15 - 17 x^6 / 315), the next term 62 x^8 / 2835 < 2^-21,
+// and with it the score times what stands in brackets, which is the score itself under a cap that is far above it.
+__device__ __forceinline__ float capped(float score, float cap, float inv_cap) {
+  const float x = score * inv_cap, x2 = x * x;
+  const float near = score * __builtin_fmaf(__builtin_fmaf(__builtin_fmaf(x2, -17.f / 315.f, 2.f / 15.f), x2, -1.f / 3.f), x2, 1.f);
+  const float far = cap * (1.f - 2.f * __builtin_amdgcn_rcpf(exp2_fast(2.f * 1.4426950408889634f * x) + 1.f));
+  return fabsf(x) < 0.25f ? near : far;
 }
 
 // The larger of an op's two sides over the sixteen lanes of a row; every lane gets it.
@@ -217,7 +227,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_kernel(AttnArgs a, const int*
   };
   auto prepare_q = [&]() INLINE {
     const float sign = a.scale < 0.f ? -1.f : 1.f;
-    const float lead = fabsf(a.soft_cap > 0.f ? a.scale / a.soft_cap : a.scale * LOG2E);
+    const float lead = fabsf(a.soft_cap > 0.f ? a.scale : a.scale * LOG2E);
 #pragma unroll
     for (int cb = 0; cb < CB; ++cb) {
       float mul = sign, back = 1.f;
@@ -428,10 +438,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_kernel(AttnArgs a, const int*
 #pragma unroll
       for (int cb = 0; cb < CB; ++cb)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {         // cap tanh(x) = cap (1 - 2 / (e^2x + 1)), in units of log2, over qk
-          const float e = exp2_fast(2.f * LOG2E * qk[cb] * sc[cb][i]);
-          sc[cb][i] = a.soft_cap * LOG2E * (1.f - 2.f * __builtin_amdgcn_rcpf(e + 1.f));
-        }
+        for (int i = 0; i < 8; ++i) sc[cb][i] = LOG2E * capped(qk[cb] * sc[cb][i], a.soft_cap, a.inv_cap);
     }
     float x_mul[CB];
     uint32_t seen[CB];
@@ -564,10 +571,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_kernel(AttnArgs a, const int*
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int i = 0; i < W; ++i) {         // as above
-          const float e = exp2_fast(2.f * LOG2E * qk[i] * sc[t][i]);
-          sc[t][i] = a.soft_cap * LOG2E * (1.f - 2.f * __builtin_amdgcn_rcpf(e + 1.f));
-        }
+        for (int i = 0; i < W; ++i) sc[t][i] = LOG2E * capped(qk[i] * sc[t][i], a.soft_cap, a.inv_cap);
     }
     float x_mul[W];
     bool seen[2][W];
@@ -974,7 +978,7 @@ TDIST_API int tdist_kv4_attn(const void* k_codes, const void* v_codes, const voi
   a.partial_lse = partial ? partial + (long long)batch * S * q_heads * splits * head_dim : nullptr;
   a.q_sb = q_sb, a.q_ss = q_ss, a.q_sh = q_sh, a.table_stride = table_stride, a.max_pages = max_pages;
   a.batch = batch, a.S = S, a.q_heads = q_heads, a.group = q_heads / kv_heads, a.splits = splits, a.causal = causal, a.out_mode = out_mode;
-  a.scale = scale, a.soft_cap = soft_cap, a.flags = flags, a.flag_columns = flag_columns;
+  a.scale = scale, a.soft_cap = soft_cap, a.inv_cap = std::min(1.f / soft_cap, 1e38f), a.flags = flags, a.flag_columns = flag_columns;
   const bool ok = dispatch(dtype, head_dim, group, [&](auto bf, auto d, auto g) {
     auto launch = [&](auto kernel) {
       for (a.first = 0; a.first < blocks; a.first += 65535)       // (the limit of a grid's third dimension)

@@ -471,6 +471,8 @@ def gqa_fwd_kv4(q: torch.Tensor, cache: Int4KVCache, kv_lens: torch.Tensor, bloc
     scale = D ** -0.5 if scale is None else float(scale)
     if not (math.isfinite(scale) and math.isfinite(soft_cap) and soft_cap >= 0):
         raise ValueError(f"scale must be finite, soft_cap 0 (off) or positive, got {scale} and {soft_cap}")
+    if soft_cap:
+        soft_cap = min(max(soft_cap, 2.0 ** -126), 2.0 ** 127)       # (ordinary fp32 numbers: 0 would be off)
     if not (kv_split == -1 or 1 <= kv_split <= 65535):
         raise ValueError(f"kv_split must be -1 (automatic) or 1 .. 65535, got {kv_split}")
     if not q.is_cuda:
