@@ -407,3 +407,31 @@ def test_caps_of_any_size(soft_cap):
     got = kv4.gqa_fwd_kv4(q, cache, int32(lens), table, scale=0.1, soft_cap=soft_cap, return_lse=True).double()
     want, lse = oracle.attention(q, [oracle.held(x, group) for x in ks], [oracle.held(x, group) for x in vs], 0.1, soft_cap)
     assert (got[..., :D] - want).abs().max() < 1e-4 and (got[..., D] - lse).abs().max() < 1e-4
+
+
+def test_lds_writes_and_reads_of_other_lanes_keep_their_order(tmp_path):
+    """Each lane writes its neighbour's word and reads its own: never the same address in one lane, so that the compiler may issue the
+    read first (and it does), unless it is told that the lanes meet there."""
+    import subprocess
+
+    from triton_distributed_gh_amd import build
+
+    source = tmp_path / "probe.hip"
+    source.write_text("""#include "tdist/kv4.hpp"
+template <bool MEET>
+__global__ void probe(float* out, const float* in) {
+  __shared__ float s[65];
+  s[threadIdx.x + 1] = in[threadIdx.x];
+  if (MEET) tdist::kv4::lanes_meet();
+  out[threadIdx.x] = s[threadIdx.x];
+}
+template __global__ void probe<true>(float*, const float*);
+""")
+    asm = subprocess.run([build._hipcc(), *build.HIPCC_FLAGS, "-S", "--cuda-device-only", "-o", "-", str(source)], check=True,
+                         capture_output=True, text=True).stdout
+    order = [line.split()[0] for line in asm.splitlines() if line.strip().startswith(("ds_write", "ds_read"))]
+    assert order == ["ds_write_b32", "ds_read_b32"]
+    # the places where the kernels hand data from lane to lane of one wave: a tile of V that is written, rows of V that are read
+    # back, a block's parameters and weights
+    for name, least in (("kv4.hip", 4), ("kv4_attn.hip", 3)):
+        assert (build.CSRC / "ops" / name).read_text().count("lanes_meet();") >= least

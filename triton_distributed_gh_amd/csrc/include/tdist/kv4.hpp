@@ -70,5 +70,15 @@ __device__ __forceinline__ Place place_of(const Cache& c, const int* table_row, 
   return Place{page >= 0 && page < c.pages ? page : -1, (int)((uint32_t)pos - i * (uint32_t)c.page_size)};
 }
 
+// Between one lane's writes to LDS and another lane's reads of them, and between those and the next writes to the same place, in one
+// wave.  A wave's LDS accesses are carried out in the order in which they are issued, so there is nothing to wait for and this is no
+// instruction; what it does is to keep the compiler from issuing them in another order, which it may where it can tell that no lane
+// meets its own address again.
+__device__ __forceinline__ void lanes_meet() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+}
+
 }  // namespace kv4
 }  // namespace tdist

@@ -202,7 +202,11 @@ __device__ __forceinline__ void store_tile(const Cache& c, const Place& at, int 
         write(std::true_type{}, p, param, code);
       }
     }
-    if (IS_V && lane * 16 < T::TILE * (D / 2)) *(u32x4*)(vbase + lane * 16) = *(const u32x4*)(stage + lane * 16);
+    if constexpr (IS_V) {
+      lanes_meet();
+      if (lane * 16 < T::TILE * (D / 2)) *(u32x4*)(vbase + lane * 16) = *(const u32x4*)(stage + lane * 16);
+      lanes_meet();                     // (the next head's tile)
+    }
   } else {
 #pragma unroll
     for (int p = 0; p < T::PASSES; ++p) {
@@ -513,6 +517,7 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(Cache c, const int* __res
             }
           }
         }
+        lanes_meet();
       }
       uint32_t word[T::PASSES], param[T::PASSES];
 #pragma unroll
@@ -555,6 +560,7 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(Cache c, const int* __res
         }
         if (i < n) *(u32x4*)(out + (r + i) * st) = pack_row8<IS_BF16>(x);
       }
+      lanes_meet();                     // (the next sequence's rows)
       r += n;
     }
   }

@@ -636,6 +636,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_kernel(AttnArgs a, const int*
           if constexpr (!IS_BF16) ps[g][1][lg * W + i][put + 4 * t] = __builtin_bit_cast(uint16_t, (_Float16)(s1 - (float)h));
         }
       }
+    lanes_meet();
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       u32x4 hi[CB], lo[CB];
@@ -660,11 +661,13 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_kernel(AttnArgs a, const int*
 #pragma unroll
       for (int g = 0; g < NG; ++g) param[g] = live ? param[g] : 0u;
     }
+    lanes_meet();                       // (the block before)
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       params[lane >> 5][g][lane & 31] = param[g];
       widest = fmaxf(widest, CAREFUL ? scale_of<IS_BF16>(param[g]) * vs[g] : scale_of<IS_BF16>(param[g]));
     }
+    lanes_meet();
     widest = max_upper_half(widest);
     if constexpr (R > 0) {
       return by_tokens(careful, n0, there0, there1, r, param, widest, after_k);
