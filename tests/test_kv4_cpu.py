@@ -435,3 +435,27 @@ template __global__ void probe<true>(float*, const float*);
     # back, a block's parameters and weights
     for name, least in (("kv4.hip", 4), ("kv4_attn.hip", 3)):
         assert (build.CSRC / "ops" / name).read_text().count("lanes_meet();") >= least
+
+
+@pytest.mark.parametrize("which", ["k_codes", "v_codes", "k_params", "v_params"])
+@pytest.mark.parametrize("change", [
+    lambda t: t.set_(t.clone()),
+    lambda t: t.resize_(4 * t.shape[0], *t.shape[1:]),
+    lambda t: setattr(t, "data", t.clone()),
+    lambda t: t.untyped_storage().resize_(0),
+])
+def test_a_cache_whose_tensors_got_other_memory_is_refused(which, change):
+    """The kernels go by the addresses that the cache was made with: what is there may have been freed."""
+    gen = _gen(54)
+    cache, table, _, _ = oracle.filled(gen, [20], 2, 64, 32, 16)
+    rows, n = oracle.rows(gen, 1, 1, 2, 64), int32([20])
+    kv4.gqa_fwd_kv4(rows, cache, n, table)
+    keep = change(getattr(cache, which))
+    rope, pos = torch.ones(32, 32), torch.zeros(1, 1, dtype=torch.int64)
+    for call in (lambda: kv4.gqa_fwd_kv4(rows, cache, n, table), lambda: kv4.kv4_append(rows, rows, cache, n, table),
+                 lambda: kv4.kv4_read(cache, table, int32([0, 20]), 20),
+                 lambda: kv4.kv4_qkv_prep(torch.cat([rows] * 3, 2).flatten(2), None, None, 0.0, 0.0, pos, rope, rope, cache, n, int32([0]),
+                                          table, 2)):
+        with pytest.raises(RuntimeError, match="other memory"):
+            call()
+    del keep

@@ -81,7 +81,8 @@ class Int4KVCache:
 
     ``k_codes [pages, kv_heads, page_size, head_dim / 2]`` and ``v_codes [pages, kv_heads, page_size / 4, 2 * head_dim]`` uint8,
     ``k_params`` / ``v_params [pages, kv_heads, head_dim / group, page_size, 2]`` (scale, low) in ``dtype``.  Checked once, here:
-    the tensors keep their memory as long as the cache is used (their contents may change, by whatever means)."""
+    the tensors keep their memory as long as the cache is used (their contents may change, by whatever means); calls refuse a cache
+    whose tensors have been given other memory since (``set_``, ``resize_``, ``.data``)."""
 
     k_codes: torch.Tensor
     v_codes: torch.Tensor
@@ -106,9 +107,10 @@ class Int4KVCache:
         for t in (k, v, kp, vp):
             _require(t.device == k.device, "the four tensors of a cache live on one device")
             _require(t.is_contiguous() and t.data_ptr() % 16 == 0, "cache tensors must be contiguous and 16-byte aligned")
-        native = (k.data_ptr(), v.data_ptr(), kp.data_ptr(), vp.data_ptr(), P, H, S, D, G)
+        where = (k.data_ptr, v.data_ptr, kp.data_ptr, vp.data_ptr)
+        memory = tuple(ptr() for ptr in where)
         for name, value in dict(num_pages=P, kv_heads=H, page_size=S, head_dim=D, group=G, dtype=kp.dtype, device=k.device,
-                                _native=native).items():
+                                _where=where, _memory=memory, _native=(*memory, P, H, S, D, G)).items():
             object.__setattr__(self, name, value)
 
     def __reduce__(self):       # (copies and pickles are caches of their own tensors)
@@ -146,10 +148,14 @@ def _check_data(cache: Int4KVCache, **rows: torch.Tensor) -> None:
 
 
 def _check_table(cache: Int4KVCache, batch: int, table: torch.Tensor) -> int:
-    """The pages of a row of the table."""
-    if table.dim() == 2 and table.dtype is torch.int32 and table.size(0) == batch and table.device == cache.device:
-        pages = table.size(1)
-        if (pages <= 1 or table.stride(1) == 1) and pages * cache.page_size <= 2 ** 30 and table.stride(0) < 2 ** 31:
+    """The pages of a row of the table.  (Every call comes here: the cache's memory is looked at too.)"""
+    k, v, kp, vp = cache._where
+    if (k(), v(), kp(), vp()) != cache._memory:
+        raise RuntimeError("the tensors of this cache have been given other memory since it was made: make a new Int4KVCache of them")
+    shape, strides = table.shape, table.stride()
+    if len(shape) == 2 and table.dtype is torch.int32 and shape[0] == batch and table.device == cache.device:
+        pages = shape[1]
+        if (pages <= 1 or strides[1] == 1) and pages * cache.page_size <= 2 ** 30 and strides[0] < 2 ** 31:
             return pages
     raise ValueError(f"block_table must be int32 [{batch}, max_pages] with contiguous rows of at most 2^30 tokens, less than 2^31 entries "
                      f"apart, on {cache.device}")
