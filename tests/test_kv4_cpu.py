@@ -459,3 +459,39 @@ def test_a_cache_whose_tensors_got_other_memory_is_refused(which, change):
         with pytest.raises(RuntimeError, match="other memory"):
             call()
     del keep
+
+
+def _calls_with(change):
+    """The entry points with each of their floating-point inputs passed through ``change`` in turn."""
+    gen = _gen(55)
+    cache, table, _, _ = oracle.filled(gen, [20], 2, 64, 32, 16)
+    x, n, pos = oracle.rows(gen, 1, 1, 2, 64), int32([20]), torch.zeros(1, 1, dtype=torch.int64)
+    qkv, w, rope = torch.cat([x] * 3, 2).flatten(2), torch.ones(64).bfloat16(), torch.ones(32, 32)
+    prep = lambda *a: kv4.kv4_qkv_prep(a[0], a[1], a[2], 0.0, 0.0, pos, a[3], a[4], cache, n, int32([0]), table, 2)  # noqa: E731
+    out = torch.zeros(20, 2, 64, dtype=torch.bfloat16)
+    for call, args in ((lambda q: kv4.gqa_fwd_kv4(q, cache, n, table), [x]),
+                       (lambda q: kv4.flash_attn_with_kv4cache(q, cache, n, table), [x]),
+                       (lambda k, v: kv4.kv4_append(k, v, cache, n, table), [x, x.clone()]),
+                       (prep, [qkv, w, w.clone(), rope, rope.clone()]),
+                       (lambda k, v: kv4.kv4_read(cache, table, int32([0, 20]), 20, out=(k, v)), [out, out.clone()])):
+        call(*args)
+        for i in range(len(args)):
+            yield lambda: call(*args[:i], change(args[i]), *args[i + 1:])
+
+
+def test_inputs_that_carry_a_tangent_or_require_a_gradient_are_refused():
+    from torch.autograd import forward_ad
+
+    for call in _calls_with(lambda t: t.clone().requires_grad_()):
+        with pytest.raises(RuntimeError, match="gradient"):
+            call()
+    with forward_ad.dual_level():
+        for call in _calls_with(lambda t: forward_ad.make_dual(t, torch.ones_like(t))):
+            with pytest.raises(RuntimeError, match="tangent"):
+                call()
+    with torch.no_grad():
+        for call in _calls_with(lambda t: t.clone().requires_grad_()):
+            call()
+    cache = kv4.Int4KVCache.alloc(1, 16, 1, 64)
+    with pytest.raises(ValueError, match="gradient"):
+        kv4.Int4KVCache(cache.k_codes, cache.v_codes, cache.k_params.clone().requires_grad_(), cache.v_params)

@@ -19,7 +19,7 @@ GPU tensors run csrc/ops/kv4.hip and csrc/ops/kv4_attn.hip, CPU tensors a PyTorc
 parameters that either writes are the same bits.  Entries of a block table that are no page of the cache are tolerated
 everywhere: rows that would go there are dropped, tokens there read as zeros and are not attended.  Everything launches
 on the current stream of the tensors' device, allocates nothing that outlives the call but its results, and can be
-captured into a graph.  None of it has a gradient: it refuses inputs that ask for one.
+captured into a graph.  None of it has a gradient: it refuses inputs that ask for one, by a backward pass or a tangent.
 """
 from __future__ import annotations
 
@@ -29,6 +29,7 @@ import math
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib
 
@@ -105,6 +106,7 @@ class Int4KVCache:
         if kp.dtype not in (torch.bfloat16, torch.float16) or vp.dtype != kp.dtype:
             raise TypeError(f"a 4-bit cache stands for bf16 or fp16 rows, got {kp.dtype} / {vp.dtype}")
         for t in (k, v, kp, vp):
+            _require(not t.requires_grad, "a 4-bit cache has no gradient: its tensors cannot require one")
             _require(t.device == k.device, "the four tensors of a cache live on one device")
             _require(t.is_contiguous() and t.data_ptr() % 16 == 0, "cache tensors must be contiguous and 16-byte aligned")
         where = (k.data_ptr, v.data_ptr, kp.data_ptr, vp.data_ptr)
@@ -143,8 +145,15 @@ def _check_data(cache: Int4KVCache, **rows: torch.Tensor) -> None:
             raise TypeError(f"{name} must be {cache.dtype} like the cache, got {t.dtype}")
         if t.device != cache.device:
             raise ValueError(f"{name} is on {t.device}, the cache on {cache.device}")
-        if t.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError(f"a 4-bit cache has no gradient: {name} requires one (detach it, or run under torch.no_grad())")
+        if t.requires_grad or forward_ad._current_level >= 0:
+            _check_no_gradient(name, t)
+
+
+def _check_no_gradient(name: str, t: torch.Tensor) -> None:
+    if t.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"a 4-bit cache has no gradient: {name} requires one (detach it, or run under torch.no_grad())")
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise RuntimeError(f"a 4-bit cache has no gradient: {name} carries a tangent")
 
 
 def _check_table(cache: Int4KVCache, batch: int, table: torch.Tensor) -> int:
@@ -313,6 +322,9 @@ def kv4_qkv_prep(qkv: torch.Tensor, q_w: Optional[torch.Tensor], k_w: Optional[t
             and cos.shape == sin.shape and cos.is_contiguous() and sin.is_contiguous() and cos.device == cache.device
             and sin.device == cache.device):
         raise ValueError(f"cos / sin must be contiguous fp32 [positions, {D // 2}] on {cache.device}")
+    if cos.requires_grad or sin.requires_grad or forward_ad._current_level >= 0:
+        _check_no_gradient("cos", cos)
+        _check_no_gradient("sin", sin)
     pages = _check_table(cache, batch, block_table)
     _check_counts(cache, batch, "kv_offset", kv_offset)
     _check_counts(cache, batch, "total_out", total_out)
