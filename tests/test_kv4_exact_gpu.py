@@ -75,6 +75,51 @@ def test_caps_of_any_size(Hq, H, S, D, group, scale, soft_cap):
                scores=max(1.0, abs(scale) * D ** 0.5))
 
 
+# ---- queries of any size, and scores up to where they are whole numbers ------------------------------------------------
+@pytest.mark.parametrize("q_size,k_size", [(2.0 ** 120, 2.0 ** -120), (2.0 ** 102, 2.0 ** -102), (2.0 ** -110, 2.0 ** 110)])
+@pytest.mark.parametrize("Hq,H,S,D,group", [*SHAPES, (40, 1, 2, 128, 64), (40, 1, 3, 256, 64)])
+def test_large_queries_over_small_keys(Hq, H, S, D, group, q_size, k_size, monkeypatch):
+    """The same scores, from far larger queries and far smaller keys or the other way round."""
+    monkeypatch.setattr(kv4, "takes_chunks", lambda *a: a[2] > 64 and a[5] == 0)
+    gen = _gen(47)
+    L, page = 150, 16
+    cache, table, ks, vs = oracle.filled(gen, [L], H, D, group, page, torch.bfloat16, "cuda")
+    k = ks[0] * k_size
+    kv4.kv4_append(k[None], vs[0][None], cache, int32([0], "cuda"), table)
+    q = oracle.rows(gen, 1, S, Hq, D, device="cuda") * q_size
+    values = [oracle.held(vs[0], group)]
+    want, lse = oracle.attention(q, [oracle.held(k, group)], values, D ** -0.5)
+    got = kv4.gqa_fwd_kv4(q, cache, int32([L], "cuda"), table, return_lse=True)
+    torch.cuda.synchronize()
+    _check(got[..., :D], want, got[..., D], lse, torch.float32, float(values[0].abs().max()))
+
+
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("Hq,H,S,D,group", [*SHAPES, (40, 1, 2, 128, 64), (40, 1, 3, 256, 64)])
+def test_scores_up_to_2_to_the_27(Hq, H, S, D, group, sign, monkeypatch):
+    """All the weight is the best token's, and the LSE is its score."""
+    monkeypatch.setattr(kv4, "takes_chunks", lambda *a: a[2] > 64 and a[5] == 0)
+    gen = _gen(48)
+    L, page = 150, 16
+    cache, table, ks, vs = oracle.filled(gen, [L], H, D, group, page, torch.bfloat16, "cuda")
+    k = sign * ks[0].abs()
+    kv4.kv4_append(k[None], vs[0][None], cache, int32([0], "cuda"), table)
+    q = (oracle.rows(gen, 1, S, Hq, D, device="cuda").abs() * 2.0 ** 22).to(torch.bfloat16)
+    keys, values = oracle.held(k, group), oracle.held(vs[0], group)
+    scores = (q[0].double().cpu().unsqueeze(1) * keys.repeat_interleave(Hq // H, 1)).sum(-1).transpose(1, 2) * D ** -0.5
+    assert 2.0 ** 24 < scores.abs().max() < 2.0 ** 27
+    scores.masked_fill_(torch.arange(L) > L - S + torch.arange(S)[:, None, None], -math.inf)
+    top, at = scores.max(-1)
+    second = scores.scatter(-1, at.unsqueeze(-1), -math.inf).max(-1).values
+    # the larger of two scores is the larger in the kernel too where they differ by what keys rounded to 2^-11 leave
+    clear = top - second > 2.0 ** -10 * top.abs()
+    assert clear.any()
+    got = kv4.gqa_fwd_kv4(q, cache, int32([L], "cuda"), table, return_lse=True)[0].double().cpu()
+    want = values.repeat_interleave(Hq // H, 1)[at, torch.arange(Hq)]
+    assert ((got[..., :D] - want).abs() <= 2.0 ** -9 * values.abs().max())[clear].all()
+    assert ((got[..., D] - top).abs() <= 2.0 ** -10 * top.abs()).all()
+
+
 # ---- many columns ---------------------------------------------------------------------------------------------------
 @pytest.fixture
 def chunks(monkeypatch):

@@ -241,7 +241,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_kernel(AttnArgs a, const int*
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(top, __shfl_xor(top, 32));
         int e = (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127;       // top in [2^e, 2^(e+1))
-        e = e < -100 ? -100 : e > 100 ? 100 : e;
+        e = e < -100 ? -100 : e;
         mul = sign * __builtin_bit_cast(float, (uint32_t)(127 + 8 - e) << 23);
         back = __builtin_bit_cast(float, (uint32_t)(127 - 8 + e) << 23);
       }

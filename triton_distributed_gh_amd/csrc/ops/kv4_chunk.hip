@@ -173,7 +173,7 @@ __global__ __launch_bounds__(NW * 64, 2) void kv4_chunk_kernel(ChunkArgs a, cons
     top = fmaxf(top, __shfl_xor(top, 16));
     top = fmaxf(top, __shfl_xor(top, 32));
     int e = (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127;           // top in [2^e, 2^(e+1))
-    e = e < -100 ? -100 : e > 100 ? 100 : e;
+    e = e < -100 ? -100 : e;
     mul *= __builtin_bit_cast(float, (uint32_t)(127 + 8 - e) << 23);
     const float back = __builtin_bit_cast(float, (uint32_t)(127 - 8 + e) << 23);
     qk[cb] = fminf(fmaxf(fabsf(a.scale * LOG2E) * back, 1e-37f), 1e37f);    // (a masked score is -inf: it stays that)

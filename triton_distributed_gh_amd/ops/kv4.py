@@ -475,7 +475,8 @@ def gqa_fwd_kv4(q: torch.Tensor, cache: Int4KVCache, kv_lens: torch.Tensor, bloc
     """Attention of ``q [batch, S, Hq, D]`` (or ``[batch, Hq, D]`` for S = 1), the last S tokens of each sequence.
 
     ``kv_lens`` int32 [batch]: cached tokens, the S new ones included; with ``causal`` query s sees the first
-    ``kv_lens[b] - S + s + 1`` of them.  Rows that see nothing are zero.  Returns q's shape in q's type, or with ``return_lse``
+    ``kv_lens[b] - S + s + 1`` of them.  Rows that see nothing are zero.  Scores (``scale`` times q . k) may be up to 2^27 in size: in
+    fp32 they are 8 apart from there on, and a row's weights mean nothing.  Returns q's shape in q's type, or with ``return_lse``
     fp32 ``[.., D + 1]`` with the natural-log LSE last (-inf for an empty row), the form
     ``flash_decode.gqa_fwd_batch_decode_inter_rank_combine`` merges over ranks that hold parts of the sequences."""
     flat = q.dim() == 3
