@@ -325,3 +325,30 @@ def test_many_columns_of_a_fp16_cache_are_as_exact_as_few(D, group):
         off = (got[0, s].double() - few[0, 0].double()).abs().cpu()
         assert (off[:, :D] <= 2.0 ** -13 * float(v.abs().max())).all(), float(off[:, :D].max())
         assert (off[:, D] <= 5e-4).all()
+
+
+# ---- more sequences than a grid's dimension holds -----------------------------------------------------------------------
+def test_more_sequences_than_a_grid_dimension_holds():
+    gen = _gen(61)
+    B, H, Hq, D, group, page = 65536 + 70, 1, 1, 64, 64, 16
+    cpu = kv4.Int4KVCache.alloc(B + 1, page, H, D, group=group)
+    gpu = kv4.Int4KVCache.alloc(B + 1, page, H, D, group=group, device="cuda")
+    table = torch.randperm(B + 1, generator=gen)[:B].view(B, 1).int()
+    x = oracle.rows(gen, B, 1, 3 * D)
+    k, v = x[..., :D].view(B, 1, 1, D), x[..., D:2 * D].view(B, 1, 1, D)
+    offset, news = torch.randint(0, 15, (B,), generator=gen).int(), torch.randint(0, 2, (B,), generator=gen).int()
+    kv4.kv4_append(k, v, cpu, offset, table, new_lens=news)
+    kv4.kv4_append(k.cuda(), v.cuda(), gpu, offset.cuda(), table.cuda(), new_lens=news.cuda())
+    torch.cuda.synchronize()
+    same = lambda: all(torch.equal(getattr(cpu, n), getattr(gpu, n).cpu()) for n in ("k_codes", "v_codes", "k_params", "v_params"))  # noqa: E731
+    assert same()
+    rope, pos, w = torch.ones(16, D // 2), offset.long().view(B, 1), torch.ones(D).bfloat16()
+    outs = []
+    for c, dev in ((cpu, "cpu"), (gpu, "cuda")):
+        total = torch.zeros(B, dtype=torch.int32, device=dev)
+        q = kv4.kv4_qkv_prep(x.to(dev), w.to(dev), None, 1e-6, 1e-6, pos.to(dev), rope.to(dev), rope.to(dev), c, offset.to(dev), total,
+                             table.to(dev), Hq)
+        outs.append((q.cpu(), total.cpu()))
+    assert same() and torch.equal(outs[0][1], outs[1][1])
+    # (Q's norm is in 32 bits on the GPU and in 64 here: a step of its rounding, and one of the result's, for values under 8)
+    assert (outs[0][0] == outs[1][0]).float().mean() > 0.999 and ((outs[0][0] - outs[1][0]).abs() <= 2.0 ** -6 * 8).all()

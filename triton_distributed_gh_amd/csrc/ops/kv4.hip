@@ -591,9 +591,14 @@ bool cache_ok(const Cache& c) {
 // tiles that S tokens can touch, wherever the first one falls
 int tiles_of(int S, int tile) { return (int)(((long long)S + tile - 1 + tile - 1) / tile); }
 
+// a grid's second dimension, and the threads of its first
+constexpr int MOST_SEQUENCES = 65535;
+bool grid_ok(long long blocks, int waves) { return blocks * waves * 64 < (1ll << 32); }
+
 // tokens are counted in 32 bits, with room for whole blocks behind the last one
 bool room_ok(const Cache& c, int max_pages) { return (long long)max_pages * c.page_size <= (1ll << 30); }
 
+constexpr const char* TOO_MANY = "too many rows for one call";
 constexpr const char* BAD_CACHE = "a 4-bit cache needs four 16-byte aligned tensors, pages of a multiple of 16 tokens";
 constexpr const char* BAD_FORM = "head_dim 64 / 128 / 256 with groups of 32 / 64 / 128 channels (at most head_dim), dtype 0 (bf16) or 1 (fp16)";
 
@@ -607,20 +612,26 @@ TDIST_API int tdist_kv4_append(void* k_codes, void* v_codes, void* k_params, voi
   const Cache c{(uint8_t*)k_codes, (uint8_t*)v_codes, (uint32_t*)k_params, (uint32_t*)v_params, pages, kv_heads, page_size};
   TDIST_REQUIRE(cache_ok(c), BAD_CACHE);
   TDIST_REQUIRE(dtype == 0 || dtype == 1, BAD_FORM);
-  TDIST_REQUIRE(batch >= 0 && batch <= 65535 && S >= 0 && max_pages >= 0 && room_ok(c, max_pages) && (long long)S * kv_heads < (1ll << 31),
+  TDIST_REQUIRE(batch >= 0 && S >= 0 && max_pages >= 0 && room_ok(c, max_pages) && (long long)S * kv_heads < (1ll << 31),
                 "bad batch / token count");
   if (batch == 0 || S == 0) return 0;
   TDIST_REQUIRE(k && v && kv_offset && (table || max_pages == 0), "null argument");
   TDIST_REQUIRE((((uintptr_t)k | (uintptr_t)v) & 15) == 0 && ((k_sb | k_ss | k_sh | v_sb | v_ss | v_sh) & 7) == 0,
                 "k / v rows must keep 16-byte alignment");
+  bool fits = true;
   const bool ok = dispatch(dtype, head_dim, group, [&](auto bf, auto d, auto g) {
     const int tiles = tiles_of(S, Tile<decltype(d)::value>::TILE), waves = std::min(tiles, 4);
-    hipLaunchKernelGGL((kv4_append_kernel<decltype(bf)::value, decltype(d)::value, decltype(g)::value>),
-                       dim3((tiles + waves - 1) / waves * 2 * kv_heads, batch), dim3(64 * waves), 0, (hipStream_t)stream, c,
-                       (const uint16_t*)k, (const uint16_t*)v, k_sb, k_ss, k_sh, v_sb, v_ss, v_sh, kv_offset, new_lens, table,
-                       table_stride, max_pages, S);
+    const int blocks = (tiles + waves - 1) / waves * 2 * kv_heads;
+    fits = grid_ok(blocks, waves);
+    for (long long b = 0; fits && b < batch; b += MOST_SEQUENCES)
+      hipLaunchKernelGGL((kv4_append_kernel<decltype(bf)::value, decltype(d)::value, decltype(g)::value>),
+                         dim3(blocks, (unsigned)std::min<long long>(MOST_SEQUENCES, batch - b)),
+                         dim3(64 * waves), 0, (hipStream_t)stream, c, (const uint16_t*)k + b * k_sb, (const uint16_t*)v + b * v_sb, k_sb,
+                         k_ss, k_sh, v_sb, v_ss, v_sh, kv_offset + b, new_lens ? new_lens + b : nullptr, table + b * table_stride,
+                         table_stride, max_pages, S);
   });
   TDIST_REQUIRE(ok, BAD_FORM);
+  TDIST_REQUIRE(fits, TOO_MANY);
   TDIST_HIP_TRY(hipGetLastError());
   return 0;
 }
@@ -633,26 +644,32 @@ TDIST_API int tdist_kv4_qkv_prep(void* k_codes, void* v_codes, void* k_params, v
                                  int batch, int S, int q_heads, void* stream) {
   const Cache c{(uint8_t*)k_codes, (uint8_t*)v_codes, (uint32_t*)k_params, (uint32_t*)v_params, pages, kv_heads, page_size};
   TDIST_REQUIRE(cache_ok(c), BAD_CACHE);
-  TDIST_REQUIRE(batch >= 0 && batch <= 65535 && S >= 0 && max_pages >= 0 && room_ok(c, max_pages) && q_heads > 0 && q_heads <= 32767 && rope_rows > 0 &&
+  TDIST_REQUIRE(batch >= 0 && S >= 0 && max_pages >= 0 && room_ok(c, max_pages) && q_heads > 0 && q_heads <= 32767 && rope_rows > 0 &&
                     (long long)S * (q_heads + 2 * kv_heads) < (1ll << 31),
                 "bad batch / token / head count");
   if (batch == 0 || S == 0) return 0;
   TDIST_REQUIRE(qkv && positions && cos_t && sin_t && q_out && kv_offset && total_out && (table || max_pages == 0), "null argument");
   TDIST_REQUIRE((((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)q_w | (uintptr_t)k_w) & 15) == 0 && ((q_sb | q_ss) & 7) == 0,
                 "qkv rows, norm weights and q must keep 16-byte alignment");
+  bool fits = true;
   const bool ok = dispatch(0, head_dim, group, [&](auto bf, auto d, auto g) {
     if constexpr (decltype(bf)::value) {
       const int tiles = tiles_of(S, PrepTile<decltype(d)::value>::TILE), waves = std::min(tiles, 4), heads = q_heads + 2 * kv_heads;
       // heads that share a fetch of the rotation's factors, where there is work for the chip without that
       const int each = (int)std::max(1ll, std::min(8ll, (long long)tiles * heads * batch / 6144));
-      hipLaunchKernelGGL((kv4_qkv_prep_kernel<decltype(d)::value, decltype(g)::value>),
-                         dim3((tiles + waves - 1) / waves * ((heads + each - 1) / each), batch), dim3(64 * waves), 0,
-                         (hipStream_t)stream, c, (const uint16_t*)qkv, q_sb, q_ss, (const uint16_t*)q_w, (const uint16_t*)k_w,
-                         q_eps, k_eps, positions, cos_t, sin_t, rope_rows, (uint16_t*)q_out, kv_offset, total_out, table,
-                         table_stride, max_pages, S, q_heads, each);
+      const int blocks = (tiles + waves - 1) / waves * ((heads + each - 1) / each);
+      fits = grid_ok(blocks, waves);
+      for (long long b = 0; fits && b < batch; b += MOST_SEQUENCES)
+        hipLaunchKernelGGL((kv4_qkv_prep_kernel<decltype(d)::value, decltype(g)::value>),
+                           dim3(blocks, (unsigned)std::min<long long>(MOST_SEQUENCES, batch - b)),
+                           dim3(64 * waves), 0, (hipStream_t)stream, c, (const uint16_t*)qkv + b * q_sb, q_sb, q_ss, (const uint16_t*)q_w,
+                           (const uint16_t*)k_w, q_eps, k_eps, positions + b * S, cos_t, sin_t, rope_rows,
+                           (uint16_t*)q_out + b * S * q_heads * head_dim, kv_offset + b, total_out + b, table + b * table_stride,
+                           table_stride, max_pages, S, q_heads, each);
     }
   });
   TDIST_REQUIRE(ok, BAD_FORM);
+  TDIST_REQUIRE(fits, TOO_MANY);
   TDIST_HIP_TRY(hipGetLastError());
   return 0;
 }
@@ -670,19 +687,23 @@ TDIST_API int tdist_kv4_read(const void* k_codes, const void* v_codes, const voi
   TDIST_REQUIRE((table || max_pages == 0) && cu && k_out && v_out, "null argument");
   TDIST_REQUIRE((((uintptr_t)k_out | (uintptr_t)v_out) & 15) == 0 && ((k_st | k_sh | v_st | v_sh) & 7) == 0,
                 "output rows must keep 16-byte alignment");
-  TDIST_REQUIRE(total * kv_heads < (1ll << 31), "too many rows for one call");
+  TDIST_REQUIRE(total * kv_heads < (1ll << 31), TOO_MANY);
+  bool fits = true;
   const bool ok = dispatch(dtype, head_dim, group, [&](auto bf, auto d, auto g) {
     // short sequences: as few of them in a wave as there can be
     using T = Tile<decltype(d)::value>;
     const int rows_each = total <= 4ll * batch ? T::ROWS : T::TILE;
     const long long tiles = (total + rows_each - 1) / rows_each;
     const int waves = (int)std::min(tiles, 4ll);
+    fits = grid_ok((tiles + waves - 1) / waves * 2 * kv_heads, waves);
+    if (!fits) return;
     hipLaunchKernelGGL((kv4_read_kernel<decltype(bf)::value, decltype(d)::value, decltype(g)::value>),
                        dim3((unsigned)((tiles + waves - 1) / waves * 2 * kv_heads)), dim3(64 * waves), 0, (hipStream_t)stream, c,
                        table, table_stride, max_pages, cu, starts, batch, total, rows_each, (uint16_t*)k_out, (uint16_t*)v_out, k_st, k_sh,
                        v_st, v_sh);
   });
   TDIST_REQUIRE(ok, BAD_FORM);
+  TDIST_REQUIRE(fits, TOO_MANY);
   TDIST_HIP_TRY(hipGetLastError());
   return 0;
 }
