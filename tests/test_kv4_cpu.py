@@ -495,3 +495,14 @@ def test_inputs_that_carry_a_tangent_or_require_a_gradient_are_refused():
     cache = kv4.Int4KVCache.alloc(1, 16, 1, 64)
     with pytest.raises(ValueError, match="gradient"):
         kv4.Int4KVCache(cache.k_codes, cache.v_codes, cache.k_params.clone().requires_grad_(), cache.v_params)
+
+
+def test_results_that_share_memory_are_refused():
+    cache, table, cu = kv4.Int4KVCache.alloc(4, 16, 2, 64, group=32), int32([[0, 1], [2, 3]]), int32([0, 3, 5])
+    x = torch.zeros(5, 4, 64, dtype=torch.bfloat16)
+    k, v = kv4.kv4_read(cache, table, cu, 5, out=(x[:, :2], x[:, 2:]))     # parts of the same rows
+    assert k.data_ptr() == x.data_ptr() and v.data_ptr() == x[:, 2:].data_ptr()
+    own = torch.zeros(5, 2, 64, dtype=torch.bfloat16)
+    for out in ((x[:, :2], x[:, :2]), (x[:1, :2].expand(5, 2, 64), own), (own, x[:, :1].expand(5, 2, 64))):
+        with pytest.raises(ValueError, match="memory"):
+            kv4.kv4_read(cache, table, cu, 5, out=out)

@@ -388,6 +388,8 @@ def kv4_read(cache: Int4KVCache, block_table: torch.Tensor, cu_seqlens: torch.Te
             _require(tuple(t.shape) == shape, f"out must be two tensors {shape}, got {tuple(t.shape)}")
             _require(t.stride(2) == 1 and t.stride(0) % 8 == 0 and t.stride(1) % 8 == 0 and t.data_ptr() % 16 == 0,
                      "rows of out must be contiguous and 16-byte aligned")
+            _require(all(n < 2 or s > 0 for n, s in zip(shape, t.stride())), "every row of out needs memory of its own")
+        _require(total == 0 or k.data_ptr() != v.data_ptr(), "K and V of out must not share memory")
     if batch == 0 or total == 0:
         return k, v
     if not cache.k_codes.is_cuda:
