@@ -305,7 +305,6 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_kernel(AttnArgs a, const int*
   };
 #pragma unroll
   for (int g = 0; g < NG; ++g) vs[g] = 1.f;
-  bool scaled = false;
   const Unpack u;
   u32x4 neg0, neg1;                     // -1024 and -64
 #pragma unroll
@@ -350,8 +349,8 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_kernel(AttnArgs a, const int*
   // after that.  false: they are far from 1, and the block is not treated as one that needs care.
   auto rescale = [&](auto careful, const uint32_t (&param)[NG], float (&ratio)[NG], float& widest) INLINE -> bool {
     constexpr bool CAREFUL = decltype(careful)::value;
-    bool off = false;
     if (!CAREFUL) {
+      bool off = false;
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
         const float w = max_upper_half(fmaxf(0.f, scale_of<IS_BF16>(param[g])));
@@ -372,10 +371,8 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_kernel(AttnArgs a, const int*
         ratio[g] = __builtin_bit_cast(float, (uint32_t)(127 - e) << 23);
         vs[g] *= ratio[g];
       }
-      off |= vs[g] != 1.f;
       widest = fmaxf(widest, w * ratio[g]);
     }
-    scaled |= off;
     return true;
   };
   // O^T += V^T . P^T for the channels of group g
