@@ -10,9 +10,10 @@
 // Measured, 8 KV heads of 128: append of 8 ragged prompts of up to 4001 tokens (groups of 128, 89 MB in and out) 25 us, 3.5 TB/s,
 // where the simple form (a lane group per row, V written unit by unit) took 40; read of 16 ragged sequences of up to 8192
 // (groups of 64, 351 MB) 79 .. 82 us, 4.3 TB/s of a copy's 4.9, simple form 199; projection epilogue of 2 x 1500 tokens, 64 query
-// heads, groups of 32 (about 115 MB) 33 us, 3.5 TB/s, simple form 65.  Append and projection are held by the ten or so vector
-// operations a channel that exact codes take, next to their bytes; one token of a sequence (6 us for write and read, 7.5 with
-// the projection) by the launches.
+// heads, groups of 32 (about 115 MB) 33 us, 3.5 TB/s, simple form 65.  Append is held by the ten or so vector operations a channel
+// that exact codes take, next to its bytes.  What the projection's epilogue waits for, 33 us where its bytes take 23.5, is not known: of
+// its 80 heads here 64 are Q's, without codes and in 32 bits.  One token of a sequence (6 us for write and read, 7.5 with the
+// projection) is held by the launches.
 // This file is compiled without fast-math: the code of a value next to a border is decided by IEEE arithmetic and is
 // the same on every path that writes a cache, the CPU's included.
 #include <algorithm>

@@ -19,11 +19,20 @@
 // the largest is 2^6: the cross-lane maximum leaves the loop, and a weight keeps all its bits down to 2^-20 of the largest
 // (2^-8 in a group of 2^-12 of the widest scale; groups further apart, or far from 1, get a power of two each).
 //
-// What bounds it: many sequences, the bytes of the cache (64 x 4096 tokens, 8 heads of 128: 286 MB in 58 us, 4.9 TB/s, a copy's
-// rate on the same card); one long sequence of 131072, those and the two launches' start and end (151 MB in 35 .. 37 us,
-// 4.1 .. 4.3 TB/s); a few tokens, the launches (6.5 us); many columns, the vector instructions of unpacking and softmax (1024
-// new tokens over 16384, 266 GFLOP: 511 us, 520 TFLOP/s; kv4_chunk.hip takes 312 and gets such calls).  bf16 high and low parts
-// of 16 + code, what this began with, took 103 us for the first of these.
+// What bounds it (calls in a row; from a graph over three caches in turn 58 .. 59 and 36 .. 38 us for the first two): many
+// sequences, the bytes of the cache (64 x 4096 tokens, 8 heads of 128: 286 MB in 55 us, 5.2 TB/s, where a copy reaches 4.9 and reading
+// alone 5.3 .. 5.6); one long sequence of 131072, those and the two launches' start and end (151 MB in 35 us, 4.3 TB/s); a few
+// tokens, the launches (6.5 us); many columns, the vector instructions of unpacking and softmax (1024 new tokens over 16384, 266
+// GFLOP: 511 .. 560 us, 520 TFLOP/s at best, and 740 in fp16; kv4_chunk.hip takes 295 for bf16 and gets such calls, but for capped
+// ones: 915).  bf16 high and low parts of 16 + code, what this began with, took 103 us for the first of these.
+//
+// What is held in fewer bits than a sum in fp32, and shows: P * scale as one fp16 number over bf16 caches, which puts errors against 64
+// bits 2 to 4 % above those of 32-bit arithmetic rounded once.  P is 2^34 at most, so that |low| up to 2^94 keeps its sums finite.
+//
+// Registers.  Spilled ones, of 256 (scratch, bytes a lane): heads of 256 in groups of 32 103 .. 156 (364 .. 512), in groups of 64
+// 1 .. 37 (8 .. 136), heads of 128 in groups of 32 with two column blocks 41 .. 48 (152 .. 180), others none.  16 x 4096 tokens, 4 heads of 256:
+// 42.7 us in groups of 32 where groups of 64 take 22.9 and of 128 20.2; 5 new tokens over 16 x 4096, 8 heads of 128: 41.7 and 30.0 us
+// in groups of 32 and 64.
 #include <algorithm>
 
 #include "tdist/kv4.hpp"
@@ -52,8 +61,9 @@ struct AttnArgs {
 typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 
-// Blocks a wave has in flight.  Three where the registers hold them (131072 tokens: 37.5 us); one where two column blocks or
-// heads of 256 channels need the registers (chunk of 1024 511 us against 531 with two, heads of 256 50.3 against 53.9).
+// Blocks a wave has in flight.  Three where the registers hold them (131072 tokens: 37.5 us); one with two column blocks or heads of
+// 256 channels, whose sums leave less room (chunk of 1024 511 us against 531 with two, heads of 256 50.3 against 53.9) - and not
+// enough: see above for what is spilled even so.
 constexpr int ring_of(int D, int CB) { return CB == 2 || D == 256 ? 1 : 3; }
 
 #define INLINE __attribute__((always_inline))     // (lambdas: a call would put what they capture into memory)

@@ -12,9 +12,9 @@
 //
 // For bf16 caches: values rounded to fp16 are within 2^-11 of themselves (but for small ones, see below) and a weight within 2^-11,
 // where the result is rounded to 2^-8; 1024 tokens over 16384 are 1.9e-3 off at most with it and with the plain form in 32 bits
-// (relative to a row's norm).  A fp16 result has steps of 2^-11 itself, and these roundings would be most of its error: 5.8e-4
-// for 2.7e-4, three times the scores 1.6e-3 for 2.4e-4, where kv4_attn.hip comes to 2.8e-4 and 2.5e-4.  So fp16 caches stay there, which costs
-// them 740 us where this kernel took 351.
+// (relative to a row's norm), at three times the scores, in groups of 32, 2.5e-3 for 2.0e-3.  A fp16 result has steps of 2^-11
+// itself, and these roundings would be most of its error: 5.8e-4 for 2.7e-4, three times the scores 1.6e-3 for 2.4e-4, where
+// kv4_attn.hip comes to 2.8e-4 and 2.5e-4.  So fp16 caches stay there, which costs them 740 us where this kernel took 351.
 //
 // fp16 does not reach as far as bf16.  Below 2^-14 its numbers are 2^-24 apart, and a value is then off by as much as 17 * 2^-25:
 // a code's 15 times what the scale lost, what low lost, and the result's own rounding.  Whose group is how large against that
@@ -28,8 +28,9 @@
 // `flags` has one int per workgroup, written by every launch; kv4_attn.hip runs behind this kernel and takes just the flagged
 // workgroups' columns.
 //
-// What bounds it: 1024 new tokens over 16384, 32 / 8 heads of 128 (266 GFLOP): 301 .. 312 us in all, 850 .. 880 TFLOP/s where a
-// large bf16 matrix product reaches 1203; the other kernel takes 511.  Of a SIMD's cycles its matrix unit has 37 %, vector
+// What bounds it: 1024 new tokens over 16384, 32 / 8 heads of 128 (266 GFLOP): 294 .. 307 us in all, 870 .. 905 TFLOP/s where a
+// large bf16 matrix product reaches 1203; the other kernel takes 511.  (A dozen calls in a row: the same call after a pause, or with
+// a wait for each, takes 350 .. 390 us until the card is busy again.)  Of a SIMD's cycles its matrix unit has 37 %, vector
 // instructions 48 %, and two waves hardly overlap the two.  Timing-only builds of 349 us (launches apart from each other): 279
 // without the unpacking, 294 without V's way back from LDS, 311 with half of the second product, 334 without the exponentials.
 // Eight waves with one set of buffers against twice four: 346 and 367 us (with half the columns for a workgroup, unpacking costs

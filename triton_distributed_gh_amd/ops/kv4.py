@@ -3,8 +3,8 @@
 A cached row (one token, one KV head) is cut into groups of ``group`` channels.  A group keeps its smallest value ``low``
 and ``scale`` = (max - low) / 15, both rounded to the cache's 16-bit type, and 4 bits per channel:
 ``code = round((x - low) / scale)`` in fp32, ties to even, 0 where ``scale`` is 0; it stands for ``scale * code + low``.  A
-group with an infinity or a NaN in it reads back as NaN.  At head_dim 128 a token of one KV head takes 136 / 144 / 160
-bytes (groups of 128 / 64 / 32 channels) where 16-bit K and V take 512.
+group with an infinity or a NaN in it, or with a range beyond fp32's, reads back as NaN.  At head_dim 128 a token of one KV
+head takes 136 / 144 / 160 bytes (groups of 128 / 64 / 32 channels) where 16-bit K and V take 512.
 
 ====================================  ====================================================================================
 ``Int4KVCache``                       pages of one layer; sequences own pages through a ``block_table [batch, max_pages]``
@@ -15,7 +15,7 @@ bytes (groups of 128 / 64 / 32 channels) where 16-bit K and V take 512.
 ``flash_attn_with_kv4cache``          the same under the argument list of ``flash_attn_with_kvcache``
 ====================================  ====================================================================================
 
-GPU tensors run csrc/ops/kv4.hip and csrc/ops/kv4_attn.hip, CPU tensors a PyTorch path over the same packed layout: codes and
+GPU tensors run csrc/ops/kv4.hip, kv4_attn.hip and kv4_chunk.hip, CPU tensors a PyTorch path over the same packed layout: codes and
 parameters that either writes are the same bits.  Entries of a block table that are no page of the cache are tolerated
 everywhere: rows that would go there are dropped, tokens there read as zeros and are not attended.  Everything launches
 on the current stream of the tensors' device, allocates nothing that outlives the call but its results, and can be
@@ -303,7 +303,9 @@ def kv4_qkv_prep(qkv: torch.Tensor, q_w: Optional[torch.Tensor], k_w: Optional[t
     ``qkv [batch, S, (Hq + 2 Hkv) * D]`` bf16: q / k heads get their optional per-head RMSNorm (``q_w`` / ``k_w`` [D]) and the
     neox rotation at ``position_ids [batch, S]`` (``cos`` / ``sin`` fp32 [positions, D / 2]; ids outside the tables take their
     first or last row), K and V become tokens ``kv_offset[b] + s`` of the cache and ``total_out[b]`` (int32) receives
-    ``kv_offset[b] + S``.  The norm's mean square and the rotation are taken in fp64.  Returns q [batch, S, Hq, D]."""
+    ``kv_offset[b] + S``.  K's mean square and rotation are taken in fp64, so that a code does not depend on the order of a sum;
+    Q's in fp32 on the GPU and in fp64 on the CPU, where a rounding to bf16 may fall the other way (a few in 10^5).  Returns q
+    [batch, S, Hq, D]."""
     D, Hkv = cache.head_dim, cache.kv_heads
     if cache.dtype != torch.bfloat16:
         raise TypeError(f"kv4_qkv_prep writes bf16 caches, got {cache.dtype}")
@@ -443,9 +445,11 @@ def attend_reference(q, cache: Int4KVCache, kv_lens, block_table, scale, soft_ca
 
 def takes_chunks(batch: int, kv_heads: int, columns: int, head_dim: int, capacity: int, soft_cap: float = 0.0) -> bool:
     """Whether a launch over a bf16 cache goes to csrc/ops/kv4_chunk.hip, which unpacks for many columns at once, and only what that
-    leaves to csrc/ops/kv4_attn.hip.  (fp16 caches stay with the latter: their results show the former's roundings.)  Measured (four query heads to a KV head, microseconds there / here): one sequence of 16384, 8 heads of
-    128: 128 columns 40 / 34, 256 46 / 50, 1024 98 / 147; of 4096: 512 columns 43 / 35, 1024 49 / 51, 2048 66 / 78; of 1024: 2048
-    columns 39 / 27; 4 x 2048: 256 columns 38 / 36, 1024 65 / 84; 4 heads of 256: 2048: 512 columns 30 / 29, 1024 36 / 40."""
+    leaves to csrc/ops/kv4_attn.hip.  (fp16 caches stay with the latter: their results show the former's roundings.)
+
+    Measured (four query heads to a KV head, microseconds there / here): one sequence of 16384, 8 heads of 128: 128 columns 40 / 34,
+    256 46 / 50, 1024 98 / 147; of 4096: 512 columns 43 / 35, 1024 49 / 51, 2048 66 / 78; of 1024: 2048 columns 39 / 27; 4 x 2048:
+    256 columns 38 / 36, 1024 65 / 84; 4 heads of 256: 2048: 512 columns 30 / 29, 1024 36 / 40."""
     work = batch * kv_heads * columns * capacity
     return soft_cap == 0 and 2 * columns > CHUNK_COLUMNS[head_dim] and work >= CHUNK_WORK[head_dim]
 
@@ -459,6 +463,8 @@ def auto_kv_splits(batch: int, kv_heads: int, columns: int, head_dim: int, capac
     splits; 16 x 4096 23.1 / 20.3 / 24.7 with 2 / 4 / 8; 64 x 4096 55.9 / 61.9 with 1 / 2.  At least 128 tokens each: 2048 tokens 9.5 /
     8.9 with 8 / 16; beyond sixteen splits 256: 8192 tokens 10.3 / 11.0 with 32 / 64.  Up to 512 tokens in one piece: 256 tokens
     6.8 / 8.3 with 1 / 2, 512 8.5 / 8.6 with 1 / 4 (640: 9.3 / 8.6 with 1 / 6), and one launch instead of two on the host, 11 / 15.
+    (Measured for a decode step; not for more columns or other heads.)  The room decides and not the lengths, which the host does
+    not know: 37 tokens take 6.6 us in a table of 37 and 9.3 in one of 32768, 512 8.7 and 9.0, 16 x 512 9.1 and 10.9.
 
     ``chunk``: of a launch that `takes_chunks`; one workgroup fills a CU there (1024 new tokens over 16384: 613 / 356 / 443 with 1 /
     2 / 3; 256 over 16384 126 / 106 / 128 with 6 / 8 / 16)."""
@@ -476,8 +482,8 @@ def gqa_fwd_kv4(q: torch.Tensor, cache: Int4KVCache, kv_lens: torch.Tensor, bloc
                 return_lse: bool = False) -> torch.Tensor:
     """Attention of ``q [batch, S, Hq, D]`` (or ``[batch, Hq, D]`` for S = 1), the last S tokens of each sequence.
 
-    ``kv_lens`` int32 [batch]: cached tokens, the S new ones included; with ``causal`` query s sees the first
-    ``kv_lens[b] - S + s + 1`` of them.  Rows that see nothing are zero.  Scores (``scale`` times q . k) may be up to 2^27 in size: in
+    ``kv_lens`` int32 [batch]: cached tokens, the S new ones included (more than the table has room for count as that room); with
+    ``causal`` query s sees the first ``kv_lens[b] - S + s + 1`` of them.  Rows that see nothing are zero.  Scores (``scale`` times q . k) may be up to 2^27 in size: in
     fp32 they are 8 apart from there on, and a row's weights mean nothing.  Returns q's shape in q's type, or with ``return_lse``
     fp32 ``[.., D + 1]`` with the natural-log LSE last (-inf for an empty row), the form
     ``flash_decode.gqa_fwd_batch_decode_inter_rank_combine`` merges over ranks that hold parts of the sequences."""
